@@ -580,6 +580,76 @@ int check_norm_rope_alignment(int dtype, const void* q, const void* k, const voi
   return HYT_OK;
 }
 
+// ------------------------------------------------------------------ chunk attention, moves, selection
+constexpr int kSms = 148;  // work is shared out over this many SMs (fewer would only queue CTAs)
+
+int check_scale(float scale) {
+  if (!(scale > 0.f) || !(scale < 3.0e38f)) return fail(HYT_ERR_INVALID, "scale must be positive and finite");
+  return HYT_OK;
+}
+
+// Pool rows that 16-byte loads can read, and pages that no 64-key tile crosses.
+int check_chunk_geometry(const Geometry& g, const void* k_pool, const void* v_pool) {
+  if (g.head_dim % 8 || g.head_dim > 256)
+    return fail(HYT_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 and at most 256");
+  if (g.page_size < 64) return fail(HYT_ERR_UNSUPPORTED, "page_size must be at least 64 tokens");
+  if (reinterpret_cast<uintptr_t>(k_pool) % 16 || reinterpret_cast<uintptr_t>(v_pool) % 16)
+    return fail(HYT_ERR_INVALID, "KV pools must be 16-byte aligned");
+  return HYT_OK;
+}
+
+int64_t chunk_max_rows(int32_t num_q_heads, int32_t num_kv_heads, int32_t query_len) {
+  return int64_t(num_q_heads / num_kv_heads) * query_len;
+}
+
+size_t chunk_workspace(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t query_len,
+                       int32_t dtype) {
+  const int64_t rows = chunk_max_rows(num_q_heads, num_kv_heads, query_len);
+  return align256(size_t(hyt::chunk_workspace_bytes(hyt::chunk_shape_general(rows, dtype, head_dim, kSms), head_dim)));
+}
+
+int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t workspace_bytes,
+                 cudaStream_t stream) {
+  const size_t need = chunk_workspace(g.num_q_heads, g.num_kv_heads, g.head_dim, g.query_len, g.dtype);
+  if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(HYT_ERR_WORKSPACE, "workspace missing, not 16-byte aligned or too small");
+  c.group = g.num_q_heads / g.num_kv_heads;
+  const int64_t rows = chunk_max_rows(g.num_q_heads, g.num_kv_heads, g.query_len);
+  const hyt::ChunkShape s = hyt::chunk_shape_general(rows, g.dtype, g.head_dim, kSms);
+  c.unit_rows = s.unit_rows;
+  c.tile_keys = s.tile_keys;
+  c.ctas = s.ctas;
+  c.ws_o = static_cast<float*>(workspace);
+  c.ws_ml = c.ws_o + int64_t(s.ctas) * 2 * s.unit_rows * g.head_dim;
+  cudaError_t err = hyt::run_chunk_attention_general(c, g.dtype, stream);
+  if (err != cudaSuccess) return cuda_fail(err, "chunk attention launch");
+  err = hyt::run_chunk_merge(c, g.dtype, stream);
+  if (err != cudaSuccess) return cuda_fail(err, "chunk attention merge launch");
+  return HYT_OK;
+}
+
+// Pools, page ids and the alignment-free part of a move's arguments.
+int move_params(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_heads, int64_t capacity,
+                int32_t head_dim, int32_t page_size, int32_t dtype, int32_t* error_word, hyt::MoveParams* p) {
+  if (!k_pool || !v_pool) return fail(HYT_ERR_INVALID, "null pointer argument");
+  Geometry g{num_layers, 0, capacity, 1, 1, 1, num_kv_heads, num_kv_heads, head_dim, page_size, dtype};
+  const int rc = check_geometry(g);
+  if (rc != HYT_OK) return rc;
+  if (int64_t(num_layers) * num_kv_heads > INT32_MAX / 4)
+    return fail(HYT_ERR_UNSUPPORTED, "too many layers times KV heads");
+  *p = hyt::MoveParams{};
+  p->k_pool = static_cast<uint8_t*>(k_pool);
+  p->v_pool = static_cast<uint8_t*>(v_pool);
+  p->row_bytes = int64_t(head_dim) * elem_bytes(dtype);
+  p->capacity = capacity;
+  p->planes = num_layers * num_kv_heads;
+  p->page_shift = log2_int(page_size);
+  p->num_pages = int32_t(capacity / page_size);
+  p->error_word = error_word;
+  if ((p->row_bytes << p->page_shift) > INT32_MAX) return fail(HYT_ERR_UNSUPPORTED, "page too large");
+  return HYT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1249,6 +1319,221 @@ int hyt_read_probe(const void* src, size_t bytes, uint32_t* sink, int32_t ctas, 
   cudaError_t err = hyt::run_read_probe(src, bytes, sink, ctas, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "read probe launch");
   return HYT_OK;
+}
+
+size_t hyt_tree_workspace_bytes(int32_t max_query_len, int32_t num_q_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t dtype) {
+  if (max_query_len < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1) return 0;
+  return chunk_workspace(num_q_heads, num_kv_heads, head_dim, max_query_len, dtype);
+}
+
+int hyt_tree_attention(const void* q, const int64_t* q_strides, const void* k_pool,
+                       const void* v_pool, int32_t num_layers, int32_t layer,
+                       int64_t capacity_tokens, const int32_t* page_table,
+                       int32_t page_table_stride, int32_t page_table_width,
+                       const int32_t* cache_lens, const int32_t* q_start, const int32_t* q_len,
+                       const int32_t* tree_mask, int32_t mask_words, void* out,
+                       const int64_t* out_strides, int32_t batch, int32_t total_tokens,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t page_size, int32_t dtype, float scale, int32_t max_query_len,
+                       void* workspace, size_t workspace_bytes, int32_t* error_word,
+                       void* stream) {
+  g_last_error.clear();
+  int rc = check_attention_pointers(q, q_strides, k_pool, v_pool, page_table, cache_lens, out,
+                                    out_strides);
+  if (rc != HYT_OK) return rc;
+  if (!q_start || !q_len) return fail(HYT_ERR_INVALID, "null pointer argument");
+  Geometry g{num_layers, layer, capacity_tokens, page_table_stride, batch, max_query_len,
+             num_q_heads, num_kv_heads, head_dim, page_size, dtype};
+  rc = check_geometry(g);
+  if (rc != HYT_OK) return rc;
+  rc = check_chunk_geometry(g, k_pool, v_pool);
+  if (rc != HYT_OK) return rc;
+  rc = check_scale(scale);
+  if (rc != HYT_OK) return rc;
+  if (total_tokens < 1) return fail(HYT_ERR_INVALID, "total_tokens must be positive");
+  if (page_table_width < 1 || (batch > 1 && page_table_width > page_table_stride))
+    return fail(HYT_ERR_INVALID, "page_table_width must be positive and at most the row stride");
+  if (tree_mask != nullptr && int64_t(mask_words) * 32 < max_query_len)
+    return fail(HYT_ERR_INVALID, "tree_mask rows hold fewer bits than max_query_len");
+  const int64_t qs[3] = {0, q_strides[1], q_strides[0]}, os[3] = {0, out_strides[1], out_strides[0]};
+  hyt::ChunkParams c{};
+  c.a = attention_params(q, qs, k_pool, v_pool, g, page_table, cache_lens, out, os, scale, error_word);
+  c.a.q_start = q_start;
+  c.a.q_len = q_len;
+  c.a.total_tokens = total_tokens;
+  c.table_width = page_table_width;
+  c.mask = tree_mask;
+  c.mask_words = mask_words;
+  return launch_chunk(c, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int hyt_copy_pages(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_heads,
+                   int64_t capacity_tokens, int32_t head_dim, int32_t page_size, int32_t dtype,
+                   const int32_t* src_pages, const int32_t* dst_pages, int32_t count,
+                   int32_t* error_word, void* stream) {
+  g_last_error.clear();
+  hyt::MoveParams p;
+  int rc = move_params(k_pool, v_pool, num_layers, num_kv_heads, capacity_tokens, head_dim, page_size,
+                       dtype, error_word, &p);
+  if (rc != HYT_OK) return rc;
+  if (count < 0) return fail(HYT_ERR_INVALID, "count must not be negative");
+  if (count == 0) return HYT_OK;
+  if (!src_pages || !dst_pages) return fail(HYT_ERR_INVALID, "null pointer argument");
+  if (count > 65535) return fail(HYT_ERR_UNSUPPORTED, "at most 65535 pages per call");
+  p.src = src_pages;
+  p.dst = dst_pages;
+  p.count = count;
+  cudaError_t err = hyt::run_copy_pages(p, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "page copy launch");
+  return HYT_OK;
+}
+
+int hyt_compact_rows(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_heads,
+                     int64_t capacity_tokens, int32_t head_dim, int32_t page_size, int32_t dtype,
+                     const int32_t* page_table, int32_t page_table_stride,
+                     int32_t page_table_width, const int32_t* base, const int32_t* src_rows,
+                     const int32_t* src_start, int32_t batch, int32_t total_rows,
+                     int32_t* error_word, void* stream) {
+  g_last_error.clear();
+  hyt::MoveParams p;
+  int rc = move_params(k_pool, v_pool, num_layers, num_kv_heads, capacity_tokens, head_dim, page_size,
+                       dtype, error_word, &p);
+  if (rc != HYT_OK) return rc;
+  if (batch < 1) return fail(HYT_ERR_INVALID, "batch must be positive");
+  if (total_rows < 0) return fail(HYT_ERR_INVALID, "total_rows must not be negative");
+  if (total_rows == 0) return HYT_OK;
+  if (!page_table || !base || !src_rows || !src_start) return fail(HYT_ERR_INVALID, "null pointer argument");
+  if (page_table_width < 1 || (batch > 1 && page_table_width > page_table_stride))
+    return fail(HYT_ERR_INVALID, "page_table_width must be positive and at most the row stride");
+  if (batch > 65535) return fail(HYT_ERR_UNSUPPORTED, "batch too large");
+  p.page_table = page_table;
+  p.page_table_stride = page_table_stride;
+  p.table_width = page_table_width;
+  p.batch = batch;
+  p.base = base;
+  p.src = src_rows;
+  p.start = src_start;
+  p.count = total_rows;
+  cudaError_t err = hyt::run_compact_rows(p, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "row compaction launch");
+  return HYT_OK;
+}
+
+int hyt_page_bounds(const void* k_pool, void* k_bounds, int32_t num_layers, int32_t first_layer,
+                    int32_t layers, int32_t num_kv_heads, int64_t capacity_tokens,
+                    int32_t head_dim, int32_t page_size, int32_t dtype, const int32_t* pages,
+                    int32_t count, int32_t* error_word, void* stream) {
+  g_last_error.clear();
+  if (!k_pool || !k_bounds) return fail(HYT_ERR_INVALID, "null pointer argument");
+  Geometry g{num_layers, first_layer, capacity_tokens, 1, 1, 1, num_kv_heads, num_kv_heads, head_dim,
+             page_size, dtype};
+  int rc = check_geometry(g);
+  if (rc != HYT_OK) return rc;
+  if (layers < 1 || int64_t(first_layer) + layers > num_layers)
+    return fail(HYT_ERR_INVALID, "layers must be within [0, num_layers)");
+  if (head_dim % 8 || head_dim > 256)
+    return fail(HYT_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 and at most 256");
+  if (reinterpret_cast<uintptr_t>(k_pool) % 16 || reinterpret_cast<uintptr_t>(k_bounds) % 16)
+    return fail(HYT_ERR_INVALID, "the K pool and the bounds must be 16-byte aligned");
+  if (count < 0) return fail(HYT_ERR_INVALID, "count must not be negative");
+  if (count == 0) return HYT_OK;
+  if (!pages) return fail(HYT_ERR_INVALID, "null pointer argument");
+  if (count > 65535 || layers > 65535) return fail(HYT_ERR_UNSUPPORTED, "at most 65535 pages and layers per call");
+  hyt::BoundsParams p;
+  p.k_pool = k_pool;
+  p.k_bounds = k_bounds;
+  p.capacity = capacity_tokens;
+  p.first_layer = first_layer;
+  p.layers = layers;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.page_shift = log2_int(page_size);
+  p.num_pages = int32_t(capacity_tokens / page_size);
+  p.pages = pages;
+  p.count = count;
+  p.error_word = error_word;
+  cudaError_t err = hyt::run_page_bounds(p, dtype, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "page bounds launch");
+  return HYT_OK;
+}
+
+size_t hyt_sparse_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                  int32_t head_dim, int32_t num_pages, int32_t dtype) {
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1 || num_pages < 1) return 0;
+  const size_t ids = align256(size_t(batch) * num_kv_heads * num_pages * 4), lens = align256(size_t(batch) * 4);
+  return ids + lens + chunk_workspace(num_q_heads, num_kv_heads, head_dim, 1, dtype);
+}
+
+int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_pool,
+                         const void* v_pool, const void* k_bounds, int32_t num_layers,
+                         int32_t layer, int64_t capacity_tokens, const int32_t* page_table,
+                         int32_t page_table_stride, int32_t page_table_width,
+                         const int32_t* cache_lens, void* out, const int64_t* out_strides,
+                         int32_t* selected, int32_t batch, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                         int32_t dtype, float scale, int32_t num_pages, void* workspace,
+                         size_t workspace_bytes, int32_t* error_word, void* stream) {
+  g_last_error.clear();
+  int rc = check_attention_pointers(q, q_strides, k_pool, v_pool, page_table, cache_lens, out,
+                                    out_strides);
+  if (rc != HYT_OK) return rc;
+  if (!k_bounds || !selected) return fail(HYT_ERR_INVALID, "null pointer argument");
+  Geometry g{num_layers, layer, capacity_tokens, page_table_stride, batch, 1,
+             num_q_heads, num_kv_heads, head_dim, page_size, dtype};
+  rc = check_geometry(g);
+  if (rc != HYT_OK) return rc;
+  rc = check_chunk_geometry(g, k_pool, v_pool);
+  if (rc != HYT_OK) return rc;
+  rc = check_scale(scale);
+  if (rc != HYT_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(k_bounds) % 16) return fail(HYT_ERR_INVALID, "the bounds must be 16-byte aligned");
+  if (num_pages < 1) return fail(HYT_ERR_INVALID, "num_pages must be positive");
+  if (page_table_width < 1 || (batch > 1 && page_table_width > page_table_stride))
+    return fail(HYT_ERR_INVALID, "page_table_width must be positive and at most the row stride");
+  if (page_table_width > hyt::kSelectMaxPages)
+    return fail(HYT_ERR_UNSUPPORTED, "a request may have at most 16384 pages");
+  if (batch > 65535 || num_kv_heads > 65535) return fail(HYT_ERR_UNSUPPORTED, "batch too large");
+  if (int64_t(num_q_heads / num_kv_heads) * head_dim * 8 > 128 * 1024)
+    return fail(HYT_ERR_UNSUPPORTED, "too many query heads per KV head for page selection");
+  if (int64_t(batch) * num_kv_heads * num_pages > INT32_MAX)
+    return fail(HYT_ERR_UNSUPPORTED, "batch times KV heads times num_pages is too large");
+  const size_t ids = align256(size_t(batch) * num_kv_heads * num_pages * 4), lens = align256(size_t(batch) * 4);
+  const size_t need = hyt_sparse_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_pages, dtype);
+  if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(HYT_ERR_WORKSPACE,
+                "workspace missing, not 16-byte aligned or smaller than hyt_sparse_workspace_bytes()");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  hyt::SelectParams s;
+  s.q = q;
+  s.q_sb = q_strides[0];
+  s.q_sh = q_strides[1];
+  s.k_bounds = k_bounds;
+  s.layer = layer;
+  s.batch = batch;
+  s.num_q_heads = num_q_heads;
+  s.num_kv_heads = num_kv_heads;
+  s.head_dim = head_dim;
+  s.page_shift = log2_int(page_size);
+  s.num_pages = int32_t(capacity_tokens / page_size);
+  s.page_table = page_table;
+  s.page_table_stride = page_table_stride;
+  s.table_width = page_table_width;
+  s.cache_lens = cache_lens;
+  s.take = num_pages;
+  s.selected = selected;
+  s.pages = reinterpret_cast<int32_t*>(ws);
+  s.lens = reinterpret_cast<int32_t*>(ws + ids);
+  s.error_word = error_word;
+  cudaError_t err = hyt::run_select_pages(s, dtype, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "page selection launch");
+  const int64_t qs[3] = {q_strides[0], q_strides[1], 0}, os[3] = {out_strides[0], out_strides[1], 0};
+  hyt::ChunkParams c{};
+  c.a = attention_params(q, qs, k_pool, v_pool, g, s.pages, s.lens, out, os, scale, error_word);
+  c.a.page_table_stride = num_kv_heads * num_pages;
+  c.table_width = num_pages;
+  c.table_head_stride = num_pages;
+  return launch_chunk(c, g, ws + ids + lens, workspace_bytes - ids - lens, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,215 @@
+// How the chunk-attention kernels (tree_attention*.cu) share out their work.
+//
+// A unit is (request b, KV head g, block of `unit_rows` query rows); rows of a request are
+// numbered t * group + hl (query t, local head hl). A unit streams the request's keys in
+// tiles of `tile_keys`. All units' tiles, request after request, form one line of W tiles;
+// CTA c of G takes tiles [c W / G, (c + 1) W / G): every CTA streams the same number of
+// tiles (+- 1) whatever the lengths, and W needs no host copy of the lengths, so a captured
+// launch follows them. A CTA's stretch falls into segments, one per unit it touches. A
+// segment that covers its unit writes the rows; another writes a partial (unnormalised O,
+// running max, sum) to one of the CTA's two slots (slot 0: its first segment, slot 1: its
+// last; those between are whole), and the merge kernel joins a unit's partials in order.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace hyt {
+
+struct ChunkRequest {
+  int len, queries;      // cached tokens, queries of this step
+  int row_blocks, tiles; // units per KV head, key tiles per unit
+  bool refused;          // lengths the page table cannot hold: nothing is visible
+};
+
+// Lengths of request b. One whose rows leave the token axis gets no work (its rows are not
+// known to be its own); one whose length is negative or needs more pages than its table
+// row holds gets one tile in which nothing is visible, so its rows become zeros.
+__device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& P, int b, int& why) {
+  const AttentionParams& p = P.a;
+  ChunkRequest r{0, 0, 0, 0, false};
+  int n = p.query_len;
+  if (p.q_start != nullptr) {
+    const int s = p.q_start[b];
+    n = p.q_len[b];
+    if (n < 0 || n > p.query_len || s < 0 || int64_t(s) + n > p.total_tokens) {
+      why |= HYT_DEVERR_PACKED_RANGE;
+      return r;
+    }
+  }
+  if (n == 0) return r;
+  r.len = p.cache_lens[b];
+  r.queries = n;
+  r.row_blocks = int((int64_t(n) * P.group + P.unit_rows - 1) / P.unit_rows);
+  const int64_t kv = int64_t(r.len) + n;
+  if (r.len < 0 || kv > (int64_t(P.table_width) << p.page_shift) || kv > INT32_MAX - 256) {
+    why |= HYT_DEVERR_TABLE_RANGE;
+    r.refused = true;
+    r.tiles = 1;
+    return r;
+  }
+  r.tiles = int((kv + P.tile_keys - 1) / P.tile_keys);
+  return r;
+}
+
+__device__ __forceinline__ int64_t chunk_work(const ChunkParams& P, const ChunkRequest& r) {
+  return int64_t(P.a.num_kv_heads) * r.row_blocks * r.tiles;
+}
+
+struct ChunkStart {
+  int64_t total;  // W
+  int64_t off;    // first tile of the CTA within request b's tiles
+  int b;
+};
+
+__device__ __forceinline__ int64_t chunk_begin(int64_t total, int c, int ctas) { return total * c / ctas; }
+
+// Where CTA c of `ctas` starts. Called by all kThreads threads; `sums` holds kThreads / 32
+// shared entries. Ends with a barrier.
+template <int kThreads>
+__device__ __forceinline__ void chunk_find_start(const ChunkParams& P, int c, int ctas, int64_t* sums,
+                                                 ChunkStart* start) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (P.a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, P.a.batch), b1 = min(b0 + per, P.a.batch);
+  int why = 0;
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += chunk_work(P, chunk_request(P, b, why));
+  if (why && c == 0) flag_error(P.a.error_word, why);
+  int64_t scan = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan += v;
+  }
+  if (lane == 31) sums[warp] = scan;
+  if (tid == 0) start->b = 0, start->off = 0;
+  __syncthreads();
+  int64_t before = scan - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  const int64_t begin = chunk_begin(total, c, ctas);
+  if (tid == 0) start->total = total;
+  if (begin >= before && begin < before + mine) {  // one thread, if total > 0 and begin < total
+    int64_t off = begin - before;
+    int b = b0;
+    for (; b < b1; ++b) {
+      const int64_t w = chunk_work(P, chunk_request(P, b, why));
+      if (off < w) break;
+      off -= w;
+    }
+    start->b = b;
+    start->off = off;
+  }
+  __syncthreads();
+}
+
+struct ChunkSegment {
+  int b, g, row0;        // request, KV head, first row of the unit
+  int len, queries, kv;  // cached tokens, queries, their sum
+  int k_lo, k_hi;        // key tiles [k_lo, k_hi) of the unit
+  bool whole, first, refused;
+};
+
+// Walks a CTA's segments; every role of the CTA walks the same ones.
+struct ChunkWalk {
+  int64_t left, off;  // tiles left to the CTA; first of them within request b's
+  int64_t work;
+  int b;
+  bool started;
+  ChunkRequest r;
+
+  __device__ __forceinline__ ChunkWalk(const ChunkParams& P, const ChunkStart& s, int c, int ctas) {
+    left = chunk_begin(s.total, c + 1, ctas) - chunk_begin(s.total, c, ctas);
+    off = s.off;
+    b = s.b;
+    started = false;
+    work = 0;
+    if (left > 0) load(P);
+  }
+  __device__ __forceinline__ void load(const ChunkParams& P) {
+    int why = 0;
+    r = chunk_request(P, b, why);
+    work = chunk_work(P, r);
+  }
+  __device__ __forceinline__ bool next(const ChunkParams& P, ChunkSegment& s) {
+    if (left <= 0) return false;
+    while (off >= work) {  // the next request that has work (left > 0: there is one)
+      off -= work;
+      ++b;
+      load(P);
+    }
+    const int64_t unit = off / r.tiles;
+    s.b = b;
+    s.g = int(unit / r.row_blocks);
+    s.row0 = int(unit - int64_t(s.g) * r.row_blocks) * P.unit_rows;
+    s.len = r.len;
+    s.queries = r.queries;
+    s.kv = r.refused ? 0 : r.len + r.queries;
+    s.k_lo = int(off - unit * r.tiles);
+    s.k_hi = int(min(int64_t(r.tiles), s.k_lo + left));
+    s.whole = s.k_lo == 0 && s.k_hi == r.tiles;
+    s.refused = r.refused;
+    s.first = !started;
+    started = true;
+    const int n = s.k_hi - s.k_lo;
+    off += n;
+    left -= n;
+    return true;
+  }
+};
+
+// Element offset of row `row` (t * group + hl) of request b, head group g, in q or out.
+__device__ __forceinline__ int64_t chunk_q_offset(const ChunkParams& P, int b, int g, int row) {
+  const int t = row / P.group, hl = row - t * P.group;
+  return att_q_row(P.a, b, t) + int64_t(g * P.group + hl) * P.a.q_sh;
+}
+__device__ __forceinline__ int64_t chunk_o_offset(const ChunkParams& P, int b, int g, int row) {
+  const int t = row / P.group, hl = row - t * P.group;
+  return att_o_row(P.a, b, t) + int64_t(g * P.group + hl) * P.a.o_sh;
+}
+
+// Page table row that request b's KV head g walks.
+__device__ __forceinline__ const int32_t* chunk_table(const ChunkParams& P, int b, int g) {
+  return P.a.page_table + int64_t(b) * P.a.page_table_stride + int64_t(g) * P.table_head_stride;
+}
+
+// Which of the 64 chunk-local nodes node0 .. node0 + 63 query t of request b sees, as bits
+// (negative nodes are cached tokens: seen by all; nodes from `queries` on exist for nobody).
+// Without a mask the chunk is causal.
+__device__ __forceinline__ uint64_t chunk_visible64(const ChunkParams& P, int b, int t, int queries, int node0) {
+  if (node0 >= queries || node0 <= -64) return node0 <= -64 ? ~0ull : 0ull;
+  const int first = max(node0, 0);
+  uint64_t bits = 0;
+  if (P.mask == nullptr) {
+    const int n = t + 1 - first;  // nodes first .. t
+    bits = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
+  } else {
+    const int64_t row = P.a.q_start != nullptr ? int64_t(P.a.q_start[b]) + t : int64_t(b) * P.a.query_len + t;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.mask) + row * P.mask_words;
+    const int w = first >> 5, sh = first & 31;
+    const uint32_t w0 = w < P.mask_words ? words[w] : 0u;
+    const uint32_t w1 = w + 1 < P.mask_words ? words[w + 1] : 0u;
+    const uint32_t w2 = w + 2 < P.mask_words ? words[w + 2] : 0u;
+    bits = uint64_t(__funnelshift_r(w0, w1, sh)) | (uint64_t(__funnelshift_r(w1, w2, sh)) << 32);
+  }
+  const int n = queries - first;  // >= 1
+  if (n < 64) bits &= (1ull << n) - 1;
+  if (node0 < 0) bits = (bits << -node0) | ((1ull << -node0) - 1);  // -63 .. -1
+  return bits;
+}
+
+// Where a partial of slot `slot` lives: O as [dims / 4][unit_rows] float4 (consecutive rows
+// next to each other), (max in log2 units, sum) per row.
+__device__ __forceinline__ float4* chunk_partial_o(const ChunkParams& P, int64_t slot) {
+  return reinterpret_cast<float4*>(P.ws_o) + slot * (int64_t(P.a.head_dim / 4) * P.unit_rows);
+}
+__device__ __forceinline__ float2* chunk_partial_ml(const ChunkParams& P, int64_t slot) {
+  return reinterpret_cast<float2*>(P.ws_ml) + slot * P.unit_rows;
+}
+
+}  // namespace hyt

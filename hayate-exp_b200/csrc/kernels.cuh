@@ -177,6 +177,86 @@ struct NormRopeParams {
 };
 cudaError_t run_norm_rope_scatter(const NormRopeParams& p, int dtype, cudaStream_t stream);
 
+// ------------------------------------------------------------ chunk attention (trees, chosen pages)
+// Attention of each request's new queries over its cached keys and, as a mask says, over
+// the step's own. `a` is the shared description: packed (a.q_start / a.q_len, q_len 0
+// allowed) or uniform (a.query_len queries each); a.req_ids is not used.
+struct ChunkParams {
+  AttentionParams a;
+  int32_t group;              // query heads per KV head
+  int32_t table_width;        // entries of one page-table row
+  int32_t table_head_stride;  // 0, or entries between two KV heads' rows of one request
+  const int32_t* mask;        // [token rows, mask_words] visibility bits of the chunk's nodes; null: causal
+  int32_t mask_words;
+  int32_t unit_rows, tile_keys;  // work units (chunk_schedule.cuh)
+  int32_t ctas;
+  float* ws_o;   // [ctas, 2 slots, head_dim / 4, unit_rows, 4] f32
+  float* ws_ml;  // [ctas, 2 slots, unit_rows, 2] f32
+};
+// Work-unit shape and CTA count a kernel uses for a problem.
+struct ChunkShape {
+  int32_t unit_rows, tile_keys, ctas;
+};
+constexpr int64_t chunk_workspace_bytes(const ChunkShape& s, int64_t head_dim) {
+  return int64_t(s.ctas) * 2 * s.unit_rows * (head_dim + 2) * 4;
+}
+// Any dtype, head_dim % 8 == 0 and <= 256, pool rows 16-byte aligned.
+ChunkShape chunk_shape_general(int64_t max_rows, int dtype, int head_dim, int num_sms);
+cudaError_t run_chunk_attention_general(const ChunkParams& p, int dtype, cudaStream_t stream);
+// Joins the partials of units that several CTAs of `p` shared.
+cudaError_t run_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t stream);
+
+// ------------------------------------------------------------ page and row moves
+struct MoveParams {
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  int64_t row_bytes, capacity;   // bytes of one token's row of one head; tokens per plane
+  int32_t planes;                // num_layers * num_kv_heads
+  int32_t page_shift, num_pages;
+  int32_t* error_word;
+  // copy_pages: entry m copies page src[m] to page dst[m]
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t count;
+  // compact_rows: request b's row base[b] + src[start[b] + i] moves to base[b] + i
+  const int32_t* page_table;
+  int32_t page_table_stride, table_width, batch;
+  const int32_t* base;
+  const int32_t* start;
+};
+cudaError_t run_copy_pages(const MoveParams& p, cudaStream_t stream);
+cudaError_t run_compact_rows(const MoveParams& p, cudaStream_t stream);
+
+// ------------------------------------------------------------ page bounds and page selection
+struct BoundsParams {
+  const void* k_pool;
+  void* k_bounds;  // [num_layers, H_kv, num_pages, 2 (min, max), head_dim]
+  int64_t capacity;
+  int32_t first_layer, layers;  // layers [first_layer, first_layer + layers)
+  int32_t num_kv_heads, head_dim, page_shift, num_pages;
+  const int32_t* pages;  // ids; -1 entries are skipped
+  int32_t count;
+  int32_t* error_word;
+};
+cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t stream);
+
+struct SelectParams {
+  const void* q;
+  int64_t q_sb, q_sh;
+  const void* k_bounds;
+  int32_t layer, batch, num_q_heads, num_kv_heads, head_dim, page_shift, num_pages;
+  const int32_t* page_table;
+  int32_t page_table_stride, table_width;
+  const int32_t* cache_lens;
+  int32_t take;          // pages per (request, KV head)
+  int32_t* selected;     // [batch, H_kv, take] logical pages, ascending, -1 past the last
+  int32_t* pages;        // [batch, H_kv, take] the same as physical ids
+  int32_t* lens;         // [batch] cached tokens as seen through `pages`
+  int32_t* error_word;
+};
+constexpr int kSelectMaxPages = 16384;  // pages of one request that a selection can rank
+cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stream);
+
 // Runs the bounded mbarrier wait into its time limit (see self_test.cu).
 cudaError_t run_wait_self_test(int32_t* error_word, int64_t* elapsed_ns, cudaStream_t stream);
 cudaError_t run_read_probe(const void* src, size_t bytes, uint32_t* sink, int ctas, cudaStream_t stream);

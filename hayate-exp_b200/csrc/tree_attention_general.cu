@@ -1,0 +1,411 @@
+// Chunk attention on CUDA cores (fp32 pools, head sizes the tensor-core kernel does not
+// take), and the merge of split units that both kernels share.
+//
+//   out[row] = sum_j softmax_j(scale * q[row] . k_j) v_j
+//
+// over the cached keys and the step's own nodes that the row's mask shows
+// (chunk_visible64); a row that sees nothing is zeros. Serves trees of drafted tokens and
+// one-token decode over chosen pages (a page-table row per KV head).
+//
+// A CTA holds a block of kRows query rows (all heads of a KV group next to each other, so a
+// key is read once for the whole group) in shared memory as fp32 and streams the unit's keys
+// in 64-key tiles: S = Q K^T from registers (thread (ty, tx): rows ty * kRows / 16 .., keys
+// tx + 16 j), online softmax in base 2 with 16-lane shuffles, P through shared memory (over
+// K's tile, which S has finished with), O += P V in registers (dims tx * 4 + 64 c). All
+// arithmetic is fp32; 16-bit inputs are widened once, on the way into shared memory.
+//
+// Masked values never reach a sum: a masked score is -inf by selection, V rows past the
+// request's end are stored as zeros if they are not finite, and so are non-finite V values
+// of drafted nodes, which are added at the end to the rows that see them (0 * inf would
+// be NaN in every row).
+//
+// Bound: fp32 FMA at 64 rows (4 FMA per operand float4 loaded), shared-memory reads at 16.
+#include <type_traits>
+
+#include "chunk_schedule.cuh"
+
+namespace hyt {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kKeys = 64;
+
+template <typename T>
+__device__ __forceinline__ void widen16(const uint4& v, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T* e = reinterpret_cast<const T*>(&w[i]);
+      f[2 * i] = Elem<T>::to_float(e[0]);
+      f[2 * i + 1] = Elem<T>::to_float(e[1]);
+    }
+  }
+}
+
+// kRows: query rows per unit; kChunks: 64-dim column chunks of O (ceil(head_dim / 64)).
+template <typename T, int kRows, int kChunks>
+__global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const ChunkParams P) {
+  constexpr int kR = kRows / 16;       // rows per thread
+  constexpr int kD = kChunks * 64;     // padded head size
+  constexpr int kLd = kD + 4;          // shared row length: consecutive rows 4 banks apart
+  constexpr int kLdP = kKeys + 4;
+  constexpr int kPer = 16 / int(sizeof(T));
+  const AttentionParams& p = P.a;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int D = p.head_dim;
+
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;                // [kRows][kLd]
+  float* ks = qs + kRows * kLd;    // [kKeys][kLd], then P [kRows][kLdP]
+  float* vs = ks + kKeys * kLd;    // [kKeys][kLd]
+  float* ps = ks;
+  __shared__ int64_t sums[kThreads / 32];
+  __shared__ ChunkStart start;
+  __shared__ int nonfinite;        // a drafted node's V is not finite
+
+  chunk_find_start<kThreads>(P, blockIdx.x, P.ctas, sums, &start);
+  ChunkWalk walk(P, start, blockIdx.x, P.ctas);
+  ChunkSegment seg;
+  const float scale_log2 = p.scale * kLog2e;
+  const int page_mask = (1 << p.page_shift) - 1;
+
+  while (walk.next(P, seg)) {
+    const int rows_left = seg.queries * P.group - seg.row0;  // valid rows of this unit (may exceed kRows)
+    const int32_t* table = chunk_table(P, seg.b, seg.g);
+    const int64_t plane = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity;
+    const T* kp = static_cast<const T*>(p.k_pool) + plane * D;
+    const T* vp = static_cast<const T*>(p.v_pool) + plane * D;
+
+    __syncthreads();  // the previous segment's shared tiles are done with
+    if (tid == 0) nonfinite = 0;
+    for (int i = tid; i < kRows * kD; i += kThreads) {
+      const int r = i / kD, d = i - r * kD;
+      float v = 0.f;
+      if (r < rows_left && d < D)
+        v = Elem<T>::to_float(static_cast<const T*>(p.q)[chunk_q_offset(P, seg.b, seg.g, seg.row0 + r) + d]);
+      qs[r * kLd + d] = v;
+    }
+
+    float o[kR][kChunks][4], m_run[kR], l_run[kR];
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      m_run[i] = -INFINITY;
+      l_run[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
+    }
+
+    for (int tile = seg.k_lo; tile < seg.k_hi; ++tile) {
+      const int k0 = tile * kKeys;
+      // a tile never crosses a page: pages are powers of two of at least 64 tokens
+      const int lp = k0 >> p.page_shift;
+      int32_t page = -1;
+      if (!seg.refused) {
+        page = table[lp];
+        if (page < 0 || page >= p.num_pages) {
+          if (tid == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
+          page = -1;
+        }
+      }
+      const int kv_here = page < 0 ? 0 : min(seg.kv - k0, kKeys);  // keys of the tile that exist
+      __syncthreads();  // Q stored (first tile); P and V of the previous tile read
+      {
+        constexpr int kChunk16 = kD / kPer;  // 16-byte chunks of a padded row
+        const int64_t slot0 = (int64_t(max(page, 0)) << p.page_shift) + (k0 & page_mask);
+        for (int i = tid; i < kKeys * kChunk16; i += kThreads) {
+          const int r = i / kChunk16, c = i - r * kChunk16, d = c * kPer;
+          uint4 kraw = make_uint4(0u, 0u, 0u, 0u), vraw = kraw;
+          if (r < kv_here && d < D) {
+            kraw = __ldg(reinterpret_cast<const uint4*>(kp + (slot0 + r) * D + d));
+            vraw = __ldg(reinterpret_cast<const uint4*>(vp + (slot0 + r) * D + d));
+          }
+          float kf[kPer], vf[kPer];
+          widen16<T>(kraw, kf);
+          widen16<T>(vraw, vf);
+          if (k0 + r >= seg.len) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+              if (!isfinite(vf[e])) {
+                vf[e] = 0.f;
+                nonfinite = 1;
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < kPer; e += 4) {
+            *reinterpret_cast<float4*>(ks + r * kLd + d + e) = make_float4(kf[e], kf[e + 1], kf[e + 2], kf[e + 3]);
+            *reinterpret_cast<float4*>(vs + r * kLd + d + e) = make_float4(vf[e], vf[e + 1], vf[e + 2], vf[e + 3]);
+          }
+        }
+      }
+      __syncthreads();
+
+      // ---- S: rows ty * kR + i, keys tx + 16 j
+      float s[kR][4];
+#pragma unroll
+      for (int i = 0; i < kR; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < kD; d += 4) {
+        float4 kf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kLd + d);
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+          const float4 qf = *reinterpret_cast<const float4*>(qs + (ty * kR + i) * kLd + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[i][j] = fmaf(qf.w, kf[j].w, fmaf(qf.z, kf[j].z, fmaf(qf.y, kf[j].y, fmaf(qf.x, kf[j].x, s[i][j]))));
+        }
+      }
+
+      // ---- mask, online softmax (base 2); a row's 64 keys sit on 16 lanes
+      float pr[kR][4];
+#pragma unroll
+      for (int i = 0; i < kR; ++i) {
+        const int row = ty * kR + i;
+        uint64_t seen = ~0ull;
+        if (page < 0 || row >= rows_left)
+          seen = 0ull;
+        else if (k0 + kKeys > seg.len)
+          seen = chunk_visible64(P, seg.b, (seg.row0 + row) / P.group, seg.queries, k0 - seg.len);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = (seen >> (tx + 16 * j)) & 1 ? s[i][j] * scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float m_new = fmaxf(m_run[i], mx);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = ex2(m_run[i] - m_use);  // 0 before anything was seen
+        m_run[i] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pr[i][j] = ex2(s[i][j] - m_use);
+          sum += pr[i][j];
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l_run[i] = l_run[i] * alpha + sum;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][c][e] *= alpha;
+      }
+      __syncthreads();  // K read by everyone: P takes its place
+#pragma unroll
+      for (int i = 0; i < kR; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ps[(ty * kR + i) * kLdP + tx + 16 * j] = pr[i][j];
+      __syncwarp();  // a row's P is written and read by the same half-warp
+
+      // ---- O += P V: dims tx * 4 + 64 c
+#pragma unroll 2
+      for (int k = 0; k < kKeys; k += 4) {
+        float4 pf[kR];
+#pragma unroll
+        for (int i = 0; i < kR; ++i) pf[i] = *reinterpret_cast<const float4*>(ps + (ty * kR + i) * kLdP + k);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const float4 vf = *reinterpret_cast<const float4*>(vs + (k + kk) * kLd + c * 64 + tx * 4);
+#pragma unroll
+            for (int i = 0; i < kR; ++i) {
+              const float w = kk == 0 ? pf[i].x : (kk == 1 ? pf[i].y : (kk == 2 ? pf[i].z : pf[i].w));
+              o[i][c][0] = fmaf(w, vf.x, o[i][c][0]);
+              o[i][c][1] = fmaf(w, vf.y, o[i][c][1]);
+              o[i][c][2] = fmaf(w, vf.z, o[i][c][2]);
+              o[i][c][3] = fmaf(w, vf.w, o[i][c][3]);
+            }
+          }
+        }
+      }
+    }
+
+    __syncthreads();
+    const bool fix = nonfinite != 0;
+    const int64_t slot = int64_t(blockIdx.x) * 2 + (seg.first ? 0 : 1);
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const int row = ty * kR + i;
+      if (row >= rows_left) continue;
+      const int t = (seg.row0 + row) / P.group;
+      if (fix && !seg.refused) {  // non-finite V of the nodes this row sees, left out above
+        const int lo = max(seg.k_lo * kKeys, seg.len), hi = min(seg.k_hi * kKeys, seg.kv);
+        for (int pos = lo; pos < hi; ++pos) {
+          if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
+          const int32_t page = table[pos >> p.page_shift];
+          if (page < 0 || page >= p.num_pages) continue;
+          const T* vrow = vp + ((int64_t(page) << p.page_shift) + (pos & page_mask)) * D;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = c * 64 + tx * 4 + e;
+              if (d >= D) continue;
+              const float v = Elem<T>::to_float(vrow[d]);
+              if (!isfinite(v)) o[i][c][e] += v;
+            }
+        }
+      }
+      if (seg.whole) {
+        const float inv = l_run[i] == 0.f ? 0.f : 1.f / l_run[i];
+        T* out = static_cast<T*>(p.out) + chunk_o_offset(P, seg.b, seg.g, seg.row0 + row);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = c * 64 + tx * 4 + e;
+            if (d < D) out[d] = Elem<T>::from_float(o[i][c][e] * inv);
+          }
+      } else {
+        float4* wo = chunk_partial_o(P, slot);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int d = c * 64 + tx * 4;
+          if (d < D)
+            wo[int64_t(d / 4) * P.unit_rows + row] = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+        }
+        if (tx == 0) chunk_partial_ml(P, slot)[row] = make_float2(m_run[i], l_run[i]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ merge
+constexpr int kMergeThreads = 256;
+
+// Boundary c = blockIdx.x + 1 of the work line; the first boundary strictly inside a unit
+// joins that unit's partials: CTA c - 1's last segment (or first, if it starts with the
+// unit) and the first segments of the CTAs from c on. Thread: (row, 4 dims), consecutive
+// threads consecutive rows, as the partials are stored. Fixed order, no atomics.
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams P) {
+  __shared__ int64_t sums[kMergeThreads / 32];
+  __shared__ ChunkStart start;
+  const AttentionParams& p = P.a;
+  const int c = int(blockIdx.x) + 1, ctas = P.ctas;
+  chunk_find_start<kMergeThreads>(P, c, ctas, sums, &start);
+  const int64_t total = start.total, begin = chunk_begin(total, c, ctas);
+  if (begin >= total) return;
+  int why = 0;
+  const ChunkRequest r = chunk_request(P, start.b, why);
+  const int64_t unit = start.off / r.tiles, unit_off = start.off - unit * r.tiles;
+  const int64_t unit_begin = begin - unit_off, unit_end = unit_begin + r.tiles;
+  if (unit_off == 0 || chunk_begin(total, c - 1, ctas) > unit_begin) return;
+  const int g = int(unit / r.row_blocks), row0 = int(unit - int64_t(g) * r.row_blocks) * P.unit_rows;
+  const int rows = min(r.queries * P.group - row0, P.unit_rows);
+  const int idx = int(blockIdx.y) * kMergeThreads + int(threadIdx.x);
+  const int row = idx % P.unit_rows, d4 = idx / P.unit_rows;
+  if (row >= rows || d4 * 4 >= p.head_dim) return;
+
+  const int64_t slot0 = int64_t(c - 1) * 2 + (chunk_begin(total, c - 1, ctas) == unit_begin ? 0 : 1);
+  auto covers = [&](int i) {  // CTA i (>= c) holds a part of the unit (it may hold nothing at all)
+    return chunk_begin(total, i, ctas) < chunk_begin(total, i + 1, ctas);
+  };
+#ifdef __CUDA_ARCH__
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+#endif
+  float m = __ldcg(&chunk_partial_ml(P, slot0)[row]).x;
+  for (int i = c; i < ctas && chunk_begin(total, i, ctas) < unit_end; ++i)
+    if (covers(i)) m = fmaxf(m, __ldcg(&chunk_partial_ml(P, int64_t(i) * 2)[row]).x);
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int64_t slot) {
+    const float2 ml = __ldcg(&chunk_partial_ml(P, slot)[row]);
+    const float4 v = __ldcg(&chunk_partial_o(P, slot)[int64_t(d4) * P.unit_rows + row]);
+    if (ml.y == 0.f) return;  // nothing seen in this part
+    const float f = ex2(ml.x - m_use);
+    l = fmaf(ml.y, f, l);
+    o.x = fmaf(v.x, f, o.x);
+    o.y = fmaf(v.y, f, o.y);
+    o.z = fmaf(v.z, f, o.z);
+    o.w = fmaf(v.w, f, o.w);
+  };
+  add(slot0);
+#pragma unroll 4
+  for (int i = c; i < ctas && chunk_begin(total, i, ctas) < unit_end; ++i)
+    if (covers(i)) add(int64_t(i) * 2);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(p.out) + chunk_o_offset(P, start.b, g, row0 + row) + d4 * 4;
+  out[0] = Elem<T>::from_float(o.x * inv);
+  out[1] = Elem<T>::from_float(o.y * inv);
+  out[2] = Elem<T>::from_float(o.z * inv);
+  out[3] = Elem<T>::from_float(o.w * inv);
+}
+
+template <typename T, int kRows, int kChunks>
+constexpr int general_smem() {
+  return (kRows + 2 * kKeys) * (kChunks * 64 + 4) * 4;
+}
+
+template <typename T, int kRows, int kChunks>
+cudaError_t launch_general(const ChunkParams& p, cudaStream_t stream) {
+  static_assert(kRows * (kKeys + 4) <= kKeys * (kChunks * 64 + 4), "P must fit in K's tile");
+  auto kernel = chunk_attention_general_kernel<T, kRows, kChunks>;
+  constexpr int smem = general_smem<T, kRows, kChunks>();
+  cudaError_t e = allow_smem(kernel, smem, stream);
+  if (e != cudaSuccess) return e;
+  kernel<<<p.ctas, kThreads, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int kRows>
+cudaError_t launch_general_dim(const ChunkParams& p, cudaStream_t stream) {
+  switch ((p.a.head_dim + 63) / 64) {
+    case 1: return launch_general<T, kRows, 1>(p, stream);
+    case 2: return launch_general<T, kRows, 2>(p, stream);
+    case 3: return launch_general<T, kRows, 3>(p, stream);
+    default: return launch_general<T, kRows, 4>(p, stream);
+  }
+}
+
+template <typename T>
+cudaError_t launch_general_rows(const ChunkParams& p, cudaStream_t stream) {
+  return p.unit_rows == 16 ? launch_general_dim<T, 16>(p, stream) : launch_general_dim<T, 64>(p, stream);
+}
+
+}  // namespace
+
+ChunkShape chunk_shape_general(int64_t max_rows, int dtype, int head_dim, int num_sms) {
+  (void)dtype;
+  const int rows = max_rows <= 16 ? 16 : 64;
+  // resident CTAs per SM by shared memory (228 KB per SM, 1 KB reserved per CTA)
+  const int smem = (rows + 2 * kKeys) * ((head_dim + 63) / 64 * 64 + 4) * 4 + 1024;
+  const int per_sm = smem * 3 <= 228 * 1024 ? 3 : (smem * 2 <= 228 * 1024 ? 2 : 1);
+  return {rows, kKeys, num_sms * per_sm};
+}
+
+cudaError_t run_chunk_attention_general(const ChunkParams& p, int dtype, cudaStream_t stream) {
+  switch (dtype) {
+    case HYT_DTYPE_BF16: return launch_general_rows<__nv_bfloat16>(p, stream);
+    case HYT_DTYPE_F16: return launch_general_rows<__half>(p, stream);
+    default: return launch_general_rows<float>(p, stream);
+  }
+}
+
+cudaError_t run_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t stream) {
+  if (p.ctas < 2) return cudaSuccess;
+  const int64_t work = int64_t(p.unit_rows) * (p.a.head_dim / 4);
+  const dim3 grid(unsigned(p.ctas - 1), unsigned((work + kMergeThreads - 1) / kMergeThreads));
+  switch (dtype) {
+    case HYT_DTYPE_BF16: chunk_merge_kernel<__nv_bfloat16><<<grid, kMergeThreads, 0, stream>>>(p); break;
+    case HYT_DTYPE_F16: chunk_merge_kernel<__half><<<grid, kMergeThreads, 0, stream>>>(p); break;
+    default: chunk_merge_kernel<float><<<grid, kMergeThreads, 0, stream>>>(p); break;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace hyt

@@ -29,6 +29,7 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
     "-Xcompiler", "-fPIC,-O2",
     "-shared",
+    "--threads", "0",  # one compiler per source file
 ]
 
 

@@ -25,6 +25,7 @@ DEVICE_ERRORS = {
     16: "tensor-core ops issued on other than exactly one lane (work skipped)",
     32: "packed batch metadata (q_start / q_len / request id) out of range",
     64: "prefill plan item out of range",
+    128: "page or row moves whose result would depend on their order",
 }
 
 _c_i32, _c_i64, _c_f32, _c_size, _c_p = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float,
@@ -79,6 +80,24 @@ SIGNATURES = {
                                                           _c_i32, _c_i32, _c_i32, _c_i32, _c_p, _c_size,
                                                           _c_p, _c_i32, _c_i32, _c_p, _c_size, _c_p,
                                                           _c_p]),
+    # drafted trees, page and row moves, decode over chosen pages
+    "hyt_tree_workspace_bytes": (_c_size, [_c_i32] * 5),
+    "hyt_tree_attention": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i64, _c_p, _c_i32,
+                                          _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_i32,
+                                          _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32,
+                                          _c_i32, _c_p, _c_size, _c_p, _c_p]),
+    "hyt_copy_pages": (ctypes.c_int, [_c_p, _c_p, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p,
+                                      _c_p, _c_i32, _c_p, _c_p]),
+    "hyt_compact_rows": (ctypes.c_int, [_c_p, _c_p, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32,
+                                        _c_p, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_p,
+                                        _c_p]),
+    "hyt_page_bounds": (ctypes.c_int, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32,
+                                       _c_i32, _c_i32, _c_p, _c_i32, _c_p, _c_p]),
+    "hyt_sparse_workspace_bytes": (_c_size, [_c_i32] * 6),
+    "hyt_sparse_attention": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i64, _c_p,
+                                            _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32,
+                                            _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_i32, _c_p,
+                                            _c_size, _c_p, _c_p]),
     "hyt_attention_workspace_bytes": (_c_size, [_c_i32] * 8),
     "hyt_workspace_init": (ctypes.c_int, [_c_p, _c_size, _c_p]),
     "hyt_wait_self_test": (ctypes.c_int, [_c_p, _c_p, _c_p]),

@@ -7,6 +7,7 @@ message if the call is refused. All launches go on the current CUDA stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -506,3 +507,242 @@ def prefill_attention_planned(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
         _stream_ptr())
     _lib.check(rc, "hyt_prefill_attention_planned")
     return out
+
+
+# ---------------------------------------------------------------------------- trees, moves, chosen pages
+def _same_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The one CUDA device all tensors are on."""
+    tensors = [t for t in tensors if t is not None]
+    _require_cuda(*tensors)
+    device = tensors[0].device
+    if any(t.device != device for t in tensors):
+        raise RuntimeError("all tensors must be on the same CUDA device")
+    return device
+
+
+def _on(device: torch.device):
+    """Launch on ``device``: its current stream, whatever the current device is."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous one-dimensional int32 tensor")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must have {numel} entries, got {t.numel()}")
+
+
+def _page_rows(page_table: torch.Tensor, batch: int) -> tuple[int, int]:
+    """(entries between rows, entries of a row) of an int32 ``[batch, pages]`` table."""
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.size(0) != batch:
+        raise ValueError("page_table must be an int32 [batch, pages] tensor")
+    width = page_table.size(1)
+    if width < 1 or (width > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must have at least one page per row and contiguous rows")
+    if batch > 1 and page_table.stride(0) < width:
+        raise ValueError("page_table rows must not overlap")
+    return max(page_table.stride(0), width), width
+
+
+def _output(out: torch.Tensor | None, like: torch.Tensor, memory: tuple[int, ...]) -> torch.Tensor:
+    """``out`` checked against ``like``, or a new one in ``[.., T, H, D]`` memory viewed as ``like``."""
+    if out is None:
+        return torch.empty(memory, dtype=like.dtype, device=like.device).transpose(1, 2)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError("out must match q")
+    return out
+
+
+def _scratch(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise RuntimeError(f"the workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    return workspace
+
+
+@functools.lru_cache(maxsize=1024)
+def tree_workspace_bytes(max_query_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                         dtype: torch.dtype) -> int:
+    """Workspace bytes of ``tree_attention`` (``hyt_tree_workspace_bytes``)."""
+    return int(_lib.lib().hyt_tree_workspace_bytes(max_query_len, num_q_heads, num_kv_heads, head_dim,
+                                                   dtype_code(dtype)))
+
+
+def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, layer: int,
+                   page_table: torch.Tensor, cache_lens: torch.Tensor, q_start: torch.Tensor,
+                   q_len: torch.Tensor, tree_mask: torch.Tensor | None, page_size: int,
+                   max_query_len: int, scale: float | None = None, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None,
+                   error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of drafted trees, ``q`` ``[1, H_q, N, D]`` on a packed batch's token axis.
+
+    Request b's nodes are rows ``q_start[b] .. q_start[b] + q_len[b] - 1`` (none if ``q_len[b]``
+    is 0), their K/V already written at positions ``cache_lens[b] + i``. Every node sees the
+    cached tokens; row i of ``tree_mask`` (int32 ``[N, words]``, bit j % 32 of word j // 32) says
+    which nodes of its own request it sees, itself included only if its bit is set. A node
+    that sees nothing gets zeros. ``None`` is a causal chunk. ``max_query_len`` is at least
+    every ``q_len``. Rows of the token axis that no request owns are left as they are.
+    ``workspace`` (``tree_workspace_bytes``, any contents) is allocated if not given.
+    """
+    device = _same_device(q, k_pool, v_pool, page_table, cache_lens, q_start, q_len, tree_mask, out,
+                          workspace, error_word)
+    num_layers, num_kv_heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
+    qs = _th_strides(q, "q")
+    _, num_q_heads, total, d = q.shape
+    if d != head_dim or q.dtype != k_pool.dtype:
+        raise ValueError("q must match the pool's head_dim and dtype")
+    batch = cache_lens.numel()
+    for t, name in ((cache_lens, "cache_lens"), (q_start, "q_start"), (q_len, "q_len")):
+        _int32_vector(t, name, batch)
+    stride, width = _page_rows(page_table, batch)
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or not tree_mask.is_contiguous():
+            raise TypeError("tree_mask must be a contiguous int32 [tokens, words] tensor")
+        words = tree_mask.size(1)
+        if tree_mask.size(0) != total or words * 32 < max_query_len:
+            raise ValueError("tree_mask must have a row per token and a bit per node")
+    out = _output(out, q, (1, total, num_q_heads, head_dim))
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    if total == 0:
+        return out
+    need = tree_workspace_bytes(max_query_len, num_q_heads, num_kv_heads, head_dim, q.dtype)
+    workspace = _scratch(workspace, need, device)
+    with _on(device):
+        rc = _lib.lib().hyt_tree_attention(
+            q.data_ptr(), _lib.int64_array(qs), k_pool.data_ptr(), v_pool.data_ptr(), num_layers, layer,
+            capacity, page_table.data_ptr(), stride, width, cache_lens.data_ptr(), q_start.data_ptr(),
+            q_len.data_ptr(), _ptr(tree_mask), words, out.data_ptr(),
+            _lib.int64_array(_th_strides(out, "out")), batch, total, num_q_heads, num_kv_heads, head_dim,
+            page_size, dtype_code(q.dtype), scale, max_query_len, workspace.data_ptr(),
+            workspace.numel(), _ptr(error_word), _stream_ptr())
+    _lib.check(rc, "hyt_tree_attention")
+    return out
+
+
+def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, src_pages: torch.Tensor,
+               dst_pages: torch.Tensor, page_size: int, error_word: torch.Tensor | None = None) -> None:
+    """Copy page ``src_pages[m]`` to page ``dst_pages[m]`` in every layer and KV head, one launch.
+
+    Of two entries with one target the later counts. An entry whose target another entry
+    reads is skipped and flagged in ``error_word``, as are ids outside the pool."""
+    device = _same_device(k_pool, v_pool, src_pages, dst_pages, error_word)
+    num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
+    _int32_vector(src_pages, "src_pages")
+    _int32_vector(dst_pages, "dst_pages", src_pages.numel())
+    with _on(device):
+        rc = _lib.lib().hyt_copy_pages(
+            k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity, head_dim, page_size,
+            dtype_code(k_pool.dtype), src_pages.data_ptr(), dst_pages.data_ptr(), src_pages.numel(),
+            _ptr(error_word), _stream_ptr())
+    _lib.check(rc, "hyt_copy_pages")
+
+
+def compact_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+                 base: torch.Tensor, src_rows: torch.Tensor, src_start: torch.Tensor, page_size: int,
+                 error_word: torch.Tensor | None = None) -> None:
+    """Move request b's K/V rows at positions ``base[b] + src_rows[src_start[b] + i]`` to
+    ``base[b] + i`` in every layer and KV head, in place.
+
+    ``src_rows`` is strictly increasing and not negative within each request (entries that
+    are not are skipped and flagged in ``error_word``); ``src_start`` has ``batch + 1`` entries
+    from 0 to ``len(src_rows)``. The accepted path of a drafted tree moves up behind the
+    context this way. No two requests may share a page in which rows move."""
+    device = _same_device(k_pool, v_pool, page_table, base, src_rows, src_start, error_word)
+    num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
+    _int32_vector(base, "base")
+    batch = base.numel()
+    _int32_vector(src_rows, "src_rows")
+    _int32_vector(src_start, "src_start", batch + 1)
+    stride, width = _page_rows(page_table, batch)
+    with _on(device):
+        rc = _lib.lib().hyt_compact_rows(
+            k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity, head_dim, page_size,
+            dtype_code(k_pool.dtype), page_table.data_ptr(), stride, width, base.data_ptr(),
+            src_rows.data_ptr(), src_start.data_ptr(), batch, src_rows.numel(), _ptr(error_word),
+            _stream_ptr())
+    _lib.check(rc, "hyt_compact_rows")
+
+
+def _check_bounds(k_bounds: torch.Tensor, k_pool: torch.Tensor, page_size: int) -> None:
+    num_layers, _, heads, capacity, head_dim = k_pool.shape
+    expect = (num_layers, heads, capacity // page_size if page_size > 0 else 0, 2, head_dim)
+    if tuple(k_bounds.shape) != expect or k_bounds.dtype != k_pool.dtype or not k_bounds.is_contiguous():
+        raise ValueError(f"k_bounds must be a contiguous {expect} tensor of the pool's dtype "
+                         "([layers, kv_heads, pages, 2, head_dim])")
+
+
+def page_bounds(k_pool: torch.Tensor, k_bounds: torch.Tensor, pages: torch.Tensor, page_size: int,
+                layer: int | None = None, error_word: torch.Tensor | None = None) -> None:
+    """Write the elementwise minimum and maximum of each listed page's keys into ``k_bounds``
+    ``[layers, H_kv, num_pages, 2, D]`` (all layers, or one), for ``sparse_attention``.
+
+    ``pages`` (int32) lists pages whose tokens are all written; -1 entries are skipped."""
+    device = _same_device(k_pool, k_bounds, pages, error_word)
+    num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, k_pool)
+    _check_bounds(k_bounds, k_pool, page_size)
+    _int32_vector(pages, "pages")
+    first, layers = (0, num_layers) if layer is None else (layer, 1)
+    with _on(device):
+        rc = _lib.lib().hyt_page_bounds(
+            k_pool.data_ptr(), k_bounds.data_ptr(), num_layers, first, layers, heads, capacity, head_dim,
+            page_size, dtype_code(k_pool.dtype), pages.data_ptr(), pages.numel(), _ptr(error_word),
+            _stream_ptr())
+    _lib.check(rc, "hyt_page_bounds")
+
+
+@functools.lru_cache(maxsize=1024)
+def sparse_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                           num_pages: int, dtype: torch.dtype) -> int:
+    """Workspace bytes of ``sparse_attention`` (``hyt_sparse_workspace_bytes``)."""
+    return int(_lib.lib().hyt_sparse_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_pages,
+                                                     dtype_code(dtype)))
+
+
+def sparse_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     k_bounds: torch.Tensor, layer: int, page_table: torch.Tensor,
+                     cache_lens: torch.Tensor, page_size: int, num_pages: int,
+                     scale: float | None = None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None,
+                     error_word: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One-token decode of ``q`` ``[B, H_q, 1, D]`` over ``num_pages`` pages per KV head.
+
+    Token b sits at position ``cache_lens[b]``, its K/V already written. Per request and KV
+    head it attends the page being written and the ``num_pages - 1`` full pages whose
+    ``k_bounds`` allow the largest score: the maximum over the KV head's query heads of
+    ``sum_d q_d * (max_d if q_d >= 0 else min_d)``, rounded once to fp32, ties to the lower
+    page. With no more than ``num_pages`` pages that is every page. Returns the rows
+    ``[B, H_q, 1, D]`` and the logical pages read, int32 ``[B, H_kv, num_pages]``, ascending,
+    -1 past the last. ``workspace`` (``sparse_workspace_bytes``, any contents) is allocated
+    if not given."""
+    device = _same_device(q, k_pool, v_pool, k_bounds, page_table, cache_lens, out, workspace, error_word)
+    num_layers, num_kv_heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
+    _check_bounds(k_bounds, k_pool, page_size)
+    qs = _bht_strides(q, "q")
+    batch, num_q_heads, query_len, d = q.shape
+    if query_len != 1:
+        raise ValueError("sparse attention takes one query token per request")
+    if d != head_dim or q.dtype != k_pool.dtype:
+        raise ValueError("q must match the pool's head_dim and dtype")
+    _int32_vector(cache_lens, "cache_lens", batch)
+    stride, width = _page_rows(page_table, batch)
+    out = _output(out, q, (batch, 1, num_q_heads, head_dim))
+    os_ = _bht_strides(out, "out")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    if num_pages < 1:
+        raise ValueError("num_pages must be positive")
+    selected = torch.empty((batch, num_kv_heads, num_pages), dtype=torch.int32, device=device)
+    need = sparse_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_pages, q.dtype)
+    workspace = _scratch(workspace, need, device)
+    with _on(device):
+        rc = _lib.lib().hyt_sparse_attention(
+            q.data_ptr(), _lib.int64_array(qs[:2]), k_pool.data_ptr(), v_pool.data_ptr(),
+            k_bounds.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride, width,
+            cache_lens.data_ptr(), out.data_ptr(), _lib.int64_array(os_[:2]), selected.data_ptr(), batch,
+            num_q_heads, num_kv_heads, head_dim, page_size, dtype_code(q.dtype), scale, num_pages,
+            workspace.data_ptr(), workspace.numel(), _ptr(error_word), _stream_ptr())
+    _lib.check(rc, "hyt_sparse_attention")
+    return out, selected

@@ -54,7 +54,8 @@ enum {
   HYT_DEVERR_WAIT_TIMEOUT = 8, /* a bounded pipeline wait gave up */
   HYT_DEVERR_ISSUE_LANE = 16,  /* tensor-core issue ran on other than exactly one lane (work skipped) */
   HYT_DEVERR_PACKED_RANGE = 32, /* packed batch: q_start/q_len/request id out of range (work skipped) */
-  HYT_DEVERR_PLAN_RANGE = 64    /* prefill plan item out of range (work skipped) */
+  HYT_DEVERR_PLAN_RANGE = 64,   /* prefill plan item out of range (work skipped) */
+  HYT_DEVERR_MOVE_ORDER = 128   /* page or row moves whose result would depend on their order (skipped) */
 };
 
 /* Message of the last failed call on this thread ("" if none). */
@@ -344,6 +345,93 @@ int hyt_wait_self_test(int32_t* error_word, int64_t* elapsed_ns, void* stream);
  * in flight per thread; writes one XOR word per CTA to sink (device, uint32[ctas]). Timed
  * around, it gives the HBM read ceiling the memory-bound decode kernel is compared with. */
 int hyt_read_probe(const void* src, size_t bytes, uint32_t* sink, int32_t ctas, void* stream);
+
+/*
+ * Attention of drafted trees over the paged cache (speculative decoding; no counterpart in
+ * the reference, whose decode step attends one token per request, hayate/engine/engine.py:
+ * 285-296). Packed like hyt_paged_attention_packed: request b's nodes are rows q_start[b] ..
+ * q_start[b] + q_len[b] - 1 of the token axis (q_len may be 0), their K/V already in slots
+ * cache_lens[b] + i. Node i sees every cached token and node j of its request if bit j % 32 of
+ * word j / 32 of its row of tree_mask [total_tokens, mask_words] is set (its own bit
+ * included); a node that sees nothing gets zeros. tree_mask NULL: the chunk is causal. q/out
+ * strides = {t, h}. page_table_width: entries of a table row (page_table_stride is the
+ * distance between rows). head_dim a multiple of 8 up to 256, page_size >= 64, scale > 0.
+ * The workspace (hyt_tree_workspace_bytes, 16-byte aligned) needs no initial contents and
+ * holds none between calls; calls that overlap need one each.
+ */
+size_t hyt_tree_workspace_bytes(int32_t max_query_len, int32_t num_q_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t dtype);
+int hyt_tree_attention(const void* q, const int64_t* q_strides, const void* k_pool,
+                       const void* v_pool, int32_t num_layers, int32_t layer,
+                       int64_t capacity_tokens, const int32_t* page_table,
+                       int32_t page_table_stride, int32_t page_table_width,
+                       const int32_t* cache_lens, const int32_t* q_start, const int32_t* q_len,
+                       const int32_t* tree_mask, int32_t mask_words, void* out,
+                       const int64_t* out_strides, int32_t batch, int32_t total_tokens,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t page_size, int32_t dtype, float scale, int32_t max_query_len,
+                       void* workspace, size_t workspace_bytes, int32_t* error_word,
+                       void* stream);
+
+/*
+ * Page src_pages[m] copied to page dst_pages[m] in every layer and KV head of both pools,
+ * one launch (copy-on-write and forks; replaces a pool slice copy per page). Of two entries
+ * with one target the later counts; an entry whose target another entry reads is skipped
+ * and flagged (HYT_DEVERR_MOVE_ORDER). At most 65535 entries.
+ */
+int hyt_copy_pages(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_heads,
+                   int64_t capacity_tokens, int32_t head_dim, int32_t page_size, int32_t dtype,
+                   const int32_t* src_pages, const int32_t* dst_pages, int32_t count,
+                   int32_t* error_word, void* stream);
+
+/*
+ * Request b's row base[b] + src_rows[src_start[b] + i] moved to row base[b] + i, i = 0 ..
+ * src_start[b + 1] - src_start[b] - 1, in every layer and KV head of both pools, in place: the
+ * accepted path of a drafted tree moves up behind the context. src_rows strictly
+ * increasing per request and never negative; an entry that is not is skipped and flagged
+ * (HYT_DEVERR_MOVE_ORDER). src_start has batch + 1 entries, the last one total_rows. No two
+ * requests of a call may share a page that a row moves in.
+ */
+int hyt_compact_rows(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_heads,
+                     int64_t capacity_tokens, int32_t head_dim, int32_t page_size, int32_t dtype,
+                     const int32_t* page_table, int32_t page_table_stride,
+                     int32_t page_table_width, const int32_t* base, const int32_t* src_rows,
+                     const int32_t* src_start, int32_t batch, int32_t total_rows,
+                     int32_t* error_word, void* stream);
+
+/*
+ * Elementwise minimum and maximum over a page's keys, for the pages listed (-1 entries are
+ * skipped), layers first_layer .. first_layer + layers - 1 and every KV head, into k_bounds
+ * [num_layers, num_kv_heads, capacity_tokens / page_size, 2, head_dim] (pool dtype; minimum
+ * first). Every token of a listed page must have been written. NaN keys give NaN bounds.
+ */
+int hyt_page_bounds(const void* k_pool, void* k_bounds, int32_t num_layers, int32_t first_layer,
+                    int32_t layers, int32_t num_kv_heads, int64_t capacity_tokens,
+                    int32_t head_dim, int32_t page_size, int32_t dtype, const int32_t* pages,
+                    int32_t count, int32_t* error_word, void* stream);
+
+/*
+ * One-token decode over chosen pages. Query token b (at position cache_lens[b], its K/V
+ * already in place) attends, per KV head, the page being written and the num_pages - 1 full
+ * pages with the largest score, or all pages if there are no more than num_pages:
+ *   score = max over the KV head's query heads of sum_d q_d * (q_d >= 0 ? max_d : min_d)
+ * summed in 64 bits and rounded once to fp32; ties go to the lower page, NaN ranks first.
+ * The logical pages read are written to selected [batch, num_kv_heads, num_pages],
+ * ascending, -1 past the last. q/out strides = {b, h}. k_bounds must hold hyt_page_bounds of
+ * every full page. Limits as for hyt_tree_attention, and at most 16384 pages per request.
+ * The workspace (hyt_sparse_workspace_bytes) needs no initial contents.
+ */
+size_t hyt_sparse_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                  int32_t head_dim, int32_t num_pages, int32_t dtype);
+int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_pool,
+                         const void* v_pool, const void* k_bounds, int32_t num_layers,
+                         int32_t layer, int64_t capacity_tokens, const int32_t* page_table,
+                         int32_t page_table_stride, int32_t page_table_width,
+                         const int32_t* cache_lens, void* out, const int64_t* out_strides,
+                         int32_t* selected, int32_t batch, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                         int32_t dtype, float scale, int32_t num_pages, void* workspace,
+                         size_t workspace_bytes, int32_t* error_word, void* stream);
 
 #ifdef __cplusplus
 }
