@@ -581,6 +581,7 @@ int check_norm_rope_alignment(int dtype, const void* q, const void* k, const voi
 }
 
 // ------------------------------------------------------------------ chunk attention, moves, selection
+constexpr int kTensorKeys = 128;  // rows of the tensor-core kernel's K/V boxes
 constexpr int kSms = 148;  // work is shared out over this many SMs (fewer would only queue CTAs)
 
 int check_scale(float scale) {
@@ -605,7 +606,10 @@ int64_t chunk_max_rows(int32_t num_q_heads, int32_t num_kv_heads, int32_t query_
 size_t chunk_workspace(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t query_len,
                        int32_t dtype) {
   const int64_t rows = chunk_max_rows(num_q_heads, num_kv_heads, query_len);
-  return align256(size_t(hyt::chunk_workspace_bytes(hyt::chunk_shape_general(rows, dtype, head_dim, kSms), head_dim)));
+  const hyt::ChunkShape general = hyt::chunk_shape_general(rows, dtype, head_dim, kSms);
+  const hyt::ChunkShape tensor = hyt::chunk_shape_tensor(rows, kSms);
+  return align256(size_t(std::max(hyt::chunk_workspace_bytes(general, head_dim),
+                                  hyt::chunk_workspace_bytes(tensor, head_dim))));
 }
 
 int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t workspace_bytes,
@@ -615,13 +619,28 @@ int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t
     return fail(HYT_ERR_WORKSPACE, "workspace missing, not 16-byte aligned or too small");
   c.group = g.num_q_heads / g.num_kv_heads;
   const int64_t rows = chunk_max_rows(g.num_q_heads, g.num_kv_heads, g.query_len);
-  const hyt::ChunkShape s = hyt::chunk_shape_general(rows, g.dtype, g.head_dim, kSms);
+  const bool tensor = g.dtype != HYT_DTYPE_F32 && g.head_dim >= 64 && g.head_dim <= 128 && g.page_size % 128 == 0;
+  const hyt::ChunkShape s = tensor ? hyt::chunk_shape_tensor(rows, kSms)
+                                   : hyt::chunk_shape_general(rows, g.dtype, g.head_dim, kSms);
   c.unit_rows = s.unit_rows;
   c.tile_keys = s.tile_keys;
   c.ctas = s.ctas;
   c.ws_o = static_cast<float*>(workspace);
   c.ws_ml = c.ws_o + int64_t(s.ctas) * 2 * s.unit_rows * g.head_dim;
-  cudaError_t err = hyt::run_chunk_attention_general(c, g.dtype, stream);
+  cudaError_t err;
+  if (tensor) {
+    CUtensorMap k_map, v_map;
+    const int64_t planes = int64_t(g.num_layers) * g.num_kv_heads;
+    int rc = pool_tensor_map(c.a.k_pool, g.dtype, g.head_dim, g.capacity, planes, kTensorKeys, &k_map);
+    if (rc != HYT_OK) return rc;
+    rc = pool_tensor_map(c.a.v_pool, g.dtype, g.head_dim, g.capacity, planes, kTensorKeys, &v_map);
+    if (rc != HYT_OK) return rc;
+    const int64_t qs[3] = {c.a.q_sb, c.a.q_sh, c.a.q_st}, os[3] = {c.a.o_sb, c.a.o_sh, c.a.o_st};
+    err = hyt::run_chunk_attention_tensor(c, rows_16b_aligned(c.a.q, qs), rows_16b_aligned(c.a.out, os), k_map,
+                                          v_map, g.dtype, stream);
+  } else {
+    err = hyt::run_chunk_attention_general(c, g.dtype, stream);
+  }
   if (err != cudaSuccess) return cuda_fail(err, "chunk attention launch");
   err = hyt::run_chunk_merge(c, g.dtype, stream);
   if (err != cudaSuccess) return cuda_fail(err, "chunk attention merge launch");

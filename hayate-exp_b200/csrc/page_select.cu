@@ -308,7 +308,7 @@ cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stre
   const int smem = group * p.head_dim * 8 + ranked * 4;
   const dim3 grid(unsigned(p.num_kv_heads), unsigned(p.batch));
   auto launch = [&](auto kernel) {
-    cudaError_t e = allow_smem(kernel, smem, stream);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     kernel<<<grid, kSelectThreads, smem, stream>>>(p);
     return cudaGetLastError();

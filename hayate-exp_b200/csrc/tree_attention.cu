@@ -1,0 +1,639 @@
+// Chunk attention on tcgen05 tensor cores: trees of drafted tokens, and one-token decode over
+// chosen pages, for bf16 / f16 and head sizes 64 .. 128.
+//
+//   out[row] = sum_j softmax_j(scale * q[row] . k_j) v_j
+//
+// over the cached keys and the step's own nodes that the row's mask shows. The rows of a
+// unit are all heads of one KV group times the request's queries (row t * group + hl), so a
+// key is read once for the whole group and a tree of 32 nodes with 4 heads fills the 128
+// lanes of an MMA. Work is shared out by chunk_schedule.cuh: 148 CTAs, one per SM, each an
+// equal stretch of 128-key tiles.
+//
+// Two streams x = 0, 1 of S / P / O keep the tensor cores and the softmax warps busy at the
+// same time:
+//   one row block per unit (kDual false, at most 128 rows): stream x takes the tiles i with
+//     i % 2 == x, both with the same Q, and the two online softmaxes are joined at the end;
+//   two row blocks (kDual true): stream x is row block x, both see every tile, so a K/V tile
+//     brought into shared memory serves 256 rows.
+// 576 threads: warps 0-7 softmax of stream 0, 8-15 of stream 1 (in a stream, warps w and
+// w + 4 own rows 32 (w % 4) .. and half of the 128 key columns each), warp 16 the TMA
+// producer, warp 17 the MMA issuer. Per tile, S = Q K^T (shared x shared), P goes back over
+// S's columns as 16-bit pairs, O += P V (TMEM x shared). Issue order PV(s), QK(s + 2).
+// TMEM (512 columns): S_0/P_0 [0,128), S_1/P_1 [128,256), O_0 [256,384), O_1 [384,512).
+// Shared memory: Q 32 KB per row block, 2 K stages, 3 (one row block) or 2 V stages of 32 KB.
+// Head sizes below 128 are padded with zeros by TMA's out-of-range fill and the Q stores;
+// up to 64, the second 64-dim half is neither loaded nor multiplied.
+//
+// Masking: scores by selection. V rows of the tiles that reach past the cached tokens are
+// looked through before they are multiplied: values that are not finite become zeros, and
+// those of drafted nodes are added at the end to the rows that see them (0 * inf would
+// be NaN in every row).
+//
+// P is rounded to the storage type (the MMA's operand type); scores, running maximum and
+// sum, and O are fp32. The running maximum may lag by up to 2^8 (O / l is exact all the same).
+#include <type_traits>
+
+#include "chunk_schedule.cuh"
+
+namespace hyt {
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kKeys = 128;
+constexpr int kSoftmaxThreads = 512;
+constexpr int kProducerWarp = 16, kMmaWarp = 17;
+constexpr int kSoftmaxBar = 9;  // named barrier of all softmax warps (1 .. 8: row-quarter pairs)
+constexpr int kThreads = 576;
+constexpr int kTileBytes = kRows * 128 * 2;
+constexpr int kChunkBytes = kTileBytes / 2;  // [128 rows x 64 elements]
+constexpr int kKStages = 2;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kOCol = 256;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr int kPrefetchTiles = 3;
+
+struct Shared {
+  uint64_t q_full;
+  uint64_t k_full[kKStages], k_empty[kKStages], v_full[3], v_empty[3];
+  uint64_t s_full[2], p_full[2];
+  uint64_t o_done, drain;
+  uint32_t tmem_base;
+  int32_t abort;       // a bounded wait gave up: later waits return at once
+  int32_t fix;         // a drafted node's V is not finite
+  int32_t refused[8];  // per tile (ring): page refused, nothing of the tile is visible
+  ChunkStart start;
+  int64_t sums[kThreads / 32];
+  float m[2][kRows];         // running maxima of the streams (joined at the end)
+  float sum[2][2][kRows];    // [stream][column half][row]
+  float max[2][2][2][kRows]; // [stream][parity][column half][row]
+};
+
+template <bool kDual>
+struct Layout {
+  static constexpr int kVStages = kDual ? 2 : 3;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + (kDual ? 2 : 1) * kTileBytes;
+  static constexpr int kV = kK + kKStages * kTileBytes;
+  static constexpr int kShared = kV + kVStages * kTileBytes;
+  static constexpr int kBytes = kShared + int(sizeof(Shared)) + 1024;
+};
+
+// Byte offset of 16-byte chunk `chunk` of row `r` in a [128 x 128] tile stored as two
+// 128B-swizzled [128 x 64] chunks.
+__device__ __forceinline__ uint32_t sw128_offset(int r, int chunk) {
+  return uint32_t((chunk >> 3) * kChunkBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+}
+
+// P = 2^(s * scale_log2 - m) of 64 scores, written to TMEM as packed 16-bit pairs; returns
+// their sum. 7 of 8 exponentials on MUFU, 1 of 8 on the FMA pipe.
+template <typename T>
+__device__ __forceinline__ float exp_tile(const float (&s)[64], uint64_t scale2, float m, uint32_t p_addr) {
+  const uint64_t neg_m2 = f2_pack(-m, -m);
+  uint64_t sum2a = f2_pack(0.f, 0.f), sum2b = sum2a;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = c * 32 + 2 * i;
+      const uint64_t x2 = f2_fma(f2_pack(s[k], s[k + 1]), scale2, neg_m2);
+      float a, b;
+      f2_unpack(x2, a, b);
+      const float pa = ex2(a);
+      const float pb = (i & 3) == 3 ? ex2_poly(b) : ex2(b);
+      if (i & 1) sum2b = f2_add(sum2b, f2_pack(pa, pb));
+      else sum2a = f2_add(sum2a, f2_pack(pa, pb));
+      packed[i] = Elem<T>::pack2(pa, pb);
+    }
+    tmem_st16(p_addr + c * 16, packed);
+  }
+  float sa0, sa1, sb0, sb1;
+  f2_unpack(sum2a, sa0, sa1);
+  f2_unpack(sum2b, sb0, sb1);
+  return (sa0 + sb0) + (sa1 + sb1);
+}
+
+struct TreeKernelParams {
+  ChunkParams c;
+  int32_t q_vec, o_vec;  // q / out rows start on 16-byte boundaries
+};
+
+// kChunks: 64-dim halves of a head (1: head_dim 64, 2: up to 128).
+template <typename T, bool kDual, int kChunks>
+__global__ void __maxnreg__(96)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map, const TreeKernelParams kp) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  using L = Layout<kDual>;
+  constexpr int kVStages = L::kVStages;
+  constexpr uint32_t kLoadBytes = kChunks * kChunkBytes;
+  const ChunkParams& P = kp.c;
+  const AttentionParams& p = P.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Shared* sh = reinterpret_cast<Shared*>(smem + L::kShared);
+  int32_t* err = p.error_word;
+  volatile int* abort = &sh->abort;
+
+  if (threadIdx.x == kProducerWarp * 32) {
+    sh->abort = 0;
+    sh->fix = 0;
+    mbar_init(&sh->q_full, kSoftmaxThreads);
+    for (int s = 0; s < kKStages; ++s) mbar_init(&sh->k_full[s], 1), mbar_init(&sh->k_empty[s], 1);
+    for (int s = 0; s < kVStages; ++s) mbar_init(&sh->v_full[s], 1), mbar_init(&sh->v_empty[s], 1);
+    for (int x = 0; x < 2; ++x) mbar_init(&sh->s_full[x], 1), mbar_init(&sh->p_full[x], kSoftmaxThreads / 2);
+    mbar_init(&sh->o_done, 1);
+    mbar_init(&sh->drain, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  if (warp == 0) {
+    tmem_alloc(&sh->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  chunk_find_start<kThreads>(P, blockIdx.x, P.ctas, sh->sums, &sh->start);  // ends with a barrier
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const uint32_t smem_base = smem_u32(smem);
+  ChunkWalk walk(P, sh->start, blockIdx.x, P.ctas);
+  ChunkSegment seg;
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      // an earlier CTA's wait gave up: load nothing, every tile counts as refused
+      const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
+      const int page_mask = (1 << p.page_shift) - 1;
+      int n = 0;  // tiles so far
+      while (walk.next(P, seg)) {
+        const int32_t* table = chunk_table(P, seg.b, seg.g);
+        const int plane = p.layer * p.num_kv_heads + seg.g;
+        auto pool_row = [&](int tile) {
+          const int tok = tile * kKeys;
+          const int32_t page = table[tok >> p.page_shift];
+          return page < 0 || page >= p.num_pages ? -1 : (page << p.page_shift) + (tok & page_mask);
+        };
+        for (int tile = seg.k_lo; tile < seg.k_hi; ++tile, ++n) {
+          int row = -1;
+          if (!seg.refused && !dead) {
+            row = pool_row(tile);
+            if (row < 0) flag_error(err, HYT_DEVERR_PAGE_RANGE);
+            if (tile + kPrefetchTiles < seg.k_hi) {
+              const int ahead = pool_row(tile + kPrefetchTiles);
+              if (ahead >= 0) {
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                  tma_prefetch_l2_3d(&k_map, c * 64, ahead, plane);
+                  tma_prefetch_l2_3d(&v_map, c * 64, ahead, plane);
+                }
+              }
+            }
+          }
+          const int ks = n % kKStages, vs = n % kVStages;
+          if (n >= kKStages) mbar_wait(&sh->k_empty[ks], (n / kKStages - 1) & 1, err, abort);
+          if (*abort) row = -1;
+          sh->refused[n & 7] = row < 0;
+          if (row >= 0) {
+            uint8_t* dst = smem + L::kK + ks * kTileBytes;
+            mbar_arrive_expect_tx(&sh->k_full[ks], kLoadBytes);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunkBytes, &k_map, &sh->k_full[ks], c * 64, row, plane);
+          } else {
+            mbar_arrive(&sh->k_full[ks]);
+          }
+          if (n >= kVStages) mbar_wait(&sh->v_empty[vs], (n / kVStages - 1) & 1, err, abort);
+          if (row >= 0 && !*abort) {
+            uint8_t* dst = smem + L::kV + vs * kTileBytes;
+            mbar_arrive_expect_tx(&sh->v_full[vs], kLoadBytes);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) tma_load_3d(dst + c * kChunkBytes, &v_map, &sh->v_full[vs], c * 64, row, plane);
+          } else {
+            mbar_arrive(&sh->v_full[vs]);
+          }
+        }
+      }
+      // nothing in flight when the CTA exits
+      for (int i = max(0, n - kKStages); i < n; ++i) mbar_drain(&sh->k_full[i % kKStages], (i / kKStages) & 1);
+      for (int i = max(0, n - kVStages); i < n; ++i) mbar_drain(&sh->v_full[i % kVStages], (i / kVStages) & 1);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    // The whole warp walks and waits; each group of MMAs and its commits is issued by the
+    // lane elect.sync picks (checked to be lane 0, so every commit covers what came before).
+    constexpr uint32_t idesc_qk = umma_idesc_f16(kBf16, 128, 128, false, false);
+    constexpr uint32_t idesc_pv = umma_idesc_f16(kBf16, 128, kChunks * 64, false, true);
+    const uint64_t q_desc = umma_desc_sw128(smem_base + L::kQ, 16);
+    const uint32_t hi = uint32_t(q_desc >> 32);
+    const uint32_t q_lo = uint32_t(q_desc);
+    const uint32_t k_lo = uint32_t(umma_desc_sw128(smem_base + L::kK, 16));
+    const uint32_t v_lo = uint32_t(umma_desc_sw128(smem_base + L::kV, kChunkBytes));
+    constexpr uint32_t kStep = kTileBytes >> 4;  // descriptor units from stage to stage
+    auto single_lane = [&]() {
+      if (__activemask() != (1u << lane) || lane != 0) {
+        flag_error(err, HYT_DEVERR_ISSUE_LANE);
+        return false;
+      }
+      return true;
+    };
+    auto qk = [&](int x, int q_block, int stage) {
+      const uint32_t a0 = q_lo + q_block * kStep, b0 = k_lo + stage * kStep;
+#pragma unroll
+      for (int kk = 0; kk < 4 * kChunks; ++kk) {
+        const uint32_t off = uint32_t(((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4);
+        umma_f16_ss_lh(tmem + x * 128, a0 + off, hi, b0 + off, hi, idesc_qk, kk > 0 ? 1u : 0u);
+      }
+      umma_commit(&sh->s_full[x]);
+    };
+    auto pv = [&](int x, int stage, bool accumulate) {
+      const uint32_t b0 = v_lo + stage * kStep;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        umma_f16_ts_lh(tmem + kOCol + x * 128, tmem + x * 128 + kk * 8, b0 + uint32_t((kk * 2048) >> 4), hi, idesc_pv,
+                       (kk > 0 || accumulate) ? 1u : 0u);
+    };
+    int n0 = 0, segs = 0;       // tiles and segments before this one
+    uint32_t pc[2] = {0u, 0u};  // P tiles taken so far, per stream
+    auto wait_k = [&](int i) { mbar_wait(&sh->k_full[i % kKStages], (i / kKStages) & 1, err, abort); };
+    auto wait_v = [&](int i) { mbar_wait(&sh->v_full[i % kVStages], (i / kVStages) & 1, err, abort); };
+    while (walk.next(P, seg)) {
+      const int n = seg.k_hi - seg.k_lo;
+      mbar_wait(&sh->q_full, segs & 1, err, abort);
+      if constexpr (!kDual) {
+        for (int s = 0; s < min(n, 2); ++s) {
+          wait_k(n0 + s);
+          if (elect_one() && single_lane()) {
+            tc_fence_after();
+            qk(s, 0, (n0 + s) % kKStages);
+            umma_commit(&sh->k_empty[(n0 + s) % kKStages]);
+          }
+          __syncwarp();
+        }
+        for (int s = 0; s < n; ++s) {
+          const int x = s & 1;
+          const bool more = s + 2 < n;
+          wait_v(n0 + s);
+          mbar_wait(&sh->p_full[x], pc[x]++ & 1, err, abort);
+          if (more) wait_k(n0 + s + 2);
+          if (elect_one() && single_lane()) {
+            tc_fence_after();
+            pv(x, (n0 + s) % kVStages, s >= 2);
+            umma_commit(&sh->v_empty[(n0 + s) % kVStages]);
+            if (more) {
+              qk(x, 0, (n0 + s + 2) % kKStages);
+              umma_commit(&sh->k_empty[(n0 + s + 2) % kKStages]);
+            }
+            if (s == n - 1) umma_commit(&sh->o_done);
+          }
+          __syncwarp();
+        }
+      } else {
+        wait_k(n0);
+        if (elect_one() && single_lane()) {
+          tc_fence_after();
+          qk(0, 0, n0 % kKStages);
+          qk(1, 1, n0 % kKStages);
+          umma_commit(&sh->k_empty[n0 % kKStages]);
+        }
+        __syncwarp();
+        for (int j = 0; j < n; ++j) {
+          const bool more = j + 1 < n;
+          const int vs = (n0 + j) % kVStages, ks = (n0 + j + 1) % kKStages;
+          wait_v(n0 + j);
+          mbar_wait(&sh->p_full[0], pc[0]++ & 1, err, abort);
+          if (more) wait_k(n0 + j + 1);
+          if (elect_one() && single_lane()) {
+            tc_fence_after();
+            pv(0, vs, j > 0);
+            if (more) qk(0, 0, ks);
+          }
+          __syncwarp();
+          mbar_wait(&sh->p_full[1], pc[1]++ & 1, err, abort);
+          if (elect_one() && single_lane()) {
+            tc_fence_after();
+            pv(1, vs, j > 0);
+            umma_commit(&sh->v_empty[vs]);
+            if (more) {
+              qk(1, 1, ks);
+              umma_commit(&sh->k_empty[ks]);
+            } else {
+              umma_commit(&sh->o_done);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      n0 += n;
+      ++segs;
+    }
+    if (elect_one() && single_lane()) umma_commit(&sh->drain);  // every MMA done before TMEM is released
+    __syncwarp();
+    mbar_drain(&sh->drain, 0);
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // row of the block == TMEM lane
+    const int block = kDual ? x : 0;    // row block this stream works on
+    const uint32_t lane_addr = tmem + (uint32_t(quarter * 32) << 16);
+    const int pair_bar = 1 + x * 4 + quarter;
+    const float scale_log2 = p.scale * kLog2e;
+    const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
+    const uint32_t s_addr = lane_addr + x * 128 + half * 64;
+    const uint32_t p_addr = lane_addr + x * 128 + half * 32;
+    const uint32_t o_addr = lane_addr + kOCol + x * 128 + half * (kChunks * 32);
+    const int D = p.head_dim;
+    int n0 = 0, segs = 0;
+    uint32_t sc = 0;  // S tiles taken so far by this stream
+
+    while (walk.next(P, seg)) {
+      const int n = seg.k_hi - seg.k_lo;
+      const int rows_left = seg.queries * P.group - seg.row0;  // may exceed the unit's rows
+      // ---- Q rows into shared memory (free: the previous segment's MMAs are all done)
+      {
+        constexpr int kBlocks = kDual ? 2 : 1;
+        constexpr int kPerThread = kBlocks * kRows * kChunks * 8 / kSoftmaxThreads;
+        uint4 v[kPerThread];
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+          const int idx = i * kSoftmaxThreads + int(threadIdx.x);  // (row, 16-byte chunk)
+          const int c = idx % (kChunks * 8), qr = idx / (kChunks * 8);
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (qr < rows_left && c * 8 < D) {
+            const T* src = static_cast<const T*>(p.q) + chunk_q_offset(P, seg.b, seg.g, seg.row0 + qr) + c * 8;
+            if (kp.q_vec) {
+              v[i] = __ldg(reinterpret_cast<const uint4*>(src));
+            } else {
+              const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+              v[i].x = e[0] | (uint32_t(e[1]) << 16);
+              v[i].y = e[2] | (uint32_t(e[3]) << 16);
+              v[i].z = e[4] | (uint32_t(e[5]) << 16);
+              v[i].w = e[6] | (uint32_t(e[7]) << 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+          const int idx = i * kSoftmaxThreads + int(threadIdx.x);
+          const int c = idx % (kChunks * 8), qr = idx / (kChunks * 8);
+          *reinterpret_cast<uint4*>(smem + L::kQ + (qr >> 7) * kTileBytes + sw128_offset(qr & (kRows - 1), c)) = v[i];
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&sh->q_full);
+      }
+
+      const int my_rows = rows_left - block * kRows;
+      const bool active = quarter * 32 < my_rows;  // warp-uniform: some of the warp's rows exist
+      const int t = min((seg.row0 + block * kRows + r) / P.group, seg.queries - 1);
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = kDual ? 0 : x; i < n; i += kDual ? 1 : 2, ++sc) {
+        mbar_wait(&sh->s_full[x], sc & 1, err, abort);
+        tc_fence_after();
+        const int k0 = (seg.k_lo + i) * kKeys;
+        const bool none = seg.refused || *reinterpret_cast<volatile int32_t*>(&sh->refused[(n0 + i) & 7]) != 0;
+        const bool masked = none || k0 + kKeys > seg.len;
+        if (masked && (!kDual || x == 0)) {
+          // values that are not finite among the rows past the cached tokens
+          const int vi = n0 + i, v0 = none ? 0 : max(seg.len - k0, 0);
+          mbar_wait(&sh->v_full[vi % kVStages], (vi / kVStages) & 1, err, abort);
+          uint8_t* tile = smem + L::kV + (vi % kVStages) * kTileBytes;
+          constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+          for (int idx = int(threadIdx.x) & 255; idx < (kKeys - v0) * kChunks * 8; idx += 256) {
+            const int vr = v0 + idx / (kChunks * 8), c = idx % (kChunks * 8);
+            uint4* at = reinterpret_cast<uint4*>(tile + sw128_offset(vr, c));
+            const uint4 raw = *at;
+            uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((w[e] & kExp) == kExp) w[e] &= 0xFFFF0000u, bad = true;
+              if ((w[e] & (kExp << 16)) == (kExp << 16)) w[e] &= 0x0000FFFFu, bad = true;
+            }
+            if (bad) {
+              *at = make_uint4(w[0], w[1], w[2], w[3]);
+              if (!none && k0 + vr < seg.kv) *reinterpret_cast<volatile int32_t*>(&sh->fix) = 1;
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (active) {
+          float s[64];
+          {
+            uint32_t raw[2][32];
+            tmem_ld32(s_addr, raw[0]);
+            tmem_ld32(s_addr + 32, raw[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(raw[c][e]);
+          }
+          if (masked) {
+            const uint64_t seen = none || r >= my_rows
+                                      ? 0ull
+                                      : chunk_visible64(P, seg.b, t, seg.queries, k0 + half * 64 - seg.len);
+            const uint32_t seen_lo = uint32_t(seen), seen_hi = uint32_t(seen >> 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              if (!((seen_lo >> c) & 1u)) s[c] = -INFINITY;
+              if (!((seen_hi >> c) & 1u)) s[32 + c] = -INFINITY;
+            }
+          }
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            mx0 = fmax3(mx0, s[c], s[c + 1]);
+            mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+          }
+          float(*slot)[kRows] = sh->max[x][sc & 1];
+          slot[half][r] = fmaxf(mx0, mx1);
+          named_bar_sync(pair_bar, 64);
+          const float m_tile = fmaxf(slot[0][r], slot[1][r]) * scale_log2;
+          const float m_new = fmaxf(m_run, m_tile);
+          const bool moves = __any_sync(0xffffffffu, m_new > m_run + kRescaleThreshold);
+          float alpha = 1.f;
+          if (moves) {
+            alpha = m_run == -INFINITY ? 0.f : ex2(m_run - m_new);
+            m_run = m_new;
+          }
+          const float tile_sum = exp_tile<T>(s, scale2, m_run == -INFINITY ? 0.f : m_run, p_addr);
+          l_run = l_run * alpha + tile_sum;
+          if (moves && i >= (kDual ? 1 : 2)) {  // O_x is stable: its last PV completed before S_x did
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(o_addr + c * 32, o);
+            }
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&sh->p_full[x]);
+      }
+
+      // ---- epilogue
+      sh->sum[x][half][r] = l_run;
+      if (half == 0) sh->m[x][r] = m_run;
+      mbar_wait(&sh->o_done, segs & 1, err, abort);
+      tc_fence_after();
+      named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
+      __syncwarp();
+      const bool fix = *reinterpret_cast<volatile int32_t*>(&sh->fix) != 0;
+      // one row block: the streams are joined, a quarter of the columns per warp; two: each
+      // stream has its own rows, half of the columns per warp
+      constexpr int kGroups = kDual ? kChunks : 1;  // 32-column groups per warp
+      const int col0 = kDual ? half * (kChunks * 32) : (x * 2 + half) * 32;
+      if (active && col0 < kChunks * 64) {
+        float f0 = 1.f, f1 = 0.f, m = m_run, l;
+        bool use0 = true, use1 = false;
+        uint32_t from = lane_addr + kOCol + (kDual ? x * 128 : 0);
+        if constexpr (kDual) {
+          l = sh->sum[x][0][r] + sh->sum[x][1][r];
+        } else {
+          const float m0 = sh->m[0][r], m1 = sh->m[1][r];
+          const float l0 = sh->sum[0][0][r] + sh->sum[0][1][r], l1 = sh->sum[1][0][r] + sh->sum[1][1][r];
+          m = fmaxf(m0, m1);
+          const float m_use = m == -INFINITY ? 0.f : m;
+          use0 = l0 != 0.f;
+          use1 = l1 != 0.f;  // also false where stream 1 had no tile
+          f0 = use0 ? ex2(m0 - m_use) : 0.f;
+          f1 = use1 ? ex2(m1 - m_use) : 0.f;
+          l = l0 * f0 + l1 * f1;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool mine = r < my_rows;
+        const int unit_row = block * kRows + r;
+        T* out = static_cast<T*>(p.out) +
+                 (mine ? chunk_o_offset(P, seg.b, seg.g, seg.row0 + unit_row) : int64_t(0));
+        const int64_t slot = int64_t(blockIdx.x) * 2 + (seg.first ? 0 : 1);
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) {
+          const int col = col0 + c * 32;
+          float f[32];
+          {
+            uint32_t o[32];
+            tmem_ld32(from + col, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = use0 ? __uint_as_float(o[e]) * f0 : 0.f;
+          }
+          if constexpr (!kDual) {
+            if (n > 1) {  // warp-uniform
+              uint32_t o[32];
+              tmem_ld32(from + 128 + col, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (use1) f[e] = fmaf(__uint_as_float(o[e]), f1, f[e]);
+            }
+          }
+          if (mine) {
+          if (fix) {  // V of the nodes this row sees that were left out because they are not finite
+            const int lo = max(seg.k_lo * kKeys, seg.len), hi_pos = min(seg.k_hi * kKeys, seg.kv);
+            const int32_t* table = chunk_table(P, seg.b, seg.g);
+            for (int pos = lo; pos < hi_pos; ++pos) {
+              if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
+              const int32_t page = table[pos >> p.page_shift];
+              if (page < 0 || page >= p.num_pages) continue;
+              const int64_t vrow = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity +
+                                   (int64_t(page) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (col + e >= D) break;
+                const float v = Elem<T>::to_float(static_cast<const T*>(p.v_pool)[vrow * D + col + e]);
+                if (!isfinite(v)) f[e] += v;
+              }
+            }
+          }
+          if (seg.whole) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              if (col + v * 8 >= D) break;
+              uint4 w;
+              w.x = Elem<T>::pack2(f[8 * v + 0] * inv, f[8 * v + 1] * inv);
+              w.y = Elem<T>::pack2(f[8 * v + 2] * inv, f[8 * v + 3] * inv);
+              w.z = Elem<T>::pack2(f[8 * v + 4] * inv, f[8 * v + 5] * inv);
+              w.w = Elem<T>::pack2(f[8 * v + 6] * inv, f[8 * v + 7] * inv);
+              if (kp.o_vec) {
+                *reinterpret_cast<uint4*>(out + col + v * 8) = w;
+              } else {
+                uint16_t* e = reinterpret_cast<uint16_t*>(out + col + v * 8);
+                e[0] = uint16_t(w.x), e[1] = uint16_t(w.x >> 16), e[2] = uint16_t(w.y), e[3] = uint16_t(w.y >> 16);
+                e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
+              }
+            }
+          } else {
+            float4* wo = chunk_partial_o(P, slot);
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              if (col + v * 4 < D)
+                wo[int64_t(col / 4 + v) * P.unit_rows + unit_row] =
+                    make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+            if (col == 0) chunk_partial_ml(P, slot)[unit_row] = make_float2(m, l);
+          }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      // O, the sums and `fix` have been read by everyone before the next segment writes them
+      named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
+      if (threadIdx.x == 0) sh->fix = 0;
+      n0 += n;
+      ++segs;
+    }
+  }
+
+  // ---- release TMEM once every warp is done with it
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, bool kDual, int kChunks>
+cudaError_t launch_tree(const TreeKernelParams& kp, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                        cudaStream_t stream) {
+  auto kernel = tree_attention_kernel<T, kDual, kChunks>;
+  constexpr int smem = Layout<kDual>::kBytes;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<kp.c.ctas, kThreads, smem, stream>>>(k_map, v_map, kp);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_tree_shape(const TreeKernelParams& kp, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                              cudaStream_t stream) {
+  const bool dual = kp.c.unit_rows > kRows;
+  if (kp.c.a.head_dim <= 64)
+    return dual ? launch_tree<T, true, 1>(kp, k_map, v_map, stream) : launch_tree<T, false, 1>(kp, k_map, v_map, stream);
+  return dual ? launch_tree<T, true, 2>(kp, k_map, v_map, stream) : launch_tree<T, false, 2>(kp, k_map, v_map, stream);
+}
+
+}  // namespace
+
+ChunkShape chunk_shape_tensor(int64_t max_rows, int num_sms) {
+  return {max_rows <= kRows ? kRows : 2 * kRows, kKeys, num_sms};
+}
+
+cudaError_t run_chunk_attention_tensor(const ChunkParams& p, bool q_vec, bool o_vec, const CUtensorMap& k_map,
+                                       const CUtensorMap& v_map, int dtype, cudaStream_t stream) {
+  const TreeKernelParams kp{p, q_vec ? 1 : 0, o_vec ? 1 : 0};
+  return dtype == HYT_DTYPE_F16 ? launch_tree_shape<__half>(kp, k_map, v_map, stream)
+                                : launch_tree_shape<__nv_bfloat16>(kp, k_map, v_map, stream);
+}
+
+}  // namespace hyt

@@ -356,7 +356,7 @@ cudaError_t launch_general(const ChunkParams& p, cudaStream_t stream) {
   static_assert(kRows * (kKeys + 4) <= kKeys * (kChunks * 64 + 4), "P must fit in K's tile");
   auto kernel = chunk_attention_general_kernel<T, kRows, kChunks>;
   constexpr int smem = general_smem<T, kRows, kChunks>();
-  cudaError_t e = allow_smem(kernel, smem, stream);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kernel<<<p.ctas, kThreads, smem, stream>>>(p);
   return cudaGetLastError();
