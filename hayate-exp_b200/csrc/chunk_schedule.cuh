@@ -3,8 +3,8 @@
 // A unit is (request b, KV head g, block of `unit_rows` query rows); rows of a request are
 // numbered t * group + hl (query t, local head hl). A unit streams the request's keys in
 // tiles of `tile_keys`. All units' tiles, request after request, form one line of W tiles;
-// CTA c of G takes tiles [c W / G, (c + 1) W / G): every CTA streams the same number of
-// tiles (+- 1) whatever the lengths, and W needs no host copy of the lengths, so a captured
+// CTA c of G takes W / G of them, the first W % G CTAs one more: every CTA streams the same number
+// of tiles whatever the lengths, and W needs no host copy of the lengths, so a captured
 // launch follows them. A CTA's stretch falls into segments, one per unit it touches. A
 // segment that covers its unit writes the rows; another writes a partial (unnormalised O,
 // running max, sum) to one of the CTA's two slots (slot 0: its first segment, slot 1: its
@@ -28,27 +28,26 @@ struct ChunkRequest {
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& P, int b, int& why) {
   const AttentionParams& p = P.a;
   ChunkRequest r{0, 0, 0, 0, false};
-  int n = p.query_len;
-  if (p.q_start != nullptr) {
-    const int s = p.q_start[b];
-    n = p.q_len[b];
-    if (n < 0 || n > p.query_len || s < 0 || int64_t(s) + n > p.total_tokens) {
-      why |= HYT_DEVERR_PACKED_RANGE;
-      return r;
-    }
+  const bool packed = p.q_start != nullptr;
+  const int len = p.cache_lens[b];  // the loads go out together
+  const int s = packed ? p.q_start[b] : 0;
+  const int n = packed ? p.q_len[b] : p.query_len;
+  if (packed && (n < 0 || n > p.query_len || s < 0 || int64_t(s) + n > p.total_tokens)) {
+    why |= HYT_DEVERR_PACKED_RANGE;
+    return r;
   }
   if (n == 0) return r;
-  r.len = p.cache_lens[b];
+  r.len = len;
   r.queries = n;
-  r.row_blocks = int((int64_t(n) * P.group + P.unit_rows - 1) / P.unit_rows);
-  const int64_t kv = int64_t(r.len) + n;
-  if (r.len < 0 || kv > (int64_t(P.table_width) << p.page_shift) || kv > INT32_MAX - 256) {
+  r.row_blocks = int((int64_t(n) * P.group + P.unit_rows - 1) >> P.unit_shift);
+  const int64_t kv = int64_t(len) + n;
+  if (len < 0 || kv > (int64_t(P.table_width) << p.page_shift) || kv > INT32_MAX - 256) {
     why |= HYT_DEVERR_TABLE_RANGE;
     r.refused = true;
     r.tiles = 1;
     return r;
   }
-  r.tiles = int((kv + P.tile_keys - 1) / P.tile_keys);
+  r.tiles = int((kv + P.tile_keys - 1) >> P.tile_shift);
   return r;
 }
 
@@ -58,11 +57,18 @@ __device__ __forceinline__ int64_t chunk_work(const ChunkParams& P, const ChunkR
 
 struct ChunkStart {
   int64_t total;  // W
+  int64_t base;   // W / CTAs, and the remainder: the first `rem` CTAs take one tile more
   int64_t off;    // first tile of the CTA within request b's tiles
+  int rem;
   int b;
+
+  __device__ __forceinline__ int64_t begin(int c) const { return base * c + min(c, rem); }
 };
 
-__device__ __forceinline__ int64_t chunk_begin(int64_t total, int c, int ctas) { return total * c / ctas; }
+// a / b for a >= 0, b > 0; nearly always within 32 bits, where it is several times cheaper
+__device__ __forceinline__ int64_t chunk_div(int64_t a, int b) {
+  return a <= 0xFFFFFFFFll ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
 
 // Where CTA c of `ctas` starts. Called by all kThreads threads; `sums` holds kThreads / 32
 // shared entries. Ends with a barrier.
@@ -92,12 +98,18 @@ __device__ __forceinline__ void chunk_find_start(const ChunkParams& P, int c, in
     if (w < warp) before += sums[w];
     total += sums[w];
   }
-  const int64_t begin = chunk_begin(total, c, ctas);
-  if (tid == 0) start->total = total;
+  const int64_t base = chunk_div(total, ctas);
+  const int rem = int(total - base * ctas);
+  const int64_t begin = base * c + min(c, rem);
+  if (tid == 0) {
+    start->total = total;
+    start->base = base;
+    start->rem = rem;
+  }
   if (begin >= before && begin < before + mine) {  // one thread, if total > 0 and begin < total
     int64_t off = begin - before;
     int b = b0;
-    for (; b < b1; ++b) {
+    for (; b < b1 - 1; ++b) {
       const int64_t w = chunk_work(P, chunk_request(P, b, why));
       if (off < w) break;
       off -= w;
@@ -123,8 +135,9 @@ struct ChunkWalk {
   bool started;
   ChunkRequest r;
 
-  __device__ __forceinline__ ChunkWalk(const ChunkParams& P, const ChunkStart& s, int c, int ctas) {
-    left = chunk_begin(s.total, c + 1, ctas) - chunk_begin(s.total, c, ctas);
+  ChunkWalk() = default;
+  __device__ __forceinline__ ChunkWalk(const ChunkParams& P, const ChunkStart& s, int c) {
+    left = s.begin(c + 1) - s.begin(c);
     off = s.off;
     b = s.b;
     started = false;
@@ -143,9 +156,9 @@ struct ChunkWalk {
       ++b;
       load(P);
     }
-    const int64_t unit = off / r.tiles;
+    const int64_t unit = chunk_div(off, r.tiles);
     s.b = b;
-    s.g = int(unit / r.row_blocks);
+    s.g = int(chunk_div(unit, r.row_blocks));
     s.row0 = int(unit - int64_t(s.g) * r.row_blocks) * P.unit_rows;
     s.len = r.len;
     s.queries = r.queries;
@@ -163,15 +176,22 @@ struct ChunkWalk {
   }
 };
 
-// Element offset of row `row` (t * group + hl) of request b, head group g, in q or out.
-__device__ __forceinline__ int64_t chunk_q_offset(const ChunkParams& P, int b, int g, int row) {
-  const int t = row / P.group, hl = row - t * P.group;
-  return att_q_row(P.a, b, t) + int64_t(g * P.group + hl) * P.a.q_sh;
-}
-__device__ __forceinline__ int64_t chunk_o_offset(const ChunkParams& P, int b, int g, int row) {
-  const int t = row / P.group, hl = row - t * P.group;
-  return att_o_row(P.a, b, t) + int64_t(g * P.group + hl) * P.a.o_sh;
-}
+// Row `r` of a unit whose first row is row0: query t and local head hl. row0 / group is the
+// same for every row of the unit; r is small, so its division is a 16-bit multiplication
+// (group_magic = ceil(2^20 / group), exact for (group - 1) + r < 1024 and group < 1024).
+struct ChunkRows {
+  int t0, hl0;  // query and local head of row0
+  __device__ __forceinline__ ChunkRows(const ChunkParams& P, int row0) {
+    t0 = row0 / P.group;
+    hl0 = row0 - t0 * P.group;
+  }
+  __device__ __forceinline__ void at(const ChunkParams& P, int r, int& t, int& hl) const {
+    const int x = hl0 + r;
+    const int dt = P.group < 512 ? int((uint32_t(x) * P.group_magic) >> 20) : x / P.group;
+    t = t0 + dt;
+    hl = x - dt * P.group;
+  }
+};
 
 // Page table row that request b's KV head g walks.
 __device__ __forceinline__ const int32_t* chunk_table(const ChunkParams& P, int b, int g) {

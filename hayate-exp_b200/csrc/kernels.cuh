@@ -188,7 +188,9 @@ struct ChunkParams {
   int32_t table_head_stride;  // 0, or entries between two KV heads' rows of one request
   const int32_t* mask;        // [token rows, mask_words] visibility bits of the chunk's nodes; null: causal
   int32_t mask_words;
-  int32_t unit_rows, tile_keys;  // work units (chunk_schedule.cuh)
+  int32_t unit_rows, tile_keys;  // work units (chunk_schedule.cuh): powers of two
+  int32_t unit_shift, tile_shift;
+  uint32_t group_magic;          // ceil(2^20 / group)
   int32_t ctas;
   float* ws_o;   // [ctas, 2 slots, head_dim / 4, unit_rows, 4] f32
   float* ws_ml;  // [ctas, 2 slots, unit_rows, 2] f32

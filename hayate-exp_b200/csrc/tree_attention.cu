@@ -15,9 +15,11 @@
 //     i % 2 == x, both with the same Q, and the two online softmaxes are joined at the end;
 //   two row blocks (kDual true): stream x is row block x, both see every tile, so a K/V tile
 //     brought into shared memory serves 256 rows.
-// 576 threads: warps 0-7 softmax of stream 0, 8-15 of stream 1 (in a stream, warps w and
+// 640 threads: warps 0-7 softmax of stream 0, 8-15 of stream 1 (in a stream, warps w and
 // w + 4 own rows 32 (w % 4) .. and half of the 128 key columns each), warp 16 the TMA
-// producer, warp 17 the MMA issuer. Per tile, S = Q K^T (shared x shared), P goes back over
+// producer, which also walks the CTA's segments and hands them to the others through a
+// shared ring, warp 17 the MMA issuer, warps 18-19 load the next segment's Q rows as soon
+// as the last S of the one before is done. Per tile, S = Q K^T (shared x shared), P goes back over
 // S's columns as 16-bit pairs, O += P V (TMEM x shared). Issue order PV(s), QK(s + 2).
 // TMEM (512 columns): S_0/P_0 [0,128), S_1/P_1 [128,256), O_0 [256,384), O_1 [384,512).
 // Shared memory: Q 32 KB per row block, 2 K stages, 3 (one row block) or 2 V stages of 32 KB.
@@ -44,7 +46,9 @@ constexpr int kKeys = 128;
 constexpr int kSoftmaxThreads = 512;
 constexpr int kProducerWarp = 16, kMmaWarp = 17;
 constexpr int kSoftmaxBar = 9;  // named barrier of all softmax warps (1 .. 8: row-quarter pairs)
-constexpr int kThreads = 576;
+constexpr int kQWarp = 18, kQThreads = 64;
+constexpr int kThreads = 640;  // 5 warps of 96 registers per sub-partition
+constexpr int kSegments = 8;   // ring of segments: the producer is at most 5 ahead (V stages + 2)
 constexpr int kTileBytes = kRows * 128 * 2;
 constexpr int kChunkBytes = kTileBytes / 2;  // [128 rows x 64 elements]
 constexpr int kKStages = 2;
@@ -54,16 +58,18 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kPrefetchTiles = 3;
 
 struct Shared {
-  uint64_t q_full;
+  uint64_t q_full, q_empty;
+  uint64_t seg_full[kSegments];
   uint64_t k_full[kKStages], k_empty[kKStages], v_full[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
   uint64_t o_done, drain;
   uint32_t tmem_base;
   int32_t abort;       // a bounded wait gave up: later waits return at once
-  int32_t fix;         // a drafted node's V is not finite
+  int32_t fix[2];      // a drafted node's V is not finite, per segment parity
   int32_t refused[8];  // per tile (ring): page refused, nothing of the tile is visible
   ChunkStart start;
   int64_t sums[kThreads / 32];
+  ChunkSegment seg[kSegments];  // segment i in entry i % kSegments; no tiles: the end
   float m[2][kRows];         // running maxima of the streams (joined at the end)
   float sum[2][2][kRows];    // [stream][column half][row]
   float max[2][2][2][kRows]; // [stream][parity][column half][row]
@@ -114,6 +120,15 @@ __device__ __forceinline__ float exp_tile(const float (&s)[64], uint64_t scale2,
   return (sa0 + sb0) + (sa1 + sb1);
 }
 
+template <int kStages>
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) stage = 0, phase ^= 1u;
+  }
+};
+
 struct TreeKernelParams {
   ChunkParams c;
   int32_t q_vec, o_vec;  // q / out rows start on 16-byte boundaries
@@ -140,8 +155,10 @@ __global__ void __maxnreg__(96)
 
   if (threadIdx.x == kProducerWarp * 32) {
     sh->abort = 0;
-    sh->fix = 0;
-    mbar_init(&sh->q_full, kSoftmaxThreads);
+    sh->fix[0] = sh->fix[1] = 0;
+    mbar_init(&sh->q_full, kQThreads);
+    mbar_init(&sh->q_empty, 1);
+    for (int s = 0; s < kSegments; ++s) mbar_init(&sh->seg_full[s], 1);
     for (int s = 0; s < kKStages; ++s) mbar_init(&sh->k_full[s], 1), mbar_init(&sh->k_empty[s], 1);
     for (int s = 0; s < kVStages; ++s) mbar_init(&sh->v_full[s], 1), mbar_init(&sh->v_empty[s], 1);
     for (int x = 0; x < 2; ++x) mbar_init(&sh->s_full[x], 1), mbar_init(&sh->p_full[x], kSoftmaxThreads / 2);
@@ -161,17 +178,30 @@ __global__ void __maxnreg__(96)
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
   const uint32_t smem_base = smem_u32(smem);
-  ChunkWalk walk(P, sh->start, blockIdx.x, P.ctas);
-  ChunkSegment seg;
+  // segment i of the CTA, once the producer has published it; null past the last (or once a
+  // wait gave up)
+  auto segment = [&](int i) -> const ChunkSegment* {
+    if (!mbar_wait(&sh->seg_full[i % kSegments], (i / kSegments) & 1, err, abort)) return nullptr;
+    const ChunkSegment* seg = &sh->seg[i % kSegments];
+    return seg->k_hi > seg->k_lo ? seg : nullptr;
+  };
+  launch_dependents();  // the merge kernel may start up; it waits for this grid's results
 
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
+      ChunkWalk walk(P, sh->start, blockIdx.x);
       // an earlier CTA's wait gave up: load nothing, every tile counts as refused
       const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
       const int page_mask = (1 << p.page_shift) - 1;
       int n = 0;  // tiles so far
-      while (walk.next(P, seg)) {
+      for (int i = 0;; ++i) {
+        ChunkSegment seg;
+        seg.k_lo = seg.k_hi = 0;
+        const bool any = walk.next(P, seg);
+        sh->seg[i % kSegments] = seg;
+        mbar_arrive(&sh->seg_full[i % kSegments]);
+        if (!any) break;
         const int32_t* table = chunk_table(P, seg.b, seg.g);
         const int plane = p.layer * p.num_kv_heads + seg.g;
         auto pool_row = [&](int tile) {
@@ -225,7 +255,7 @@ __global__ void __maxnreg__(96)
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp walks and waits; each group of MMAs and its commits is issued by the
-    // lane elect.sync picks (checked to be lane 0, so every commit covers what came before).
+    // lane elect.sync picks.
     constexpr uint32_t idesc_qk = umma_idesc_f16(kBf16, 128, 128, false, false);
     constexpr uint32_t idesc_pv = umma_idesc_f16(kBf16, 128, kChunks * 64, false, true);
     const uint64_t q_desc = umma_desc_sw128(smem_base + L::kQ, 16);
@@ -234,12 +264,17 @@ __global__ void __maxnreg__(96)
     const uint32_t k_lo = uint32_t(umma_desc_sw128(smem_base + L::kK, 16));
     const uint32_t v_lo = uint32_t(umma_desc_sw128(smem_base + L::kV, kChunkBytes));
     constexpr uint32_t kStep = kTileBytes >> 4;  // descriptor units from stage to stage
-    auto single_lane = [&]() {
-      if (__activemask() != (1u << lane) || lane != 0) {
-        flag_error(err, HYT_DEVERR_ISSUE_LANE);
-        return false;
+    // run f on the elected lane (checked to be lane 0: every commit covers what came before)
+    auto issue = [&](auto&& f) {
+      if (elect_one()) {
+        if (__activemask() == (1u << lane) && lane == 0) {
+          tc_fence_after();
+          f();
+        } else {
+          flag_error(err, HYT_DEVERR_ISSUE_LANE);
+        }
       }
-      return true;
+      __syncwarp();
     };
     auto qk = [&](int x, int q_block, int stage) {
       const uint32_t a0 = q_lo + q_block * kStep, b0 = k_lo + stage * kStep;
@@ -257,83 +292,124 @@ __global__ void __maxnreg__(96)
         umma_f16_ts_lh(tmem + kOCol + x * 128, tmem + x * 128 + kk * 8, b0 + uint32_t((kk * 2048) >> 4), hi, idesc_pv,
                        (kk > 0 || accumulate) ? 1u : 0u);
     };
-    int n0 = 0, segs = 0;       // tiles and segments before this one
-    uint32_t pc[2] = {0u, 0u};  // P tiles taken so far, per stream
-    auto wait_k = [&](int i) { mbar_wait(&sh->k_full[i % kKStages], (i / kKStages) & 1, err, abort); };
-    auto wait_v = [&](int i) { mbar_wait(&sh->v_full[i % kVStages], (i / kVStages) & 1, err, abort); };
-    while (walk.next(P, seg)) {
-      const int n = seg.k_hi - seg.k_lo;
-      mbar_wait(&sh->q_full, segs & 1, err, abort);
+    Ring<kKStages> kr;  // next K tile to multiply, next V tile
+    Ring<kVStages> vr;
+    uint32_t p_phase[2] = {0u, 0u}, q_phase = 0u;
+    auto wait_p = [&](int x) {
+      mbar_wait(&sh->p_full[x], p_phase[x], err, abort);
+      p_phase[x] ^= 1u;
+    };
+    for (int i = 0;; ++i) {
+      const ChunkSegment* found = segment(i);
+      if (found == nullptr) break;
+      const int n = found->k_hi - found->k_lo;
+      mbar_wait(&sh->q_full, q_phase, err, abort);
+      q_phase ^= 1u;
       if constexpr (!kDual) {
-        for (int s = 0; s < min(n, 2); ++s) {
-          wait_k(n0 + s);
-          if (elect_one() && single_lane()) {
-            tc_fence_after();
-            qk(s, 0, (n0 + s) % kKStages);
-            umma_commit(&sh->k_empty[(n0 + s) % kKStages]);
-          }
-          __syncwarp();
+        for (int s = 0; s < min(n, 2); ++s, kr.next()) {
+          mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
+          issue([&] {
+            qk(s, 0, kr.stage);
+            umma_commit(&sh->k_empty[kr.stage]);
+            if (s == n - 1) umma_commit(&sh->q_empty);  // no further product reads this Q
+          });
         }
-        for (int s = 0; s < n; ++s) {
+        for (int s = 0; s < n; ++s, vr.next()) {
           const int x = s & 1;
           const bool more = s + 2 < n;
-          wait_v(n0 + s);
-          mbar_wait(&sh->p_full[x], pc[x]++ & 1, err, abort);
-          if (more) wait_k(n0 + s + 2);
-          if (elect_one() && single_lane()) {
-            tc_fence_after();
-            pv(x, (n0 + s) % kVStages, s >= 2);
-            umma_commit(&sh->v_empty[(n0 + s) % kVStages]);
-            if (more) {
-              qk(x, 0, (n0 + s + 2) % kKStages);
-              umma_commit(&sh->k_empty[(n0 + s + 2) % kKStages]);
-            }
-            if (s == n - 1) umma_commit(&sh->o_done);
+          mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
+          wait_p(x);
+          issue([&] {
+            pv(x, vr.stage, s >= 2);
+            umma_commit(&sh->v_empty[vr.stage]);
+            if (!more && s == n - 1) umma_commit(&sh->o_done);
+          });
+          if (more) {
+            mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
+            issue([&] {
+              qk(x, 0, kr.stage);
+              umma_commit(&sh->k_empty[kr.stage]);
+              if (s + 2 == n - 1) umma_commit(&sh->q_empty);
+            });
+            kr.next();
           }
-          __syncwarp();
         }
       } else {
-        wait_k(n0);
-        if (elect_one() && single_lane()) {
-          tc_fence_after();
-          qk(0, 0, n0 % kKStages);
-          qk(1, 1, n0 % kKStages);
-          umma_commit(&sh->k_empty[n0 % kKStages]);
-        }
-        __syncwarp();
-        for (int j = 0; j < n; ++j) {
+        mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
+        issue([&] {
+          qk(0, 0, kr.stage);
+          qk(1, 1, kr.stage);
+          umma_commit(&sh->k_empty[kr.stage]);
+          if (n == 1) umma_commit(&sh->q_empty);  // no further product reads this Q
+        });
+        kr.next();
+        for (int j = 0; j < n; ++j, vr.next()) {
           const bool more = j + 1 < n;
-          const int vs = (n0 + j) % kVStages, ks = (n0 + j + 1) % kKStages;
-          wait_v(n0 + j);
-          mbar_wait(&sh->p_full[0], pc[0]++ & 1, err, abort);
-          if (more) wait_k(n0 + j + 1);
-          if (elect_one() && single_lane()) {
-            tc_fence_after();
-            pv(0, vs, j > 0);
-            if (more) qk(0, 0, ks);
-          }
-          __syncwarp();
-          mbar_wait(&sh->p_full[1], pc[1]++ & 1, err, abort);
-          if (elect_one() && single_lane()) {
-            tc_fence_after();
-            pv(1, vs, j > 0);
-            umma_commit(&sh->v_empty[vs]);
+          mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
+          wait_p(0);
+          if (more) mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
+          issue([&] {
+            pv(0, vr.stage, j > 0);
+            if (more) qk(0, 0, kr.stage);
+          });
+          wait_p(1);
+          issue([&] {
+            pv(1, vr.stage, j > 0);
+            umma_commit(&sh->v_empty[vr.stage]);
             if (more) {
-              qk(1, 1, ks);
-              umma_commit(&sh->k_empty[ks]);
+              qk(1, 1, kr.stage);
+              umma_commit(&sh->k_empty[kr.stage]);
+              if (j + 2 == n) umma_commit(&sh->q_empty);
             } else {
               umma_commit(&sh->o_done);
             }
-          }
-          __syncwarp();
+          });
+          if (more) kr.next();
         }
       }
-      n0 += n;
-      ++segs;
     }
-    if (elect_one() && single_lane()) umma_commit(&sh->drain);  // every MMA done before TMEM is released
-    __syncwarp();
+    issue([&] { umma_commit(&sh->drain); });  // every MMA done before TMEM is released
     mbar_drain(&sh->drain, 0);
+  } else if (warp >= kQWarp) {
+    // ------------------------------------------------------------ Q loaders
+    const int tid = int(threadIdx.x) - kQWarp * 32, D = p.head_dim;
+    constexpr int kRowChunks = kChunks * 8;                         // 16-byte chunks of a padded row
+    constexpr int kEach = (kDual ? 2 : 1) * kRows * kRowChunks / kQThreads;
+    for (int i = 0;; ++i) {
+      const ChunkSegment* found = segment(i);
+      if (found == nullptr) break;
+      const ChunkSegment& seg = *found;
+      const ChunkRows unit(P, seg.row0);
+      const int rows = seg.queries * P.group - seg.row0;
+      const int c = tid % kRowChunks;
+      const T* base = static_cast<const T*>(p.q) + att_q_row(p, seg.b, 0) + int64_t(seg.g) * P.group * p.q_sh + c * 8;
+      if (i > 0) mbar_wait(&sh->q_empty, (i - 1) & 1, err, abort);
+#pragma unroll 4
+      for (int u = 0; u < kEach; ++u) {
+        const int qr = (u * kQThreads + tid) / kRowChunks;
+        const bool there = qr < rows && c * 8 < D;
+        int t, hl;
+        unit.at(P, there ? qr : 0, t, hl);
+        const T* src = base + int64_t(t) * p.q_st + int64_t(hl) * p.q_sh;
+        uint8_t* dst = smem + L::kQ + (qr >> 7) * kTileBytes + sw128_offset(qr & (kRows - 1), c);
+        if (kp.q_vec) {
+          cp_async16(dst, there ? src : static_cast<const T*>(p.q), there ? 16 : 0);  // 0: zeros
+        } else {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (there) {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+            v.x = e[0] | (uint32_t(e[1]) << 16);
+            v.y = e[2] | (uint32_t(e[3]) << 16);
+            v.z = e[4] | (uint32_t(e[5]) << 16);
+            v.w = e[6] | (uint32_t(e[7]) << 16);
+          }
+          *reinterpret_cast<uint4*>(dst) = v;
+        }
+      }
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      mbar_arrive(&sh->q_full);
+    }
   } else {
     // ------------------------------------------------------------ softmax warps
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
@@ -350,45 +426,18 @@ __global__ void __maxnreg__(96)
     int n0 = 0, segs = 0;
     uint32_t sc = 0;  // S tiles taken so far by this stream
 
-    while (walk.next(P, seg)) {
+    for (;;) {
+      const ChunkSegment* found = segment(segs);
+      if (found == nullptr) break;
+      const ChunkSegment& seg = *found;
       const int n = seg.k_hi - seg.k_lo;
       const int rows_left = seg.queries * P.group - seg.row0;  // may exceed the unit's rows
-      // ---- Q rows into shared memory (free: the previous segment's MMAs are all done)
-      {
-        constexpr int kBlocks = kDual ? 2 : 1;
-        constexpr int kPerThread = kBlocks * kRows * kChunks * 8 / kSoftmaxThreads;
-        uint4 v[kPerThread];
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-          const int idx = i * kSoftmaxThreads + int(threadIdx.x);  // (row, 16-byte chunk)
-          const int c = idx % (kChunks * 8), qr = idx / (kChunks * 8);
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (qr < rows_left && c * 8 < D) {
-            const T* src = static_cast<const T*>(p.q) + chunk_q_offset(P, seg.b, seg.g, seg.row0 + qr) + c * 8;
-            if (kp.q_vec) {
-              v[i] = __ldg(reinterpret_cast<const uint4*>(src));
-            } else {
-              const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
-              v[i].x = e[0] | (uint32_t(e[1]) << 16);
-              v[i].y = e[2] | (uint32_t(e[3]) << 16);
-              v[i].z = e[4] | (uint32_t(e[5]) << 16);
-              v[i].w = e[6] | (uint32_t(e[7]) << 16);
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-          const int idx = i * kSoftmaxThreads + int(threadIdx.x);
-          const int c = idx % (kChunks * 8), qr = idx / (kChunks * 8);
-          *reinterpret_cast<uint4*>(smem + L::kQ + (qr >> 7) * kTileBytes + sw128_offset(qr & (kRows - 1), c)) = v[i];
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&sh->q_full);
-      }
-
+      const ChunkRows unit(P, seg.row0);
       const int my_rows = rows_left - block * kRows;
       const bool active = quarter * 32 < my_rows;  // warp-uniform: some of the warp's rows exist
-      const int t = min((seg.row0 + block * kRows + r) / P.group, seg.queries - 1);
+      int t, hl;
+      unit.at(P, block * kRows + r, t, hl);
+      t = min(t, seg.queries - 1);
       float m_run = -INFINITY, l_run = 0.f;
       for (int i = kDual ? 0 : x; i < n; i += kDual ? 1 : 2, ++sc) {
         mbar_wait(&sh->s_full[x], sc & 1, err, abort);
@@ -415,7 +464,7 @@ __global__ void __maxnreg__(96)
             }
             if (bad) {
               *at = make_uint4(w[0], w[1], w[2], w[3]);
-              if (!none && k0 + vr < seg.kv) *reinterpret_cast<volatile int32_t*>(&sh->fix) = 1;
+              if (!none && k0 + vr < seg.kv) *reinterpret_cast<volatile int32_t*>(&sh->fix[segs & 1]) = 1;
             }
           }
           fence_proxy_async_smem();
@@ -487,7 +536,7 @@ __global__ void __maxnreg__(96)
       tc_fence_after();
       named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
       __syncwarp();
-      const bool fix = *reinterpret_cast<volatile int32_t*>(&sh->fix) != 0;
+      const bool fix = *reinterpret_cast<volatile int32_t*>(&sh->fix[segs & 1]) != 0;
       // one row block: the streams are joined, a quarter of the columns per warp; two: each
       // stream has its own rows, half of the columns per warp
       constexpr int kGroups = kDual ? kChunks : 1;  // 32-column groups per warp
@@ -513,7 +562,7 @@ __global__ void __maxnreg__(96)
         const bool mine = r < my_rows;
         const int unit_row = block * kRows + r;
         T* out = static_cast<T*>(p.out) +
-                 (mine ? chunk_o_offset(P, seg.b, seg.g, seg.row0 + unit_row) : int64_t(0));
+                 (mine ? att_o_row(p, seg.b, t) + int64_t(seg.g * P.group + hl) * p.o_sh : int64_t(0));
         const int64_t slot = int64_t(blockIdx.x) * 2 + (seg.first ? 0 : 1);
 #pragma unroll
         for (int c = 0; c < kGroups; ++c) {
@@ -585,9 +634,10 @@ __global__ void __maxnreg__(96)
         }
       }
       tc_fence_before();
-      // O, the sums and `fix` have been read by everyone before the next segment writes them
+      // O, the sums and this segment's `fix` have been read by everyone (the entry's next user
+      // is two segments on, after another of these barriers)
       named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
-      if (threadIdx.x == 0) sh->fix = 0;
+      if (threadIdx.x == 0) sh->fix[segs & 1] = 0;
       n0 += n;
       ++segs;
     }

@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
   __shared__ int nonfinite;        // a drafted node's V is not finite
 
   chunk_find_start<kThreads>(P, blockIdx.x, P.ctas, sums, &start);
-  ChunkWalk walk(P, start, blockIdx.x, P.ctas);
+  launch_dependents();  // the merge kernel may start up; it waits for this grid's results
+  ChunkWalk walk(P, start, blockIdx.x);
   ChunkSegment seg;
   const float scale_log2 = p.scale * kLog2e;
   const int page_mask = (1 << p.page_shift) - 1;
@@ -81,13 +82,21 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
     const T* kp = static_cast<const T*>(p.k_pool) + plane * D;
     const T* vp = static_cast<const T*>(p.v_pool) + plane * D;
 
+    const ChunkRows unit(P, seg.row0);
+    auto row_at = [&](int r, int64_t head_stride) {  // query of row r, and its head's offset
+      int t, hl;
+      unit.at(P, r, t, hl);
+      return longlong2{t, int64_t(seg.g * P.group + hl) * head_stride};
+    };
     __syncthreads();  // the previous segment's shared tiles are done with
     if (tid == 0) nonfinite = 0;
     for (int i = tid; i < kRows * kD; i += kThreads) {
       const int r = i / kD, d = i - r * kD;
       float v = 0.f;
-      if (r < rows_left && d < D)
-        v = Elem<T>::to_float(static_cast<const T*>(p.q)[chunk_q_offset(P, seg.b, seg.g, seg.row0 + r) + d]);
+      if (r < rows_left && d < D) {
+        const longlong2 at = row_at(r, p.q_sh);
+        v = Elem<T>::to_float(static_cast<const T*>(p.q)[att_q_row(p, seg.b, int(at.x)) + at.y + d]);
+      }
       qs[r * kLd + d] = v;
     }
 
@@ -175,7 +184,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
         if (page < 0 || row >= rows_left)
           seen = 0ull;
         else if (k0 + kKeys > seg.len)
-          seen = chunk_visible64(P, seg.b, (seg.row0 + row) / P.group, seg.queries, k0 - seg.len);
+          seen = chunk_visible64(P, seg.b, int(row_at(row, 0).x), seg.queries, k0 - seg.len);
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -240,7 +249,8 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
     for (int i = 0; i < kR; ++i) {
       const int row = ty * kR + i;
       if (row >= rows_left) continue;
-      const int t = (seg.row0 + row) / P.group;
+      const longlong2 at = row_at(row, p.o_sh);
+      const int t = int(at.x);
       if (fix && !seg.refused) {  // non-finite V of the nodes this row sees, left out above
         const int lo = max(seg.k_lo * kKeys, seg.len), hi = min(seg.k_hi * kKeys, seg.kv);
         for (int pos = lo; pos < hi; ++pos) {
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
       }
       if (seg.whole) {
         const float inv = l_run[i] == 0.f ? 0.f : 1.f / l_run[i];
-        T* out = static_cast<T*>(p.out) + chunk_o_offset(P, seg.b, seg.g, seg.row0 + row);
+        T* out = static_cast<T*>(p.out) + att_o_row(p, seg.b, t) + at.y;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -289,57 +299,68 @@ constexpr int kMergeThreads = 256;
 // Boundary c = blockIdx.x + 1 of the work line; the first boundary strictly inside a unit
 // joins that unit's partials: CTA c - 1's last segment (or first, if it starts with the
 // unit) and the first segments of the CTAs from c on. Thread: (row, 4 dims), consecutive
-// threads consecutive rows, as the partials are stored. Fixed order, no atomics.
+// threads consecutive rows, as the partials are stored; four parts' loads at a time. Fixed
+// order, no atomics. Launched while the attention kernel runs (its own start-up reads only
+// the step's lengths) and waits for that kernel's results.
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams P) {
   __shared__ int64_t sums[kMergeThreads / 32];
   __shared__ ChunkStart start;
   const AttentionParams& p = P.a;
-  const int c = int(blockIdx.x) + 1, ctas = P.ctas;
-  chunk_find_start<kMergeThreads>(P, c, ctas, sums, &start);
-  const int64_t total = start.total, begin = chunk_begin(total, c, ctas);
-  if (begin >= total) return;
+  const int c = int(blockIdx.x) + 1;
+  chunk_find_start<kMergeThreads>(P, c, P.ctas, sums, &start);
+  const int64_t begin = start.begin(c);
+  if (begin >= start.total) return;
   int why = 0;
   const ChunkRequest r = chunk_request(P, start.b, why);
-  const int64_t unit = start.off / r.tiles, unit_off = start.off - unit * r.tiles;
+  const int64_t unit = chunk_div(start.off, r.tiles), unit_off = start.off - unit * r.tiles;
   const int64_t unit_begin = begin - unit_off, unit_end = unit_begin + r.tiles;
-  if (unit_off == 0 || chunk_begin(total, c - 1, ctas) > unit_begin) return;
-  const int g = int(unit / r.row_blocks), row0 = int(unit - int64_t(g) * r.row_blocks) * P.unit_rows;
+  const int64_t before = start.begin(c - 1);
+  if (unit_off == 0 || before > unit_begin) return;
+  const int g = int(chunk_div(unit, r.row_blocks));
+  const int row0 = int(unit - int64_t(g) * r.row_blocks) * P.unit_rows;
   const int rows = min(r.queries * P.group - row0, P.unit_rows);
   const int idx = int(blockIdx.y) * kMergeThreads + int(threadIdx.x);
-  const int row = idx % P.unit_rows, d4 = idx / P.unit_rows;
+  const int row = idx & (P.unit_rows - 1), d4 = idx >> P.unit_shift;
   if (row >= rows || d4 * 4 >= p.head_dim) return;
 
-  const int64_t slot0 = int64_t(c - 1) * 2 + (chunk_begin(total, c - 1, ctas) == unit_begin ? 0 : 1);
-  auto covers = [&](int i) {  // CTA i (>= c) holds a part of the unit (it may hold nothing at all)
-    return chunk_begin(total, i, ctas) < chunk_begin(total, i + 1, ctas);
-  };
-#ifdef __CUDA_ARCH__
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-#endif
-  float m = __ldcg(&chunk_partial_ml(P, slot0)[row]).x;
-  for (int i = c; i < ctas && chunk_begin(total, i, ctas) < unit_end; ++i)
-    if (covers(i)) m = fmaxf(m, __ldcg(&chunk_partial_ml(P, int64_t(i) * 2)[row]).x);
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  // part 0: CTA c - 1; part i: CTA c - 1 + i, its first segment (CTAs with no tiles come last)
+  const int64_t slot0 = int64_t(c - 1) * 2 + (before == unit_begin ? 0 : 1);
+  int parts = 1;
+  while (c - 1 + parts < P.ctas && start.begin(c - 1 + parts) < unit_end) ++parts;
+  wait_for_primary();
+  constexpr int kAhead = 4;
+  float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int64_t slot) {
-    const float2 ml = __ldcg(&chunk_partial_ml(P, slot)[row]);
-    const float4 v = __ldcg(&chunk_partial_o(P, slot)[int64_t(d4) * P.unit_rows + row]);
-    if (ml.y == 0.f) return;  // nothing seen in this part
-    const float f = ex2(ml.x - m_use);
-    l = fmaf(ml.y, f, l);
-    o.x = fmaf(v.x, f, o.x);
-    o.y = fmaf(v.y, f, o.y);
-    o.z = fmaf(v.z, f, o.z);
-    o.w = fmaf(v.w, f, o.w);
-  };
-  add(slot0);
-#pragma unroll 4
-  for (int i = c; i < ctas && chunk_begin(total, i, ctas) < unit_end; ++i)
-    if (covers(i)) add(int64_t(i) * 2);
+  for (int i0 = 0; i0 < parts; i0 += kAhead) {
+    float2 ml[kAhead];
+    float4 v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t slot = i0 + u == 0 ? slot0 : int64_t(c - 1 + i0 + u) * 2;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (i0 + u < parts) {
+        ml[u] = __ldcg(&chunk_partial_ml(P, slot)[row]);
+        v[u] = __ldcg(&chunk_partial_o(P, slot)[int64_t(d4) * P.unit_rows + row]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (ml[u].y == 0.f) continue;  // nothing seen in this part
+      const float m_new = fmaxf(m, ml[u].x), m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float f = ex2(ml[u].x - m_use), keep = m == -INFINITY ? 0.f : ex2(m - m_use);
+      l = fmaf(ml[u].y, f, l * keep);
+      o.x = fmaf(v[u].x, f, o.x * keep);
+      o.y = fmaf(v[u].y, f, o.y * keep);
+      o.z = fmaf(v[u].z, f, o.z * keep);
+      o.w = fmaf(v[u].w, f, o.w * keep);
+      m = m_new;
+    }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(p.out) + chunk_o_offset(P, start.b, g, row0 + row) + d4 * 4;
+  int t, hl;
+  ChunkRows(P, row0).at(P, row, t, hl);
+  T* out = static_cast<T*>(p.out) + att_o_row(p, start.b, t) + int64_t(g * P.group + hl) * p.o_sh + d4 * 4;
   out[0] = Elem<T>::from_float(o.x * inv);
   out[1] = Elem<T>::from_float(o.y * inv);
   out[2] = Elem<T>::from_float(o.z * inv);
@@ -401,11 +422,10 @@ cudaError_t run_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t stream
   const int64_t work = int64_t(p.unit_rows) * (p.a.head_dim / 4);
   const dim3 grid(unsigned(p.ctas - 1), unsigned((work + kMergeThreads - 1) / kMergeThreads));
   switch (dtype) {
-    case HYT_DTYPE_BF16: chunk_merge_kernel<__nv_bfloat16><<<grid, kMergeThreads, 0, stream>>>(p); break;
-    case HYT_DTYPE_F16: chunk_merge_kernel<__half><<<grid, kMergeThreads, 0, stream>>>(p); break;
-    default: chunk_merge_kernel<float><<<grid, kMergeThreads, 0, stream>>>(p); break;
+    case HYT_DTYPE_BF16: return launch_after(chunk_merge_kernel<__nv_bfloat16>, grid, kMergeThreads, 0, stream, p);
+    case HYT_DTYPE_F16: return launch_after(chunk_merge_kernel<__half>, grid, kMergeThreads, 0, stream, p);
+    default: return launch_after(chunk_merge_kernel<float>, grid, kMergeThreads, 0, stream, p);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace hyt
