@@ -624,12 +624,14 @@ int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t
                                    : hyt::chunk_shape_general(rows, g.dtype, g.head_dim, kSms);
   c.unit_rows = s.unit_rows;
   c.tile_keys = s.tile_keys;
+  c.unit_cost = s.unit_cost;
   c.unit_shift = log2_int(s.unit_rows);
   c.tile_shift = log2_int(s.tile_keys);
   c.group_magic = uint32_t(((1 << 20) + c.group - 1) / c.group);
   c.ctas = s.ctas;
   c.ws_o = static_cast<float*>(workspace);
   c.ws_ml = c.ws_o + int64_t(s.ctas) * 2 * s.unit_rows * g.head_dim;
+  c.ws_join = reinterpret_cast<hyt::ChunkJoin*>(c.ws_ml + int64_t(s.ctas) * 2 * s.unit_rows * 2);
   cudaError_t err;
   if (tensor) {
     CUtensorMap k_map, v_map;

@@ -2,13 +2,15 @@
 //
 // A unit is (request b, KV head g, block of `unit_rows` query rows); rows of a request are
 // numbered t * group + hl (query t, local head hl). A unit streams the request's keys in
-// tiles of `tile_keys`. All units' tiles, request after request, form one line of W tiles;
-// CTA c of G takes W / G of them, the first W % G CTAs one more: every CTA streams the same number
-// of tiles whatever the lengths, and W needs no host copy of the lengths, so a captured
-// launch follows them. A CTA's stretch falls into segments, one per unit it touches. A
-// segment that covers its unit writes the rows; another writes a partial (unnormalised O,
-// running max, sum) to one of the CTA's two slots (slot 0: its first segment, slot 1: its
-// last; those between are whole), and the merge kernel joins a unit's partials in order.
+// tiles of `tile_keys`, and starting and ending it costs about as much as `unit_cost` tiles.
+// All units, request after request, form one line of W positions: unit_cost for a unit's
+// ends, then its tiles. CTA c of G takes W / G of them, the first W % G CTAs one more: every CTA
+// works about as long whatever the lengths, and W needs no host copy of the lengths, so a
+// captured launch follows them. A CTA's stretch falls into segments, one per unit it has
+// tiles of. A segment that covers its unit writes the rows; another writes a partial
+// (unnormalised O, running max, sum) to one of the CTA's two slots (slot 0: its first segment,
+// slot 1: its last; those between are whole), and the merge kernel joins a unit's partials
+// in order, as the join record of the CTA with the unit's second part says.
 #pragma once
 
 #include "common.cuh"
@@ -51,14 +53,15 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& P, int 
   return r;
 }
 
+// Line positions of a request.
 __device__ __forceinline__ int64_t chunk_work(const ChunkParams& P, const ChunkRequest& r) {
-  return int64_t(P.a.num_kv_heads) * r.row_blocks * r.tiles;
+  return r.tiles == 0 ? 0 : int64_t(P.a.num_kv_heads) * r.row_blocks * (r.tiles + P.unit_cost);
 }
 
 struct ChunkStart {
   int64_t total;  // W
-  int64_t base;   // W / CTAs, and the remainder: the first `rem` CTAs take one tile more
-  int64_t off;    // first tile of the CTA within request b's tiles
+  int64_t base;   // W / CTAs, and the remainder: the first `rem` CTAs take one more
+  int64_t off;    // first position of the CTA within request b's
   int rem;
   int b;
 
@@ -129,13 +132,12 @@ struct ChunkSegment {
 
 // Walks a CTA's segments; every role of the CTA walks the same ones.
 struct ChunkWalk {
-  int64_t left, off;  // tiles left to the CTA; first of them within request b's
+  int64_t left, off;  // positions left to the CTA; first of them within request b's
   int64_t work;
   int b;
   bool started;
   ChunkRequest r;
 
-  ChunkWalk() = default;
   __device__ __forceinline__ ChunkWalk(const ChunkParams& P, const ChunkStart& s, int c) {
     left = s.begin(c + 1) - s.begin(c);
     off = s.off;
@@ -150,31 +152,58 @@ struct ChunkWalk {
     work = chunk_work(P, r);
   }
   __device__ __forceinline__ bool next(const ChunkParams& P, ChunkSegment& s) {
-    if (left <= 0) return false;
-    while (off >= work) {  // the next request that has work (left > 0: there is one)
-      off -= work;
-      ++b;
-      load(P);
+    while (left > 0) {
+      while (off >= work) {  // the next request that has work (left > 0: there is one)
+        off -= work;
+        ++b;
+        load(P);
+      }
+      const int span = r.tiles + P.unit_cost;
+      const int64_t unit = chunk_div(off, span);
+      const int o = int(off - unit * span), n = int(min(int64_t(span - o), left));
+      s.k_lo = max(o - P.unit_cost, 0);
+      s.k_hi = o + n - P.unit_cost;
+      off += n;
+      left -= n;
+      if (s.k_hi <= s.k_lo) continue;  // the stretch ends before the unit's first tile
+      s.b = b;
+      s.g = int(chunk_div(unit, r.row_blocks));
+      s.row0 = int(unit - int64_t(s.g) * r.row_blocks) * P.unit_rows;
+      s.len = r.len;
+      s.queries = r.queries;
+      s.kv = r.refused ? 0 : r.len + r.queries;
+      s.whole = s.k_lo == 0 && s.k_hi == r.tiles;
+      s.refused = r.refused;
+      s.first = !started;
+      started = true;
+      return true;
     }
-    const int64_t unit = chunk_div(off, r.tiles);
-    s.b = b;
-    s.g = int(chunk_div(unit, r.row_blocks));
-    s.row0 = int(unit - int64_t(s.g) * r.row_blocks) * P.unit_rows;
-    s.len = r.len;
-    s.queries = r.queries;
-    s.kv = r.refused ? 0 : r.len + r.queries;
-    s.k_lo = int(off - unit * r.tiles);
-    s.k_hi = int(min(int64_t(r.tiles), s.k_lo + left));
-    s.whole = s.k_lo == 0 && s.k_hi == r.tiles;
-    s.refused = r.refused;
-    s.first = !started;
-    started = true;
-    const int n = s.k_hi - s.k_lo;
-    off += n;
-    left -= n;
-    return true;
+    return false;
   }
 };
+
+// CTA c's join record, written by one thread with the CTA's first segment (null: it has none):
+// if that segment is its unit's second part, what the merge kernel joins; else no rows.
+__device__ __forceinline__ void chunk_write_join(const ChunkParams& P, const ChunkStart& start, int c,
+                                                 const ChunkSegment* seg) {
+  ChunkJoin j{0, 0, 0, 0, 0, 0, 0, 0};
+  if (seg != nullptr && seg->k_lo > 0) {
+    const int64_t begin = start.begin(c), unit_begin = begin - seg->k_lo - P.unit_cost;
+    const int64_t before = start.begin(c - 1);
+    if (before <= unit_begin + P.unit_cost) {  // CTA c - 1 holds the unit's first tile
+      const int64_t kv = seg->refused ? 1 : int64_t(seg->len) + seg->queries;
+      const int64_t unit_end = unit_begin + P.unit_cost + ((kv + P.tile_keys - 1) >> P.tile_shift);
+      j.b = seg->b;
+      j.g = seg->g;
+      j.row0 = seg->row0;
+      j.rows = min(seg->queries * P.group - seg->row0, P.unit_rows);
+      j.slot0 = (c - 1) * 2 + (before >= unit_begin ? 0 : 1);
+      j.parts = 2;
+      while (c - 1 + j.parts < P.ctas && start.begin(c - 1 + j.parts) < unit_end) ++j.parts;
+    }
+  }
+  P.ws_join[c] = j;
+}
 
 // Row `r` of a unit whose first row is row0: query t and local head hl. row0 / group is the
 // same for every row of the unit; r is small, so its division is a 16-bit multiplication

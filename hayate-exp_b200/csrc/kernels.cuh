@@ -181,6 +181,9 @@ cudaError_t run_norm_rope_scatter(const NormRopeParams& p, int dtype, cudaStream
 // Attention of each request's new queries over its cached keys and, as a mask says, over
 // the step's own. `a` is the shared description: packed (a.q_start / a.q_len, q_len 0
 // allowed) or uniform (a.query_len queries each); a.req_ids is not used.
+struct ChunkJoin {  // a unit in parts: CTA c - 1's slot0 and slots 2 (c - 1 + i), i = 1 .. parts - 1
+  int32_t b, g, row0, rows, slot0, parts, pad0, pad1;
+};
 struct ChunkParams {
   AttentionParams a;
   int32_t group;              // query heads per KV head
@@ -190,17 +193,19 @@ struct ChunkParams {
   int32_t mask_words;
   int32_t unit_rows, tile_keys;  // work units (chunk_schedule.cuh): powers of two
   int32_t unit_shift, tile_shift;
+  int32_t unit_cost;             // of a unit's start and end, in tiles
   uint32_t group_magic;          // ceil(2^20 / group)
   int32_t ctas;
   float* ws_o;   // [ctas, 2 slots, head_dim / 4, unit_rows, 4] f32
   float* ws_ml;  // [ctas, 2 slots, unit_rows, 2] f32
+  ChunkJoin* ws_join;  // [ctas]
 };
 // Work-unit shape and CTA count a kernel uses for a problem.
 struct ChunkShape {
-  int32_t unit_rows, tile_keys, ctas;
+  int32_t unit_rows, tile_keys, unit_cost, ctas;
 };
 constexpr int64_t chunk_workspace_bytes(const ChunkShape& s, int64_t head_dim) {
-  return int64_t(s.ctas) * 2 * s.unit_rows * (head_dim + 2) * 4;
+  return int64_t(s.ctas) * (2 * s.unit_rows * (head_dim + 2) * 4 + int64_t(sizeof(ChunkJoin)));
 }
 // Any dtype, head_dim % 8 == 0 and <= 256, pool rows 16-byte aligned.
 ChunkShape chunk_shape_general(int64_t max_rows, int dtype, int head_dim, int num_sms);

@@ -27,9 +27,10 @@
 // up to 64, the second 64-dim half is neither loaded nor multiplied.
 //
 // Masking: scores by selection. V rows of the tiles that reach past the cached tokens are
-// looked through before they are multiplied: values that are not finite become zeros, and
-// those of drafted nodes are added at the end to the rows that see them (0 * inf would
-// be NaN in every row).
+// looked through (by the Q warps, beside the softmax) before they are multiplied: values that
+// are not finite become zeros, and those of drafted nodes are added at the end to the rows
+// that see them (0 * inf would be NaN in every row). A tile whose page was refused is not
+// multiplied.
 //
 // P is rounded to the storage type (the MMA's operand type); scores, running maximum and
 // sum, and O are fp32. The running maximum may lag by up to 2^8 (O / l is exact all the same).
@@ -55,10 +56,12 @@ constexpr int kKStages = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-constexpr int kPrefetchTiles = 3;
+
+constexpr int kUnitCost = 4;
 
 struct Shared {
   uint64_t q_full, q_empty;
+  uint64_t v_check, v_ok;  // V of a tile past the cached tokens: to be looked through; done
   uint64_t seg_full[kSegments];
   uint64_t k_full[kKStages], k_empty[kKStages], v_full[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
@@ -134,11 +137,58 @@ struct TreeKernelParams {
   int32_t q_vec, o_vec;  // q / out rows start on 16-byte boundaries
 };
 
+// The rare paths are kept out of line: the code between two segments is fetched cold (the
+// softmax loop has pushed it out of the instruction cache), so its size is time.
+
+__device__ __noinline__ void store_unaligned16(void* at, uint4 w) {
+  uint16_t* e = static_cast<uint16_t*>(at);
+  e[0] = uint16_t(w.x), e[1] = uint16_t(w.x >> 16), e[2] = uint16_t(w.y), e[3] = uint16_t(w.y >> 16);
+  e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
+}
+
+// The CTA's n-th tile, of segment `seg`: nothing of it is visible, its stages hold something else.
+__device__ __forceinline__ bool tile_refused(const Shared* sh, const ChunkSegment& seg, int n) {
+  return seg.refused || *reinterpret_cast<const volatile int32_t*>(&sh->refused[n & 7]) != 0;
+}
+// First tile of the segment that reaches past the cached tokens: from there on V is checked.
+__device__ __forceinline__ int first_checked(const ChunkSegment& seg) {
+  return seg.refused ? seg.k_hi : max(seg.k_lo, seg.len / kKeys);
+}
+
+// Adds V of the nodes query t sees that were left out because they are not finite to columns
+// [col, col + n) of its row, as just written: to `out`, or to its partial.
+template <typename T>
+__device__ __noinline__ void add_not_finite(const ChunkParams& P, const ChunkSegment& seg, int t, int col, int n,
+                                            T* out, float* partial) {
+  const AttentionParams& p = P.a;
+  const int lo = max(seg.k_lo * kKeys, seg.len), hi = min(seg.k_hi * kKeys, seg.kv);
+  const int32_t* table = chunk_table(P, seg.b, seg.g);
+  for (int pos = lo; pos < hi; ++pos) {
+    if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
+    const int32_t page = table[pos >> p.page_shift];
+    if (page < 0 || page >= p.num_pages) continue;
+    const int64_t vrow = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity +
+                         (int64_t(page) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+    const T* v = static_cast<const T*>(p.v_pool) + vrow * p.head_dim + col;
+    for (int e = 0; e < n; ++e) {
+      const float x = Elem<T>::to_float(v[e]);
+      if (isfinite(x)) continue;
+      if (seg.whole) {
+        out[e] = Elem<T>::from_float(Elem<T>::to_float(out[e]) + x);
+      } else {
+        float* at = partial + int64_t((col + e) / 4) * P.unit_rows * 4 + (e & 3);
+        *at += x;
+      }
+    }
+  }
+}
+
 // kChunks: 64-dim halves of a head (1: head_dim 64, 2: up to 128).
 template <typename T, bool kDual, int kChunks>
 __global__ void __maxnreg__(96)
     tree_attention_kernel(const __grid_constant__ CUtensorMap k_map,
-                          const __grid_constant__ CUtensorMap v_map, const TreeKernelParams kp) {
+                          const __grid_constant__ CUtensorMap v_map,
+                          const __grid_constant__ TreeKernelParams kp) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   using L = Layout<kDual>;
   constexpr int kVStages = L::kVStages;
@@ -158,6 +208,8 @@ __global__ void __maxnreg__(96)
     sh->fix[0] = sh->fix[1] = 0;
     mbar_init(&sh->q_full, kQThreads);
     mbar_init(&sh->q_empty, 1);
+    mbar_init(&sh->v_check, 1);
+    mbar_init(&sh->v_ok, kQThreads);
     for (int s = 0; s < kSegments; ++s) mbar_init(&sh->seg_full[s], 1);
     for (int s = 0; s < kKStages; ++s) mbar_init(&sh->k_full[s], 1), mbar_init(&sh->k_empty[s], 1);
     for (int s = 0; s < kVStages; ++s) mbar_init(&sh->v_full[s], 1), mbar_init(&sh->v_empty[s], 1);
@@ -195,35 +247,26 @@ __global__ void __maxnreg__(96)
       const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
       const int page_mask = (1 << p.page_shift) - 1;
       int n = 0;  // tiles so far
+      auto pool_row = [&](const int32_t* table, int tile) {
+        const int tok = tile * kKeys;
+        const int32_t page = table[tok >> p.page_shift];
+        return page < 0 || page >= p.num_pages ? -1 : (page << p.page_shift) + (tok & page_mask);
+      };
       for (int i = 0;; ++i) {
         ChunkSegment seg;
         seg.k_lo = seg.k_hi = 0;
         const bool any = walk.next(P, seg);
         sh->seg[i % kSegments] = seg;
         mbar_arrive(&sh->seg_full[i % kSegments]);
+        if (i == 0) chunk_write_join(P, sh->start, blockIdx.x, any ? &seg : nullptr);
         if (!any) break;
         const int32_t* table = chunk_table(P, seg.b, seg.g);
         const int plane = p.layer * p.num_kv_heads + seg.g;
-        auto pool_row = [&](int tile) {
-          const int tok = tile * kKeys;
-          const int32_t page = table[tok >> p.page_shift];
-          return page < 0 || page >= p.num_pages ? -1 : (page << p.page_shift) + (tok & page_mask);
-        };
         for (int tile = seg.k_lo; tile < seg.k_hi; ++tile, ++n) {
           int row = -1;
           if (!seg.refused && !dead) {
-            row = pool_row(tile);
+            row = pool_row(table, tile);
             if (row < 0) flag_error(err, HYT_DEVERR_PAGE_RANGE);
-            if (tile + kPrefetchTiles < seg.k_hi) {
-              const int ahead = pool_row(tile + kPrefetchTiles);
-              if (ahead >= 0) {
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                  tma_prefetch_l2_3d(&k_map, c * 64, ahead, plane);
-                  tma_prefetch_l2_3d(&v_map, c * 64, ahead, plane);
-                }
-              }
-            }
           }
           const int ks = n % kKStages, vs = n % kVStages;
           if (n >= kKStages) mbar_wait(&sh->k_empty[ks], (n / kKStages - 1) & 1, err, abort);
@@ -294,15 +337,27 @@ __global__ void __maxnreg__(96)
     };
     Ring<kKStages> kr;  // next K tile to multiply, next V tile
     Ring<kVStages> vr;
-    uint32_t p_phase[2] = {0u, 0u}, q_phase = 0u;
-    auto wait_p = [&](int x) {
+    uint32_t p_phase[2] = {0u, 0u}, q_phase = 0u, ok_phase = 0u;
+    int n0 = 0;  // tiles before this segment
+    // P and V of tile i of the segment (stream x): V in shared memory and, past the cached tokens,
+    // looked through by the checkers, who start as soon as it is there
+    auto wait_pv = [&](const ChunkSegment& seg, int x, int i) {
+      mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
+      const bool check = seg.k_lo + i >= first_checked(seg) && (!kDual || x == 0);
+      if (check && lane == 0) mbar_arrive(&sh->v_check);
       mbar_wait(&sh->p_full[x], p_phase[x], err, abort);
       p_phase[x] ^= 1u;
+      if (check) {
+        mbar_wait(&sh->v_ok, ok_phase, err, abort);
+        ok_phase ^= 1u;
+      }
     };
     for (int i = 0;; ++i) {
       const ChunkSegment* found = segment(i);
       if (found == nullptr) break;
-      const int n = found->k_hi - found->k_lo;
+      const ChunkSegment& seg = *found;
+      const int n = seg.k_hi - seg.k_lo;
+      uint32_t begun = 0u;  // streams whose O holds something of this segment
       mbar_wait(&sh->q_full, q_phase, err, abort);
       q_phase ^= 1u;
       if constexpr (!kDual) {
@@ -317,10 +372,10 @@ __global__ void __maxnreg__(96)
         for (int s = 0; s < n; ++s, vr.next()) {
           const int x = s & 1;
           const bool more = s + 2 < n;
-          mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
-          wait_p(x);
+          wait_pv(seg, x, s);
+          const bool refused = tile_refused(sh, seg, n0 + s);
           issue([&] {
-            pv(x, vr.stage, s >= 2);
+            if (!refused) pv(x, vr.stage, (begun >> x) & 1u);
             umma_commit(&sh->v_empty[vr.stage]);
             if (!more && s == n - 1) umma_commit(&sh->o_done);
           });
@@ -333,6 +388,7 @@ __global__ void __maxnreg__(96)
             });
             kr.next();
           }
+          if (!refused) begun |= 1u << x;
         }
       } else {
         mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
@@ -345,16 +401,16 @@ __global__ void __maxnreg__(96)
         kr.next();
         for (int j = 0; j < n; ++j, vr.next()) {
           const bool more = j + 1 < n;
-          mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
-          wait_p(0);
+          wait_pv(seg, 0, j);
+          const bool refused = tile_refused(sh, seg, n0 + j);
           if (more) mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
           issue([&] {
-            pv(0, vr.stage, j > 0);
+            if (!refused) pv(0, vr.stage, begun != 0u);
             if (more) qk(0, 0, kr.stage);
           });
-          wait_p(1);
+          wait_pv(seg, 1, j);
           issue([&] {
-            pv(1, vr.stage, j > 0);
+            if (!refused) pv(1, vr.stage, begun != 0u);
             umma_commit(&sh->v_empty[vr.stage]);
             if (more) {
               qk(1, 1, kr.stage);
@@ -365,25 +421,23 @@ __global__ void __maxnreg__(96)
             }
           });
           if (more) kr.next();
+          if (!refused) begun = 1u;
         }
       }
+      n0 += n;
     }
     issue([&] { umma_commit(&sh->drain); });  // every MMA done before TMEM is released
     mbar_drain(&sh->drain, 0);
   } else if (warp >= kQWarp) {
-    // ------------------------------------------------------------ Q loaders
+    // ------------------------------------------------------------ Q loaders, V checkers
     const int tid = int(threadIdx.x) - kQWarp * 32, D = p.head_dim;
     constexpr int kRowChunks = kChunks * 8;                         // 16-byte chunks of a padded row
     constexpr int kEach = (kDual ? 2 : 1) * kRows * kRowChunks / kQThreads;
-    for (int i = 0;; ++i) {
-      const ChunkSegment* found = segment(i);
-      if (found == nullptr) break;
-      const ChunkSegment& seg = *found;
+    const int c = tid % kRowChunks;
+    auto load_q = [&](const ChunkSegment& seg) {
       const ChunkRows unit(P, seg.row0);
       const int rows = seg.queries * P.group - seg.row0;
-      const int c = tid % kRowChunks;
       const T* base = static_cast<const T*>(p.q) + att_q_row(p, seg.b, 0) + int64_t(seg.g) * P.group * p.q_sh + c * 8;
-      if (i > 0) mbar_wait(&sh->q_empty, (i - 1) & 1, err, abort);
 #pragma unroll 4
       for (int u = 0; u < kEach; ++u) {
         const int qr = (u * kQThreads + tid) / kRowChunks;
@@ -406,9 +460,62 @@ __global__ void __maxnreg__(96)
           *reinterpret_cast<uint4*>(dst) = v;
         }
       }
+    };
+    auto q_ready = [&]() {
       cp_async_wait_all();
       fence_proxy_async_smem();
       mbar_arrive(&sh->q_full);
+    };
+    // V of the CTA's n-th tile: values that are not finite become zeros among the rows past the
+    // cached tokens
+    uint32_t check_phase = 0u;
+    auto check_v = [&](const ChunkSegment& seg, int i, int tile, int n) {
+      const int stage = n % kVStages;
+      mbar_wait(&sh->v_check, check_phase, err, abort);
+      check_phase ^= 1u;
+      mbar_wait(&sh->v_full[stage], (n / kVStages) & 1, err, abort);  // done; orders TMA's writes before the reads
+      const int k0 = tile * kKeys, v0 = max(seg.len - k0, 0);
+      uint8_t* at0 = smem + L::kV + stage * kTileBytes;
+      constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+      bool found = false;
+#pragma unroll 4
+      for (int vr = v0 + tid / kRowChunks; vr < kKeys; vr += kQThreads / kRowChunks) {
+        uint4* at = reinterpret_cast<uint4*>(at0 + sw128_offset(vr, c));
+        const uint4 raw = *at;
+        uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((w[e] & kExp) == kExp) w[e] &= 0xFFFF0000u, bad = true;
+          if ((w[e] & (kExp << 16)) == (kExp << 16)) w[e] &= 0x0000FFFFu, bad = true;
+        }
+        if (bad) {
+          *at = make_uint4(w[0], w[1], w[2], w[3]);
+          found |= k0 + vr < seg.kv;
+        }
+      }
+      if (found) *reinterpret_cast<volatile int32_t*>(&sh->fix[i & 1]) = 1;
+      fence_proxy_async_smem();
+      mbar_arrive(&sh->v_ok);
+    };
+    // Per segment: the tiles to check but the last; then, once the segment's last S is done, the
+    // next segment's Q on its way; then the last tile
+    const ChunkSegment* now = segment(0);
+    if (now != nullptr) {
+      load_q(*now);
+      q_ready();
+    }
+    for (int i = 0, n0 = 0; now != nullptr; ++i) {
+      const ChunkSegment seg = *now;
+      const int n = seg.k_hi - seg.k_lo;
+      const int first = first_checked(seg);
+      for (int tile = first; tile < seg.k_hi - 1; ++tile) check_v(seg, i, tile, n0 + tile - seg.k_lo);
+      mbar_wait(&sh->q_empty, i & 1, err, abort);
+      now = segment(i + 1);
+      if (now != nullptr) load_q(*now);
+      if (first < seg.k_hi) check_v(seg, i, seg.k_hi - 1, n0 + n - 1);
+      if (now != nullptr) q_ready();
+      n0 += n;
     }
   } else {
     // ------------------------------------------------------------ softmax warps
@@ -443,32 +550,8 @@ __global__ void __maxnreg__(96)
         mbar_wait(&sh->s_full[x], sc & 1, err, abort);
         tc_fence_after();
         const int k0 = (seg.k_lo + i) * kKeys;
-        const bool none = seg.refused || *reinterpret_cast<volatile int32_t*>(&sh->refused[(n0 + i) & 7]) != 0;
+        const bool none = tile_refused(sh, seg, n0 + i);
         const bool masked = none || k0 + kKeys > seg.len;
-        if (masked && (!kDual || x == 0)) {
-          // values that are not finite among the rows past the cached tokens
-          const int vi = n0 + i, v0 = none ? 0 : max(seg.len - k0, 0);
-          mbar_wait(&sh->v_full[vi % kVStages], (vi / kVStages) & 1, err, abort);
-          uint8_t* tile = smem + L::kV + (vi % kVStages) * kTileBytes;
-          constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
-          for (int idx = int(threadIdx.x) & 255; idx < (kKeys - v0) * kChunks * 8; idx += 256) {
-            const int vr = v0 + idx / (kChunks * 8), c = idx % (kChunks * 8);
-            uint4* at = reinterpret_cast<uint4*>(tile + sw128_offset(vr, c));
-            const uint4 raw = *at;
-            uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((w[e] & kExp) == kExp) w[e] &= 0xFFFF0000u, bad = true;
-              if ((w[e] & (kExp << 16)) == (kExp << 16)) w[e] &= 0x0000FFFFu, bad = true;
-            }
-            if (bad) {
-              *at = make_uint4(w[0], w[1], w[2], w[3]);
-              if (!none && k0 + vr < seg.kv) *reinterpret_cast<volatile int32_t*>(&sh->fix[segs & 1]) = 1;
-            }
-          }
-          fence_proxy_async_smem();
-        }
         __syncwarp();
         if (active) {
           float s[64];
@@ -547,6 +630,7 @@ __global__ void __maxnreg__(96)
         uint32_t from = lane_addr + kOCol + (kDual ? x * 128 : 0);
         if constexpr (kDual) {
           l = sh->sum[x][0][r] + sh->sum[x][1][r];
+          use0 = l != 0.f;  // nothing seen: O may hold anything
         } else {
           const float m0 = sh->m[0][r], m1 = sh->m[1][r];
           const float l0 = sh->sum[0][0][r] + sh->sum[0][1][r], l1 = sh->sum[1][0][r] + sh->sum[1][1][r];
@@ -564,7 +648,7 @@ __global__ void __maxnreg__(96)
         T* out = static_cast<T*>(p.out) +
                  (mine ? att_o_row(p, seg.b, t) + int64_t(seg.g * P.group + hl) * p.o_sh : int64_t(0));
         const int64_t slot = int64_t(blockIdx.x) * 2 + (seg.first ? 0 : 1);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kGroups; ++c) {
           const int col = col0 + c * 32;
           float f[32];
@@ -586,23 +670,6 @@ __global__ void __maxnreg__(96)
             }
           }
           if (mine) {
-          if (fix) {  // V of the nodes this row sees that were left out because they are not finite
-            const int lo = max(seg.k_lo * kKeys, seg.len), hi_pos = min(seg.k_hi * kKeys, seg.kv);
-            const int32_t* table = chunk_table(P, seg.b, seg.g);
-            for (int pos = lo; pos < hi_pos; ++pos) {
-              if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
-              const int32_t page = table[pos >> p.page_shift];
-              if (page < 0 || page >= p.num_pages) continue;
-              const int64_t vrow = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity +
-                                   (int64_t(page) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if (col + e >= D) break;
-                const float v = Elem<T>::to_float(static_cast<const T*>(p.v_pool)[vrow * D + col + e]);
-                if (!isfinite(v)) f[e] += v;
-              }
-            }
-          }
           if (seg.whole) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -612,13 +679,8 @@ __global__ void __maxnreg__(96)
               w.y = Elem<T>::pack2(f[8 * v + 2] * inv, f[8 * v + 3] * inv);
               w.z = Elem<T>::pack2(f[8 * v + 4] * inv, f[8 * v + 5] * inv);
               w.w = Elem<T>::pack2(f[8 * v + 6] * inv, f[8 * v + 7] * inv);
-              if (kp.o_vec) {
-                *reinterpret_cast<uint4*>(out + col + v * 8) = w;
-              } else {
-                uint16_t* e = reinterpret_cast<uint16_t*>(out + col + v * 8);
-                e[0] = uint16_t(w.x), e[1] = uint16_t(w.x >> 16), e[2] = uint16_t(w.y), e[3] = uint16_t(w.y >> 16);
-                e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
-              }
+              if (kp.o_vec) *reinterpret_cast<uint4*>(out + col + v * 8) = w;
+              else store_unaligned16(out + col + v * 8, w);
             }
           } else {
             float4* wo = chunk_partial_o(P, slot);
@@ -629,6 +691,9 @@ __global__ void __maxnreg__(96)
                     make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
             if (col == 0) chunk_partial_ml(P, slot)[unit_row] = make_float2(m, l);
           }
+          if (fix)
+            add_not_finite<T>(P, seg, t, col, min(32, D - col), out + col,
+                              reinterpret_cast<float*>(chunk_partial_o(P, slot)) + unit_row * 4);
           }
           __syncwarp();
         }
@@ -676,7 +741,7 @@ cudaError_t launch_tree_shape(const TreeKernelParams& kp, const CUtensorMap& k_m
 }  // namespace
 
 ChunkShape chunk_shape_tensor(int64_t max_rows, int num_sms) {
-  return {max_rows <= kRows ? kRows : 2 * kRows, kKeys, num_sms};
+  return {max_rows <= kRows ? kRows : 2 * kRows, kKeys, kUnitCost, num_sms};
 }
 
 cudaError_t run_chunk_attention_tensor(const ChunkParams& p, bool q_vec, bool o_vec, const CUtensorMap& k_map,

@@ -75,7 +75,9 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
   const float scale_log2 = p.scale * kLog2e;
   const int page_mask = (1 << p.page_shift) - 1;
 
-  while (walk.next(P, seg)) {
+  bool more = walk.next(P, seg);
+  if (tid == 0) chunk_write_join(P, start, blockIdx.x, more ? &seg : nullptr);
+  for (; more; more = walk.next(P, seg)) {
     const int rows_left = seg.queries * P.group - seg.row0;  // valid rows of this unit (may exceed kRows)
     const int32_t* table = chunk_table(P, seg.b, seg.g);
     const int64_t plane = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity;
@@ -296,52 +298,45 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
 // ------------------------------------------------------------------ merge
 constexpr int kMergeThreads = 256;
 
-// Boundary c = blockIdx.x + 1 of the work line; the first boundary strictly inside a unit
-// joins that unit's partials: CTA c - 1's last segment (or first, if it starts with the
-// unit) and the first segments of the CTAs from c on. Thread: (row, 4 dims), consecutive
-// threads consecutive rows, as the partials are stored; four parts' loads at a time. Fixed
-// order, no atomics. Launched while the attention kernel runs (its own start-up reads only
-// the step's lengths) and waits for that kernel's results.
-template <typename T>
-__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams P) {
-  __shared__ int64_t sums[kMergeThreads / 32];
-  __shared__ ChunkStart start;
-  const AttentionParams& p = P.a;
-  const int c = int(blockIdx.x) + 1;
-  chunk_find_start<kMergeThreads>(P, c, P.ctas, sums, &start);
-  const int64_t begin = start.begin(c);
-  if (begin >= start.total) return;
-  int why = 0;
-  const ChunkRequest r = chunk_request(P, start.b, why);
-  const int64_t unit = chunk_div(start.off, r.tiles), unit_off = start.off - unit * r.tiles;
-  const int64_t unit_begin = begin - unit_off, unit_end = unit_begin + r.tiles;
-  const int64_t before = start.begin(c - 1);
-  if (unit_off == 0 || before > unit_begin) return;
-  const int g = int(chunk_div(unit, r.row_blocks));
-  const int row0 = int(unit - int64_t(g) * r.row_blocks) * P.unit_rows;
-  const int rows = min(r.queries * P.group - row0, P.unit_rows);
-  const int idx = int(blockIdx.y) * kMergeThreads + int(threadIdx.x);
-  const int row = idx & (P.unit_rows - 1), d4 = idx >> P.unit_shift;
-  if (row >= rows || d4 * 4 >= p.head_dim) return;
+// CTA (c - 1, y): rows 32 y .. of the unit that CTA c's join record names. Warp w, lane r: row r,
+// dims 4 (w + 8 k): the partials are stored with consecutive rows next to each other, so every
+// load is 512 contiguous bytes; the joined rows go through shared memory so that the stores
+// are contiguous too (storing from the accumulators, 2 bytes of 32 rows at a time, cost
+// 30 us on 8 requests x 256 nodes). kAhead parts' loads at a time. Fixed order, no atomics.
+// Launched while the attention kernel runs; waits for its results before it reads anything.
+constexpr int kMergeRows = 32;
 
-  // part 0: CTA c - 1; part i: CTA c - 1 + i, its first segment (CTAs with no tiles come last)
-  const int64_t slot0 = int64_t(c - 1) * 2 + (before == unit_begin ? 0 : 1);
-  int parts = 1;
-  while (c - 1 + parts < P.ctas && start.begin(c - 1 + parts) < unit_end) ++parts;
+// kGroups: ceil(head_dim / 32)
+template <typename T, int kGroups>
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams P) {
+  __shared__ T rows_s[kMergeRows][kGroups * 32 + 2];
+  const AttentionParams& p = P.a;
+  const int c = int(blockIdx.x) + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = int(blockIdx.y) * kMergeRows + lane;
   wait_for_primary();
-  constexpr int kAhead = 4;
+  const int4 j0 = __ldcg(reinterpret_cast<const int4*>(P.ws_join + c));
+  const int4 j1 = __ldcg(reinterpret_cast<const int4*>(P.ws_join + c) + 1);
+  const int b = j0.x, g = j0.y, row0 = j0.z, rows = j0.w, slot0 = j1.x, parts = j1.y;
+  const int here = min(rows - int(blockIdx.y) * kMergeRows, kMergeRows);  // rows of this CTA
+  if (here <= 0) return;
+  const int dims4 = p.head_dim / 4;
+  constexpr int kAhead = 2;
   float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 o[kGroups];
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < parts; i0 += kAhead) {
     float2 ml[kAhead];
-    float4 v[kAhead];
+    float4 v[kAhead][kGroups];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int64_t slot = i0 + u == 0 ? slot0 : int64_t(c - 1 + i0 + u) * 2;
       ml[u] = make_float2(-INFINITY, 0.f);
-      if (i0 + u < parts) {
+      if (i0 + u < parts && lane < here) {
         ml[u] = __ldcg(&chunk_partial_ml(P, slot)[row]);
-        v[u] = __ldcg(&chunk_partial_o(P, slot)[int64_t(d4) * P.unit_rows + row]);
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k)
+          if (warp + 8 * k < dims4) v[u][k] = __ldcg(&chunk_partial_o(P, slot)[int64_t(warp + 8 * k) * P.unit_rows + row]);
       }
     }
 #pragma unroll
@@ -350,21 +345,44 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
       const float m_new = fmaxf(m, ml[u].x), m_use = m_new == -INFINITY ? 0.f : m_new;
       const float f = ex2(ml[u].x - m_use), keep = m == -INFINITY ? 0.f : ex2(m - m_use);
       l = fmaf(ml[u].y, f, l * keep);
-      o.x = fmaf(v[u].x, f, o.x * keep);
-      o.y = fmaf(v[u].y, f, o.y * keep);
-      o.z = fmaf(v[u].z, f, o.z * keep);
-      o.w = fmaf(v[u].w, f, o.w * keep);
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        o[k].x = fmaf(v[u][k].x, f, o[k].x * keep);
+        o[k].y = fmaf(v[u][k].y, f, o[k].y * keep);
+        o[k].z = fmaf(v[u][k].z, f, o[k].z * keep);
+        o[k].w = fmaf(v[u][k].w, f, o[k].w * keep);
+      }
       m = m_new;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  int t, hl;
-  ChunkRows(P, row0).at(P, row, t, hl);
-  T* out = static_cast<T*>(p.out) + att_o_row(p, start.b, t) + int64_t(g * P.group + hl) * p.o_sh + d4 * 4;
-  out[0] = Elem<T>::from_float(o.x * inv);
-  out[1] = Elem<T>::from_float(o.y * inv);
-  out[2] = Elem<T>::from_float(o.z * inv);
-  out[3] = Elem<T>::from_float(o.w * inv);
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) {
+    const int d = (warp + 8 * k) * 4;
+    if (d >= p.head_dim) break;
+    rows_s[lane][d] = Elem<T>::from_float(o[k].x * inv);
+    rows_s[lane][d + 1] = Elem<T>::from_float(o[k].y * inv);
+    rows_s[lane][d + 2] = Elem<T>::from_float(o[k].z * inv);
+    rows_s[lane][d + 3] = Elem<T>::from_float(o[k].w * inv);
+  }
+  __syncthreads();
+  const ChunkRows unit(P, row0);
+  for (int r = warp; r < here; r += kMergeThreads / 32) {
+    int t, hl;
+    unit.at(P, int(blockIdx.y) * kMergeRows + r, t, hl);
+    T* out = static_cast<T*>(p.out) + att_o_row(p, b, t) + int64_t(g * P.group + hl) * p.o_sh;
+#pragma unroll
+    for (int d = lane; d < kGroups * 32; d += 32)
+      if (d < p.head_dim) out[d] = rows_s[r][d];
+  }
+}
+
+template <typename T>
+cudaError_t launch_merge(const ChunkParams& p, cudaStream_t stream) {
+  const dim3 grid(unsigned(p.ctas - 1), unsigned((p.unit_rows + kMergeRows - 1) / kMergeRows));
+  if (p.a.head_dim <= 64) return launch_after(chunk_merge_kernel<T, 2>, grid, kMergeThreads, 0, stream, p);
+  if (p.a.head_dim <= 128) return launch_after(chunk_merge_kernel<T, 4>, grid, kMergeThreads, 0, stream, p);
+  return launch_after(chunk_merge_kernel<T, 8>, grid, kMergeThreads, 0, stream, p);
 }
 
 template <typename T, int kRows, int kChunks>
@@ -406,7 +424,7 @@ ChunkShape chunk_shape_general(int64_t max_rows, int dtype, int head_dim, int nu
   // resident CTAs per SM by shared memory (228 KB per SM, 1 KB reserved per CTA)
   const int smem = (rows + 2 * kKeys) * ((head_dim + 63) / 64 * 64 + 4) * 4 + 1024;
   const int per_sm = smem * 3 <= 228 * 1024 ? 3 : (smem * 2 <= 228 * 1024 ? 2 : 1);
-  return {rows, kKeys, num_sms * per_sm};
+  return {rows, kKeys, 1, num_sms * per_sm};
 }
 
 cudaError_t run_chunk_attention_general(const ChunkParams& p, int dtype, cudaStream_t stream) {
@@ -419,12 +437,10 @@ cudaError_t run_chunk_attention_general(const ChunkParams& p, int dtype, cudaStr
 
 cudaError_t run_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t stream) {
   if (p.ctas < 2) return cudaSuccess;
-  const int64_t work = int64_t(p.unit_rows) * (p.a.head_dim / 4);
-  const dim3 grid(unsigned(p.ctas - 1), unsigned((work + kMergeThreads - 1) / kMergeThreads));
   switch (dtype) {
-    case HYT_DTYPE_BF16: return launch_after(chunk_merge_kernel<__nv_bfloat16>, grid, kMergeThreads, 0, stream, p);
-    case HYT_DTYPE_F16: return launch_after(chunk_merge_kernel<__half>, grid, kMergeThreads, 0, stream, p);
-    default: return launch_after(chunk_merge_kernel<float>, grid, kMergeThreads, 0, stream, p);
+    case HYT_DTYPE_BF16: return launch_merge<__nv_bfloat16>(p, stream);
+    case HYT_DTYPE_F16: return launch_merge<__half>(p, stream);
+    default: return launch_merge<float>(p, stream);
   }
 }
 
