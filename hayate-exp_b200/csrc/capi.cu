@@ -1517,9 +1517,6 @@ int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_
     return fail(HYT_ERR_INVALID, "page_table_width must be positive and at most the row stride");
   if (page_table_width > hyt::kSelectMaxPages)
     return fail(HYT_ERR_UNSUPPORTED, "a request may have at most 16384 pages");
-  if (batch > 65535 || num_kv_heads > 65535) return fail(HYT_ERR_UNSUPPORTED, "batch too large");
-  if (int64_t(num_q_heads / num_kv_heads) * head_dim * 8 > 128 * 1024)
-    return fail(HYT_ERR_UNSUPPORTED, "too many query heads per KV head for page selection");
   if (int64_t(batch) * num_kv_heads * num_pages > INT32_MAX)
     return fail(HYT_ERR_UNSUPPORTED, "batch times KV heads times num_pages is too large");
   const size_t ids = align256(size_t(batch) * num_kv_heads * num_pages * 4), lens = align256(size_t(batch) * 4);
@@ -1557,6 +1554,7 @@ int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_
   c.a.page_table_stride = num_kv_heads * num_pages;
   c.table_width = num_pages;
   c.table_head_stride = num_pages;
+  c.after_selection = 1;
   return launch_chunk(c, g, ws + ids + lens, workspace_bytes - ids - lens, static_cast<cudaStream_t>(stream));
 }
 

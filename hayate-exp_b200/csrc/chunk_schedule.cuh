@@ -80,6 +80,7 @@ __device__ __forceinline__ void chunk_find_start(const ChunkParams& P, int c, in
                                                  ChunkStart* start) {
   constexpr int kWarps = kThreads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  wait_for_primary();  // page selection writes the lengths and pages of a decode over chosen pages
   const int per = (P.a.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, P.a.batch), b1 = min(b0 + per, P.a.batch);
   int why = 0;

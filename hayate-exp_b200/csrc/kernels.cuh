@@ -196,6 +196,7 @@ struct ChunkParams {
   int32_t unit_cost;             // of a unit's start and end, in tiles
   uint32_t group_magic;          // ceil(2^20 / group)
   int32_t ctas;
+  int32_t after_selection;  // launched while run_select_pages still runs
   float* ws_o;   // [ctas, 2 slots, head_dim / 4, unit_rows, 4] f32
   float* ws_ml;  // [ctas, 2 slots, unit_rows, 2] f32
   ChunkJoin* ws_join;  // [ctas]

@@ -8,10 +8,16 @@
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
 // the most a key of the page can score; the take - 1 best full pages (ties: the lowest page)
 // and the page being written, in ascending order. Which page is read hangs on scores next
-// to each other, so the sums run in 64 bits (a product of two 16-bit values is exact there)
-// and are rounded once to fp32: the choice does not depend on the order of summation.
-// One CTA per (request, KV head): 8 lanes per page, 2 rows of bounds per page read once; the
-// take - 1 best by a radix selection on order-preserving 32-bit keys in shared memory.
+// to each other, so a score must not depend on the order of summation: products of 16-bit
+// values are exact in fp32 (fp32 ones keep their rounding error by an FMA), the sums carry
+// their rounding errors along (Knuth's two-sum, on packed pairs), lanes meet in 64 bits, and
+// the result is rounded once. That costs 5.5 instructions a term; converting to 64 bits term
+// by term took 80 us on 64 requests x 256 pages x 8 KV heads (4 heads a group), this 20.
+// A cluster of 1 to 8 CTAs per (request, KV head) shares the pages out, 16 lanes per page and
+// the bounds read once; the keys (order-preserving 32-bit scores) meet in the first CTA's
+// shared memory, which finds the (take - 1)-th largest 8 bits at a time.
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "chunk_schedule.cuh"
@@ -113,36 +119,61 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kHeadsAtOnce = 4;
+// A sum of fp32 terms with its rounding errors, two at a time.
+struct PairSum {
+  uint64_t s = 0, e = 0;  // packed pairs of +0
+  __device__ __forceinline__ void add(uint64_t p) {
+    const uint64_t minus = f2_pack(-1.f, -1.f);
+    const uint64_t t = f2_add(s, p), bb = f2_fma(s, minus, t);   // t = s + p rounded; bb = t - s
+    const uint64_t back = f2_fma(bb, minus, t);                  // t - bb
+    e = f2_add(e, f2_add(f2_fma(back, minus, s), f2_fma(bb, minus, p)));
+    s = t;
+  }
+  __device__ __forceinline__ double total() const {
+    float s0, s1, e0, e1;
+    f2_unpack(s, s0, s1);
+    f2_unpack(e, e0, e1);
+    // a sum that overflowed or met a NaN or infinity has no error term worth having
+    return isfinite(s0) && isfinite(s1) ? (double(s0) + double(s1)) + (double(e0) + double(e1)) : double(s0) + double(s1);
+  }
+};
 
-template <typename T>
+// kHeads: query heads scored per pass over a page's bounds.
+template <typename T, int kHeads>
 __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const SelectParams p) {
   constexpr int kPer = 16 / int(sizeof(T));
   constexpr int kWarps = kSelectThreads / 32;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  const int g = blockIdx.x, b = blockIdx.y;
+  constexpr int kLanes = 16;  // per page
+  extern __shared__ __align__(16) uint32_t keys[];  // [last], the first CTA's are used
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int unit = int(blockIdx.x) / ranks;
+  const int b = unit / p.num_kv_heads, g = unit - b * p.num_kv_heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int D = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
-  double* qs = reinterpret_cast<double*>(smem_raw);               // [group][D]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(qs + group * D);   // [last]
   __shared__ int hist[256];
   __shared__ int warp_count[kWarps];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
+  launch_dependents();  // the attention kernel may start up; it waits for this grid's results
 
   const int64_t out_row = (int64_t(b) * p.num_kv_heads + g) * p.take;
   const int32_t* table = p.page_table + int64_t(b) * p.page_table_stride;
   const int len = p.cache_lens[b];
   const int last = len >= 0 ? len >> p.page_shift : p.table_width;  // the page being written
   if (last >= p.table_width || last > kSelectMaxPages) {
+    if (rank != 0) return;
     if (tid == 0 && g == 0) flag_error(p.error_word, HYT_DEVERR_TABLE_RANGE);
     for (int i = tid; i < p.take; i += kSelectThreads) p.selected[out_row + i] = p.pages[out_row + i] = -1;
     if (g == 0 && tid == 0) p.lens[b] = 0;
     return;
   }
   const int count = min(last + 1, p.take);
-  if (g == 0 && tid == 0) p.lens[b] = ((count - 1) << p.page_shift) + (len & ((1 << p.page_shift) - 1));
+  if (g == 0 && rank == 0 && tid == 0)
+    p.lens[b] = ((count - 1) << p.page_shift) + (len & ((1 << p.page_shift) - 1));
   if (last < p.take) {  // every page is read
+    if (rank != 0) return;
     for (int i = tid; i < p.take; i += kSelectThreads) {
       p.selected[out_row + i] = i < count ? i : -1;
       p.pages[out_row + i] = i < count ? table[i] : -1;
@@ -150,59 +181,78 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
     return;
   }
 
-  const T* q = static_cast<const T*>(p.q) + int64_t(b) * p.q_sb + int64_t(g) * group * p.q_sh;
-  for (int i = tid; i < group * D; i += kSelectThreads)
-    qs[i] = double(Elem<T>::to_float(q[int64_t(i / D) * p.q_sh + i % D]));
-  __syncthreads();
-
-  // ---- scores of the full pages 0 .. last - 1, 8 lanes per page
-  const T* bounds = static_cast<const T*>(p.k_bounds) +
-                    (int64_t(p.layer) * p.num_kv_heads + g) * p.num_pages * 2 * D;
-  const int sub = lane >> 3, l8 = lane & 7, chunks = D / kPer;
-  for (int i0 = warp * 4; i0 < last; i0 += kWarps * 4) {
-    const int i = i0 + sub;
-    int32_t page = -1;
-    if (i < last) {
-      page = table[i];
-      if (page < 0 || page >= p.num_pages) {
-        if (l8 == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
-        page = -1;
+  // ---- scores of the full pages 0 .. last - 1: this CTA's share, 16 lanes per page
+  {
+    if (ranks > 1) cluster.sync();  // the first CTA has started: its shared memory may be written
+    uint32_t* to = cluster.map_shared_rank(keys, 0);
+    const T* bounds = static_cast<const T*>(p.k_bounds) +
+                      (int64_t(p.layer) * p.num_kv_heads + g) * p.num_pages * 2 * D;
+    const T* q0 = static_cast<const T*>(p.q) + int64_t(b) * p.q_sb + int64_t(g) * group * p.q_sh;
+    const int sub = lane / kLanes, l16 = lane % kLanes, chunks = D / kPer;
+    constexpr int kPages = kWarps * (32 / kLanes);  // pages a CTA scores at a time
+    for (int i0 = rank * kPages; i0 < last; i0 += ranks * kPages) {
+      const int i = i0 + warp * (32 / kLanes) + sub;
+      int32_t page = -1;
+      if (i < last) {
+        page = table[i];
+        if (page < 0 || page >= p.num_pages) {
+          if (l16 == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
+          page = -1;
+        }
       }
-    }
-    const T* lo = bounds + int64_t(max(page, 0)) * 2 * D;
-    float best = -INFINITY;
-    bool nan = false;
-    for (int h0 = 0; h0 < group; h0 += kHeadsAtOnce) {
-      double acc[kHeadsAtOnce] = {0., 0., 0., 0.};
-      for (int c = l8; c < chunks; c += 8) {
-        float fl[kPer], fh[kPer];
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(lo) + c), fl);
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(lo + D) + c), fh);
+      const T* lo = bounds + int64_t(max(page, 0)) * 2 * D;
+      float best = -INFINITY;
+      bool nan = false;
+      for (int h0 = 0; h0 < group; h0 += kHeads) {
+        PairSum acc[kHeads];
+        for (int c = l16; c < chunks; c += kLanes) {
+          const uint4 lraw = __ldg(reinterpret_cast<const uint4*>(lo) + c);
+          const uint4 hraw = __ldg(reinterpret_cast<const uint4*>(lo + D) + c);
+          const uint32_t lw[4] = {lraw.x, lraw.y, lraw.z, lraw.w}, hw[4] = {hraw.x, hraw.y, hraw.z, hraw.w};
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const double dl = fl[e], dh = fh[e];
-#pragma unroll
-          for (int h = 0; h < kHeadsAtOnce; ++h) {
+          for (int h = 0; h < kHeads; ++h) {
             if (h0 + h >= group) break;
-            const double qv = qs[(h0 + h) * D + c * kPer + e];
-            acc[h] = fma(qv, qv >= 0. ? dh : dl, acc[h]);
+            const T* qh = q0 + int64_t(h0 + h) * p.q_sh + c * kPer;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const float qa = Elem<T>::to_float(qh[2 * w]), qb = Elem<T>::to_float(qh[2 * w + 1]);
+                const uint32_t m = (qa >= 0.f ? 0x0000FFFFu : 0u) | (qb >= 0.f ? 0xFFFF0000u : 0u);
+                const uint32_t x = (hw[w] & m) | (lw[w] & ~m);
+                const T* xe = reinterpret_cast<const T*>(&x);
+                acc[h].add(f2_mul(f2_pack(qa, qb), f2_pack(Elem<T>::to_float(xe[0]), Elem<T>::to_float(xe[1]))));
+              }
+            } else {
+#pragma unroll
+              for (int w = 0; w < 4; w += 2) {
+                const float qa = qh[w], qb = qh[w + 1];
+                const uint64_t q2 = f2_pack(qa, qb);
+                const uint64_t x2 = f2_pack(__uint_as_float(qa >= 0.f ? hw[w] : lw[w]),
+                                            __uint_as_float(qb >= 0.f ? hw[w + 1] : lw[w + 1]));
+                const uint64_t prod = f2_mul(q2, x2);
+                acc[h].add(prod);
+                acc[h].e = f2_add(acc[h].e, f2_fma(q2, x2, f2_mul(prod, f2_pack(-1.f, -1.f))));
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          double total = acc[h].total();
+#pragma unroll
+          for (int off = kLanes / 2; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+          if (h0 + h < group) {
+            const float x = float(total);
+            nan |= isnan(x);
+            best = fmaxf(best, x);
           }
         }
       }
-#pragma unroll
-      for (int h = 0; h < kHeadsAtOnce; ++h) {
-#pragma unroll
-        for (int off = 4; off > 0; off >>= 1) acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], off);
-        if (h0 + h < group) {
-          const float x = float(acc[h]);
-          nan |= isnan(x);
-          best = fmaxf(best, x);
-        }
-      }
+      if (i < last && l16 == 0) to[i] = page < 0 ? 0u : (nan ? 0xFFFFFFFFu : score_key(best));
     }
-    if (i < last && l8 == 0) keys[i] = page < 0 ? 0u : (nan ? 0xFFFFFFFFu : score_key(best));
   }
-  __syncthreads();
+  cluster.sync();
+  if (rank != 0) return;
 
   // ---- the (take - 1)-th largest key, 8 bits at a time
   int need = p.take - 1;  // of the keys that match the prefix so far, this many are wanted
@@ -253,11 +303,11 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
     equal += __popc(__ballot_sync(0xffffffffu, i < end && keys[i] == prefix));
   if (lane == 0) warp_count[warp] = equal;
   __syncthreads();
-  int rank = 0;  // equal keys before this warp's
-  for (int w = 0; w < warp; ++w) rank += warp_count[w];
+  int equal_before = 0;  // equal keys before this warp's
+  for (int w = 0; w < warp; ++w) equal_before += warp_count[w];
   __syncthreads();
   const bool any = p.take > 1;
-  int mine = 0, r = rank;
+  int mine = 0, r = equal_before;
   for (int i = first + lane; i < first + share; i += 32) {
     const bool eq = any && i < end && keys[i] == prefix, gt = any && i < end && keys[i] > prefix;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
@@ -269,7 +319,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   __syncthreads();
   int at = 0;
   for (int w = 0; w < warp; ++w) at += warp_count[w];
-  r = rank;
+  r = equal_before;
   for (int i = first + lane; i < first + share; i += 32) {
     const bool eq = any && i < end && keys[i] == prefix, gt = any && i < end && keys[i] > prefix;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
@@ -303,20 +353,36 @@ cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t strea
 }
 
 cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stream) {
-  const int group = p.num_q_heads / p.num_kv_heads;
+  const int group = p.num_q_heads / p.num_kv_heads, units = p.batch * p.num_kv_heads;
   const int ranked = p.table_width < kSelectMaxPages ? p.table_width : kSelectMaxPages;
-  const int smem = group * p.head_dim * 8 + ranked * 4;
-  const dim3 grid(unsigned(p.num_kv_heads), unsigned(p.batch));
+  // CTAs per unit: enough to give every SM two, none with less than 32 pages
+  int ranks = 1;
+  while (ranks < 8 && units * ranks < 2 * 148 && ranked >= 64 * ranks) ranks *= 2;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(ranks);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(units * ranks));
+  config.blockDim = dim3(kSelectThreads);
+  config.dynamicSmemBytes = size_t(ranked) * 4;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
   auto launch = [&](auto kernel) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    kernel<<<grid, kSelectThreads, smem, stream>>>(p);
-    return cudaGetLastError();
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(config.dynamicSmemBytes));
+    return e != cudaSuccess ? e : cudaLaunchKernelEx(&config, kernel, p);
+  };
+  auto heads = [&](auto type) {
+    using T = decltype(type);
+    if (group == 1) return launch(select_pages_kernel<T, 1>);
+    if (group == 2) return launch(select_pages_kernel<T, 2>);
+    return launch(select_pages_kernel<T, 4>);
   };
   switch (dtype) {
-    case HYT_DTYPE_BF16: return launch(select_pages_kernel<__nv_bfloat16>);
-    case HYT_DTYPE_F16: return launch(select_pages_kernel<__half>);
-    default: return launch(select_pages_kernel<float>);
+    case HYT_DTYPE_BF16: return heads(__nv_bfloat16{});
+    case HYT_DTYPE_F16: return heads(__half{});
+    default: return heads(float{});
   }
 }
 

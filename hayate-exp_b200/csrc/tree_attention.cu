@@ -735,6 +735,7 @@ cudaError_t launch_tree(const TreeKernelParams& kp, const CUtensorMap& k_map, co
   static_assert(smem <= 227 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
+  if (kp.c.after_selection) return launch_after(kernel, dim3(kp.c.ctas), kThreads, smem, stream, k_map, v_map, kp);
   kernel<<<kp.c.ctas, kThreads, smem, stream>>>(k_map, v_map, kp);
   return cudaGetLastError();
 }

@@ -397,6 +397,7 @@ cudaError_t launch_general(const ChunkParams& p, cudaStream_t stream) {
   constexpr int smem = general_smem<T, kRows, kChunks>();
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
+  if (p.after_selection) return launch_after(kernel, dim3(p.ctas), kThreads, smem, stream, p);
   kernel<<<p.ctas, kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }

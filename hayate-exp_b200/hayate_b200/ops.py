@@ -7,7 +7,6 @@ message if the call is refused. All launches go on the current CUDA stream.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
@@ -510,21 +509,25 @@ def prefill_attention_planned(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
 
 
 # ---------------------------------------------------------------------------- trees, moves, chosen pages
-def _same_device(*tensors: torch.Tensor | None) -> torch.device:
-    """The one CUDA device all tensors are on."""
-    tensors = [t for t in tensors if t is not None]
-    _require_cuda(*tensors)
-    device = tensors[0].device
-    if any(t.device != device for t in tensors):
-        raise RuntimeError("all tensors must be on the same CUDA device")
-    return device
+def _device_index(*tensors: torch.Tensor | None) -> int:
+    """Index of the one CUDA device all tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _require_cuda(*(t for t in tensors if t is not None))
+            raise RuntimeError("all tensors must be on the same CUDA device")
+    if index < 0:
+        _require_cuda(tensors[0])
+    return index
 
 
-def _on(device: torch.device):
-    """Launch on ``device``: its current stream, whatever the current device is."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _on_device(index: int, fn, *args):
+    """Call ``fn(*args, stream)`` with ``index`` as the current device, on its current stream."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
+        return fn(*args, stream)
+    with torch.cuda.device(index):
+        return fn(*args, stream)
 
 
 def _int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> None:
@@ -546,10 +549,11 @@ def _page_rows(page_table: torch.Tensor, batch: int) -> tuple[int, int]:
     return max(page_table.stride(0), width), width
 
 
-def _output(out: torch.Tensor | None, like: torch.Tensor, memory: tuple[int, ...]) -> torch.Tensor:
-    """``out`` checked against ``like``, or a new one in ``[.., T, H, D]`` memory viewed as ``like``."""
+def _output(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    """``out`` checked against ``like`` ``[B, H, T, D]``, or a new one in ``[B, T, H, D]`` memory."""
     if out is None:
-        return torch.empty(memory, dtype=like.dtype, device=like.device).transpose(1, 2)
+        b, h, t, d = like.shape
+        return torch.empty_strided((b, h, t, d), (t * h * d, d, h * d, 1), dtype=like.dtype, device=like.device)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError("out must match q")
     return out
@@ -587,7 +591,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     every ``q_len``. Rows of the token axis that no request owns are left as they are.
     ``workspace`` (``tree_workspace_bytes``, any contents) is allocated if not given.
     """
-    device = _same_device(q, k_pool, v_pool, page_table, cache_lens, q_start, q_len, tree_mask, out,
+    index = _device_index(q, k_pool, v_pool, page_table, cache_lens, q_start, q_len, tree_mask, out,
                           workspace, error_word)
     num_layers, num_kv_heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
     qs = _th_strides(q, "q")
@@ -605,20 +609,19 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         words = tree_mask.size(1)
         if tree_mask.size(0) != total or words * 32 < max_query_len:
             raise ValueError("tree_mask must have a row per token and a bit per node")
-    out = _output(out, q, (1, total, num_q_heads, head_dim))
+    out = _output(out, q)
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     if total == 0:
         return out
     need = tree_workspace_bytes(max_query_len, num_q_heads, num_kv_heads, head_dim, q.dtype)
-    workspace = _scratch(workspace, need, device)
-    with _on(device):
-        rc = _lib.lib().hyt_tree_attention(
-            q.data_ptr(), _lib.int64_array(qs), k_pool.data_ptr(), v_pool.data_ptr(), num_layers, layer,
-            capacity, page_table.data_ptr(), stride, width, cache_lens.data_ptr(), q_start.data_ptr(),
-            q_len.data_ptr(), _ptr(tree_mask), words, out.data_ptr(),
-            _lib.int64_array(_th_strides(out, "out")), batch, total, num_q_heads, num_kv_heads, head_dim,
-            page_size, dtype_code(q.dtype), scale, max_query_len, workspace.data_ptr(),
-            workspace.numel(), _ptr(error_word), _stream_ptr())
+    workspace = _scratch(workspace, need, q.device)
+    rc = _on_device(
+        index, _lib.lib().hyt_tree_attention, q.data_ptr(), _lib.int64_array(qs), k_pool.data_ptr(),
+        v_pool.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride, width,
+        cache_lens.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), _ptr(tree_mask), words, out.data_ptr(),
+        _lib.int64_array(_th_strides(out, "out")), batch, total, num_q_heads, num_kv_heads, head_dim,
+        page_size, dtype_code(q.dtype), scale, max_query_len, workspace.data_ptr(), workspace.numel(),
+        _ptr(error_word))
     _lib.check(rc, "hyt_tree_attention")
     return out
 
@@ -629,15 +632,14 @@ def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, src_pages: torch.Tens
 
     Of two entries with one target the later counts. An entry whose target another entry
     reads is skipped and flagged in ``error_word``, as are ids outside the pool."""
-    device = _same_device(k_pool, v_pool, src_pages, dst_pages, error_word)
+    index = _device_index(k_pool, v_pool, src_pages, dst_pages, error_word)
     num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
     _int32_vector(src_pages, "src_pages")
     _int32_vector(dst_pages, "dst_pages", src_pages.numel())
-    with _on(device):
-        rc = _lib.lib().hyt_copy_pages(
-            k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity, head_dim, page_size,
-            dtype_code(k_pool.dtype), src_pages.data_ptr(), dst_pages.data_ptr(), src_pages.numel(),
-            _ptr(error_word), _stream_ptr())
+    rc = _on_device(
+        index, _lib.lib().hyt_copy_pages, k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity,
+        head_dim, page_size, dtype_code(k_pool.dtype), src_pages.data_ptr(), dst_pages.data_ptr(),
+        src_pages.numel(), _ptr(error_word))
     _lib.check(rc, "hyt_copy_pages")
 
 
@@ -651,19 +653,17 @@ def compact_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.T
     are not are skipped and flagged in ``error_word``); ``src_start`` has ``batch + 1`` entries
     from 0 to ``len(src_rows)``. The accepted path of a drafted tree moves up behind the
     context this way. No two requests may share a page in which rows move."""
-    device = _same_device(k_pool, v_pool, page_table, base, src_rows, src_start, error_word)
+    index = _device_index(k_pool, v_pool, page_table, base, src_rows, src_start, error_word)
     num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
     _int32_vector(base, "base")
     batch = base.numel()
     _int32_vector(src_rows, "src_rows")
     _int32_vector(src_start, "src_start", batch + 1)
     stride, width = _page_rows(page_table, batch)
-    with _on(device):
-        rc = _lib.lib().hyt_compact_rows(
-            k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity, head_dim, page_size,
-            dtype_code(k_pool.dtype), page_table.data_ptr(), stride, width, base.data_ptr(),
-            src_rows.data_ptr(), src_start.data_ptr(), batch, src_rows.numel(), _ptr(error_word),
-            _stream_ptr())
+    rc = _on_device(
+        index, _lib.lib().hyt_compact_rows, k_pool.data_ptr(), v_pool.data_ptr(), num_layers, heads, capacity,
+        head_dim, page_size, dtype_code(k_pool.dtype), page_table.data_ptr(), stride, width, base.data_ptr(),
+        src_rows.data_ptr(), src_start.data_ptr(), batch, src_rows.numel(), _ptr(error_word))
     _lib.check(rc, "hyt_compact_rows")
 
 
@@ -681,16 +681,15 @@ def page_bounds(k_pool: torch.Tensor, k_bounds: torch.Tensor, pages: torch.Tenso
     ``[layers, H_kv, num_pages, 2, D]`` (all layers, or one), for ``sparse_attention``.
 
     ``pages`` (int32) lists pages whose tokens are all written; -1 entries are skipped."""
-    device = _same_device(k_pool, k_bounds, pages, error_word)
+    index = _device_index(k_pool, k_bounds, pages, error_word)
     num_layers, heads, capacity, head_dim = _pool_geometry(k_pool, k_pool)
     _check_bounds(k_bounds, k_pool, page_size)
     _int32_vector(pages, "pages")
     first, layers = (0, num_layers) if layer is None else (layer, 1)
-    with _on(device):
-        rc = _lib.lib().hyt_page_bounds(
-            k_pool.data_ptr(), k_bounds.data_ptr(), num_layers, first, layers, heads, capacity, head_dim,
-            page_size, dtype_code(k_pool.dtype), pages.data_ptr(), pages.numel(), _ptr(error_word),
-            _stream_ptr())
+    rc = _on_device(
+        index, _lib.lib().hyt_page_bounds, k_pool.data_ptr(), k_bounds.data_ptr(), num_layers, first, layers,
+        heads, capacity, head_dim, page_size, dtype_code(k_pool.dtype), pages.data_ptr(), pages.numel(),
+        _ptr(error_word))
     _lib.check(rc, "hyt_page_bounds")
 
 
@@ -718,7 +717,7 @@ def sparse_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     ``[B, H_q, 1, D]`` and the logical pages read, int32 ``[B, H_kv, num_pages]``, ascending,
     -1 past the last. ``workspace`` (``sparse_workspace_bytes``, any contents) is allocated
     if not given."""
-    device = _same_device(q, k_pool, v_pool, k_bounds, page_table, cache_lens, out, workspace, error_word)
+    index = _device_index(q, k_pool, v_pool, k_bounds, page_table, cache_lens, out, workspace, error_word)
     num_layers, num_kv_heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
     _check_bounds(k_bounds, k_pool, page_size)
     qs = _bht_strides(q, "q")
@@ -729,20 +728,19 @@ def sparse_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
         raise ValueError("q must match the pool's head_dim and dtype")
     _int32_vector(cache_lens, "cache_lens", batch)
     stride, width = _page_rows(page_table, batch)
-    out = _output(out, q, (batch, 1, num_q_heads, head_dim))
+    out = _output(out, q)
     os_ = _bht_strides(out, "out")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     if num_pages < 1:
         raise ValueError("num_pages must be positive")
-    selected = torch.empty((batch, num_kv_heads, num_pages), dtype=torch.int32, device=device)
+    selected = torch.empty((batch, num_kv_heads, num_pages), dtype=torch.int32, device=q.device)
     need = sparse_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_pages, q.dtype)
-    workspace = _scratch(workspace, need, device)
-    with _on(device):
-        rc = _lib.lib().hyt_sparse_attention(
-            q.data_ptr(), _lib.int64_array(qs[:2]), k_pool.data_ptr(), v_pool.data_ptr(),
-            k_bounds.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride, width,
-            cache_lens.data_ptr(), out.data_ptr(), _lib.int64_array(os_[:2]), selected.data_ptr(), batch,
-            num_q_heads, num_kv_heads, head_dim, page_size, dtype_code(q.dtype), scale, num_pages,
-            workspace.data_ptr(), workspace.numel(), _ptr(error_word), _stream_ptr())
+    workspace = _scratch(workspace, need, q.device)
+    rc = _on_device(
+        index, _lib.lib().hyt_sparse_attention, q.data_ptr(), _lib.int64_array(qs[:2]), k_pool.data_ptr(),
+        v_pool.data_ptr(), k_bounds.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride,
+        width, cache_lens.data_ptr(), out.data_ptr(), _lib.int64_array(os_[:2]), selected.data_ptr(), batch,
+        num_q_heads, num_kv_heads, head_dim, page_size, dtype_code(q.dtype), scale, num_pages,
+        workspace.data_ptr(), workspace.numel(), _ptr(error_word))
     _lib.check(rc, "hyt_sparse_attention")
     return out, selected
