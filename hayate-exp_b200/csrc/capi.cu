@@ -1529,6 +1529,8 @@ int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_
   s.q = q;
   s.q_sb = q_strides[0];
   s.q_sh = q_strides[1];
+  const int64_t q_rows[3] = {q_strides[0], q_strides[1], 0};
+  s.q_vec = rows_16b_aligned(q, q_rows) ? 1 : 0;
   s.k_bounds = k_bounds;
   s.layer = layer;
   s.batch = batch;

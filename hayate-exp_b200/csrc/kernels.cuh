@@ -255,6 +255,7 @@ cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t strea
 struct SelectParams {
   const void* q;
   int64_t q_sb, q_sh;
+  int32_t q_vec;  // q's rows start on 16-byte boundaries
   const void* k_bounds;
   int32_t layer, batch, num_q_heads, num_kv_heads, head_dim, page_shift, num_pages;
   const int32_t* page_table;
@@ -264,6 +265,7 @@ struct SelectParams {
   int32_t* selected;     // [batch, H_kv, take] logical pages, ascending, -1 past the last
   int32_t* pages;        // [batch, H_kv, take] the same as physical ids
   int32_t* lens;         // [batch] cached tokens as seen through `pages`
+  int32_t ranked;        // pages a selection can rank (set by run_select_pages)
   int32_t* error_word;
 };
 constexpr int kSelectMaxPages = 16384;  // pages of one request that a selection can rank

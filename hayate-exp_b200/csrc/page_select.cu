@@ -7,15 +7,21 @@
 // select_pages: score(page) = max over the KV group's query heads of
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
 // the most a key of the page can score; the take - 1 best full pages (ties: the lowest page)
-// and the page being written, in ascending order. Which page is read hangs on scores next
-// to each other, so a score must not depend on the order of summation: products of 16-bit
-// values are exact in fp32 (fp32 ones keep their rounding error by an FMA), the sums carry
-// their rounding errors along (Knuth's two-sum, on packed pairs), lanes meet in 64 bits, and
-// the result is rounded once. That costs 5.5 instructions a term; converting to 64 bits term
-// by term took 80 us on 64 requests x 256 pages x 8 KV heads (4 heads a group), this 20.
-// A cluster of 1 to 8 CTAs per (request, KV head) shares the pages out, 16 lanes per page and
-// the bounds read once; the keys (order-preserving 32-bit scores) meet in the first CTA's
-// shared memory, which finds the (take - 1)-th largest 8 bits at a time.
+// and the page being written, in ascending order. A cluster of 1 to 8 CTAs per (request, KV
+// head) shares the pages out; their scores meet in the first CTA's shared memory.
+//
+// Which page is read hangs on scores next to each other, so the choice must not depend on the
+// order of summation: a score is its exact sum rounded once to fp32 (products of 16-bit values
+// are exact in fp32, fp32 ones keep their rounding error by an FMA; the sums carry their
+// rounding errors along, Knuth's two-sum; lanes meet in 64 bits). For 16-bit types only the
+// pages whose place is in doubt are summed that way: all are scored first on the tensor
+// cores (the dot product of [q > 0, q < 0] with [max, min], 8 pages and 8 heads per mma, each
+// bound read once), with the sum of the terms' magnitudes beside it, which bounds the error;
+// pages further than that from the threshold are in or out for certain. Exact sums of every
+// page took 62 us on 64 requests x 256 pages x 8 KV heads x 4 heads, conversions to 64 bits
+// 80; the bounds' bytes need 10.
+//
+// Bound: HBM reads of the bounds on large batches, the chain of barriers on small ones.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -138,13 +144,49 @@ struct PairSum {
   }
 };
 
-// kHeads: query heads scored per pass over a page's bounds.
-template <typename T, int kHeads>
-__global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const SelectParams p) {
+constexpr int kLanes = 16;  // lanes that sum one page exactly
+
+// Key of one head's exact score of a page, on all 16 lanes of the half-warp (both halves call
+// together). lo: the page's bounds.
+template <typename T>
+__device__ __forceinline__ uint32_t exact_key(int head_dim, const T* qh, const T* lo, int l16) {
   constexpr int kPer = 16 / int(sizeof(T));
+  PairSum acc;
+  for (int c = l16; c < head_dim / kPer; c += kLanes) {
+    float fl[kPer], fh[kPer];
+    unpack16<T>(__ldg(reinterpret_cast<const uint4*>(lo) + c), fl);
+    unpack16<T>(__ldg(reinterpret_cast<const uint4*>(lo + head_dim) + c), fh);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float qa = Elem<T>::to_float(qh[c * kPer + e]), qb = Elem<T>::to_float(qh[c * kPer + e + 1]);
+      const uint64_t q2 = f2_pack(qa, qb), x2 = f2_pack(qa >= 0.f ? fh[e] : fl[e], qb >= 0.f ? fh[e + 1] : fl[e + 1]);
+      const uint64_t prod = f2_mul(q2, x2);
+      acc.add(prod);
+      if constexpr (sizeof(T) == 4) acc.e = f2_add(acc.e, f2_fma(q2, x2, f2_mul(prod, f2_pack(-1.f, -1.f))));
+    }
+  }
+  double total = acc.total();
+#pragma unroll
+  for (int off = kLanes / 2; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  return score_key(float(total));
+}
+
+// The tensor cores' fp32 accumulation of 16 products and the running sum may drop bits below
+// 2^-23 of the largest of them; 4 steps of 17 terms per 32 dims keep the error of a score
+// under 2^-20 of the sum of the terms' magnitudes per dim, with a factor of 3 to spare.
+__device__ __forceinline__ float score_slack(int head_dim, float magnitude) {
+  return magnitude * float((head_dim + 31) / 32 * 32) * 9.5367432e-7f;
+}
+
+// kSteps: 16-byte chunks of a bounds row per lane of a quad (head_dim <= 32 kSteps).
+template <typename T, int kSteps>
+__global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const SelectParams p) {
+  constexpr bool kTensor = sizeof(T) == 2;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int kWarps = kSelectThreads / 32;
-  constexpr int kLanes = 16;  // per page
-  extern __shared__ __align__(16) uint32_t keys[];  // [last], the first CTA's are used
+  extern __shared__ __align__(16) uint32_t keys[];  // [last], then as many page ids and list entries; the
+  int32_t* ids = reinterpret_cast<int32_t*>(keys) + p.ranked;  // first CTA's are used
+  int32_t* doubtful = ids + p.ranked;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -152,10 +194,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   const int b = unit / p.num_kv_heads, g = unit - b * p.num_kv_heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int D = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
-  __shared__ int hist[256];
-  __shared__ int warp_count[kWarps];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+  __shared__ int counts[2][3][kWarps], warp_count[kWarps];
+  __shared__ int s_doubtful;
+  __shared__ int s_magnitude;  // largest sum of magnitudes of a score, as the bits of a float
   launch_dependents();  // the attention kernel may start up; it waits for this grid's results
 
   const int64_t out_row = (int64_t(b) * p.num_kv_heads + g) * p.take;
@@ -181,135 +222,271 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
     return;
   }
 
-  // ---- scores of the full pages 0 .. last - 1: this CTA's share, 16 lanes per page
-  {
-    if (ranks > 1) cluster.sync();  // the first CTA has started: its shared memory may be written
-    uint32_t* to = cluster.map_shared_rank(keys, 0);
-    const T* bounds = static_cast<const T*>(p.k_bounds) +
-                      (int64_t(p.layer) * p.num_kv_heads + g) * p.num_pages * 2 * D;
-    const T* q0 = static_cast<const T*>(p.q) + int64_t(b) * p.q_sb + int64_t(g) * group * p.q_sh;
-    const int sub = lane / kLanes, l16 = lane % kLanes, chunks = D / kPer;
+  // ---- scores of the full pages 0 .. last - 1: this CTA's share
+  const T* bounds = static_cast<const T*>(p.k_bounds) + (int64_t(p.layer) * p.num_kv_heads + g) * p.num_pages * 2 * D;
+  const T* q0 = static_cast<const T*>(p.q) + int64_t(b) * p.q_sb + int64_t(g) * group * p.q_sh;
+  auto page_at = [&](int i) {  // physical page, -1 past the end or refused
+    if (i >= last) return -1;
+    const int32_t page = table[i];
+    if (page >= 0 && page < p.num_pages) return int(page);
+    flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
+    return -1;
+  };
+  if (tid == 0) s_magnitude = 0, s_doubtful = 0;
+  // the first CTA has started and cleared its magnitude: its shared memory may be written
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+  uint32_t* to = cluster.map_shared_rank(keys, 0);
+  int32_t* to_id = cluster.map_shared_rank(ids, 0);
+  if constexpr (kTensor) {
+    // 8 pages per warp and turn: lane (n = lane / 4, j = lane % 4) reads 16-byte chunks j + 4 t
+    // of page n's two rows; a chunk's words 0, 1 and 2, 3 are the B operands of two k = 16
+    // steps, and q's chunks, read the same way for head n, the A operands: the order of
+    // the dims differs from memory's, alike on both sides
+    const int n = lane >> 2, j = lane & 3, chunks = D / 8;
+    const int first = (rank * kWarps + warp) * 8, stride = ranks * kWarps * 8;
+    float magnitude = 0.f;
+    int page = page_at(first + n);
+    for (int i0 = first; i0 < last; i0 += stride) {
+      const uint4* lo = reinterpret_cast<const uint4*>(bounds + int64_t(max(page, 0)) * 2 * D);
+      uint4 l4[kSteps], h4[kSteps];  // all loads of the turn go out together
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const int c = j + 4 * t;
+        l4[t] = h4[t] = make_uint4(0u, 0u, 0u, 0u);
+        if (c < chunks) {
+          l4[t] = __ldg(lo + c);
+          h4[t] = __ldg(lo + chunks + c);
+        }
+      }
+      const int next = page_at(i0 + stride + n);
+      float top[2] = {-INFINITY, -INFINITY};  // best over the heads, pages 2 j and 2 j + 1
+      bool nan[2] = {false, false};
+      for (int h0 = 0; h0 < group; h0 += 8) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+        const T* qh = q0 + int64_t(min(h0 + n, group - 1)) * p.q_sh;
+        uint4 q4[kSteps];
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+          const int c = j + 4 * t;
+          q4[t] = make_uint4(0u, 0u, 0u, 0u);
+          if (c >= chunks) continue;
+          if (p.q_vec) {
+            q4[t] = __ldg(reinterpret_cast<const uint4*>(qh) + c);
+          } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(qh + c * 8);
+            q4[t].x = e[0] | (uint32_t(e[1]) << 16);
+            q4[t].y = e[2] | (uint32_t(e[3]) << 16);
+            q4[t].z = e[4] | (uint32_t(e[5]) << 16);
+            q4[t].w = e[6] | (uint32_t(e[7]) << 16);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+          const uint32_t lw[4] = {l4[t].x, l4[t].y, l4[t].z, l4[t].w}, hw[4] = {h4[t].x, h4[t].y, h4[t].z, h4[t].w};
+          const uint32_t qw[4] = {q4[t].x, q4[t].y, q4[t].z, q4[t].w};
+          constexpr uint32_t kAbs = 0x7FFF7FFFu;
+#pragma unroll
+          for (int w = 0; w < 4; w += 2) {
+            uint32_t plus[4] = {0u, 0u, 0u, 0u}, minus[4] = {0u, 0u, 0u, 0u};  // rows 8 .. 15 unused
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t sign = qw[w + k] & 0x80008000u, mask = (sign >> 15) * 0xFFFFu;  // ones where q < 0
+              plus[2 * k] = qw[w + k] & ~mask;
+              minus[2 * k] = qw[w + k] & mask;
+            }
+            mma_16816<kHalf>(s, plus, hw[w], hw[w + 1]);
+            mma_16816<kHalf>(s, minus, lw[w], lw[w + 1]);
+            mma_16816<kHalf>(m, plus, hw[w] & kAbs, hw[w + 1] & kAbs);
+            const uint32_t minus_abs[4] = {minus[0] & kAbs, 0u, minus[2] & kAbs, 0u};
+            mma_16816<kHalf>(m, minus_abs, lw[w] & kAbs, lw[w + 1] & kAbs);
+          }
+        }
+        if (h0 + n < group) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            nan[e] |= isnan(s[e]);
+            top[e] = fmaxf(top[e], s[e]);
+            if (i0 + 2 * j + e < last) magnitude = max_nan(magnitude, m[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {  // over the heads
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], off));
+          nan[e] |= __shfl_xor_sync(0xffffffffu, nan[e] ? 1 : 0, off) != 0;
+        }
+      }
+      const int even = __shfl_sync(0xffffffffu, page, 8 * j), odd = __shfl_sync(0xffffffffu, page, 8 * j + 4);
+      if (n < 2) {
+        const int i = i0 + 2 * j + n, id = n == 0 ? even : odd;
+        const uint32_t key = (n == 0 ? nan[0] : nan[1]) ? 0xFFFFFFFFu : score_key(n == 0 ? top[0] : top[1]);
+        if (i < last) {
+          to[i] = id < 0 ? 0u : key;
+          to_id[i] = id;
+        }
+      }
+      page = next;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) magnitude = max_nan(magnitude, __shfl_xor_sync(0xffffffffu, magnitude, off));
+    // bits of floats >= 0 are ordered like the floats, NaN above all
+    if (lane == 0) atomicMax(cluster.map_shared_rank(&s_magnitude, 0), __float_as_int(magnitude) & 0x7FFFFFFF);
+  } else {
+    const int l16 = lane % kLanes;
     constexpr int kPages = kWarps * (32 / kLanes);  // pages a CTA scores at a time
     for (int i0 = rank * kPages; i0 < last; i0 += ranks * kPages) {
-      const int i = i0 + warp * (32 / kLanes) + sub;
-      int32_t page = -1;
-      if (i < last) {
-        page = table[i];
-        if (page < 0 || page >= p.num_pages) {
-          if (l16 == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
-          page = -1;
-        }
+      const int i = i0 + warp * (32 / kLanes) + lane / kLanes;
+      const int page = page_at(i);
+      uint32_t key = 0u;
+      for (int h = 0; h < group; ++h)
+        key = max(key, exact_key<T>(D, q0 + int64_t(h) * p.q_sh, bounds + int64_t(max(page, 0)) * 2 * D, l16));
+      if (i < last && l16 == 0) {
+        to[i] = page < 0 ? 0u : key;
+        to_id[i] = page;
       }
-      const T* lo = bounds + int64_t(max(page, 0)) * 2 * D;
-      float best = -INFINITY;
-      bool nan = false;
-      for (int h0 = 0; h0 < group; h0 += kHeads) {
-        PairSum acc[kHeads];
-        for (int c = l16; c < chunks; c += kLanes) {
-          const uint4 lraw = __ldg(reinterpret_cast<const uint4*>(lo) + c);
-          const uint4 hraw = __ldg(reinterpret_cast<const uint4*>(lo + D) + c);
-          const uint32_t lw[4] = {lraw.x, lraw.y, lraw.z, lraw.w}, hw[4] = {hraw.x, hraw.y, hraw.z, hraw.w};
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) {
-            if (h0 + h >= group) break;
-            const T* qh = q0 + int64_t(h0 + h) * p.q_sh + c * kPer;
-            if constexpr (sizeof(T) == 2) {
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const float qa = Elem<T>::to_float(qh[2 * w]), qb = Elem<T>::to_float(qh[2 * w + 1]);
-                const uint32_t m = (qa >= 0.f ? 0x0000FFFFu : 0u) | (qb >= 0.f ? 0xFFFF0000u : 0u);
-                const uint32_t x = (hw[w] & m) | (lw[w] & ~m);
-                const T* xe = reinterpret_cast<const T*>(&x);
-                acc[h].add(f2_mul(f2_pack(qa, qb), f2_pack(Elem<T>::to_float(xe[0]), Elem<T>::to_float(xe[1]))));
-              }
-            } else {
-#pragma unroll
-              for (int w = 0; w < 4; w += 2) {
-                const float qa = qh[w], qb = qh[w + 1];
-                const uint64_t q2 = f2_pack(qa, qb);
-                const uint64_t x2 = f2_pack(__uint_as_float(qa >= 0.f ? hw[w] : lw[w]),
-                                            __uint_as_float(qb >= 0.f ? hw[w + 1] : lw[w + 1]));
-                const uint64_t prod = f2_mul(q2, x2);
-                acc[h].add(prod);
-                acc[h].e = f2_add(acc[h].e, f2_fma(q2, x2, f2_mul(prod, f2_pack(-1.f, -1.f))));
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          double total = acc[h].total();
-#pragma unroll
-          for (int off = kLanes / 2; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-          if (h0 + h < group) {
-            const float x = float(total);
-            nan |= isnan(x);
-            best = fmaxf(best, x);
-          }
-        }
-      }
-      if (i < last && l16 == 0) to[i] = page < 0 ? 0u : (nan ? 0xFFFFFFFFu : score_key(best));
     }
   }
-  cluster.sync();
-  if (rank != 0) return;
+  if (ranks > 1) {
+    cluster.sync();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
 
-  // ---- the (take - 1)-th largest key, 8 bits at a time
-  int need = p.take - 1;  // of the keys that match the prefix so far, this many are wanted
-  uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+  // counts over the CTA of what each thread counted for three questions; one barrier
+  int step = 0;
+  auto count3 = [&](int a, int b3, int c, int (&all)[3]) {
+    const int mine[3] = {__reduce_add_sync(0xffffffffu, a), __reduce_add_sync(0xffffffffu, b3),
+                         __reduce_add_sync(0xffffffffu, c)};
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (lane == k) counts[step & 1][k][warp] = mine[k];
     __syncthreads();
-    for (int i = tid; i < last; i += kSelectThreads)
-      if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      all[k] = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) all[k] += counts[step & 1][k][w];
+    }
+    ++step;
+  };
+  const int want = p.take - 1;  // 0 .. last
+  // The largest value that at least `want` keys reach (want >= 1), two bits at a time from the
+  // highest in which the keys differ: they are scores of one query, so a histogram of their
+  // leading bits would pile up in one bin. `exactly`: ended early, exactly `want` keys reach it.
+  bool exactly = false;
+  auto threshold_of = [&]() {
+    uint32_t ones = 0xFFFFFFFFu, any = 0u;
+    for (int i = tid; i < last; i += kSelectThreads) ones &= keys[i], any |= keys[i];
+    ones = __reduce_and_sync(0xffffffffu, ones);
+    any = __reduce_or_sync(0xffffffffu, any);
+    if (lane == 0) counts[step & 1][0][warp] = int(ones), counts[step & 1][1][warp] = int(any);
     __syncthreads();
-    if (warp == 0) {  // lane l: bins 255 - 8 l .. 248 - 8 l, from the top
-      int bin[8], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        bin[j] = hist[255 - lane * 8 - j];
-        sum += bin[j];
+    for (int w = 0; w < kWarps; ++w) ones &= uint32_t(counts[step & 1][0][w]), any |= uint32_t(counts[step & 1][1][w]);
+    ++step;
+    exactly = false;
+    if (ones == any) return ones;  // all keys are the same
+    int bit = (31 - __clz(ones ^ any)) | 1;  // the upper bit of the pair that holds the highest difference
+    uint32_t t = bit == 31 ? 0u : ones & ~((2u << bit) - 1u);
+    for (; bit >= 0 && !exactly; bit -= 2) {
+      const uint32_t unit = 1u << (bit - 1);
+      int c[3] = {0, 0, 0}, all[3];
+      for (int i = tid; i < last; i += kSelectThreads) {
+        const uint32_t key = keys[i];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) c[k] += key >= t + unit * uint32_t(k + 1) ? 1 : 0;
       }
-      int scan = sum;
+      count3(c[0], c[1], c[2], all);
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, scan, off);
-        if (lane >= off) scan += v;
-      }
-      int above = scan - sum;
-      if (above < need && need <= scan) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (above < need && need <= above + bin[j]) {
-            s_prefix = prefix | (uint32_t(255 - lane * 8 - j) << shift);
-            s_need = need - above;
-          }
-          above += bin[j];
+      for (int k = 2; k >= 0; --k) {
+        if (all[k] >= want) {
+          t += unit * uint32_t(k + 1);
+          exactly = all[k] == want;
+          break;
         }
       }
     }
+    return t;
+  };
+  if (kTensor && want > 0) {
+    // scores within the error of the want-th best are in doubt: those are summed exactly. Those
+    // above count as the best there is, those below as the worst
+    uint32_t t = threshold_of();
+    if (exactly) {  // the smallest key that reaches t, instead of t itself
+      uint32_t least = 0xFFFFFFFFu;
+      for (int i = tid; i < last; i += kSelectThreads)
+        if (keys[i] >= t) least = min(least, keys[i]);
+      least = __reduce_min_sync(0xffffffffu, least);
+      if (lane == 0) warp_count[warp] = int(least);
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) least = min(least, uint32_t(warp_count[w]));
+      t = least;
+    }
+    const float score = __uint_as_float((t & 0x80000000u) ? (t & 0x7FFFFFFFu) : ~t);
+    const float slack = 2.f * score_slack(D, __int_as_float(s_magnitude));
+    const uint32_t above0 = score_key(score + slack), below0 = score_key(score - slack);
+    int c[3] = {0, 0, 0}, all[3];
+    for (int i = tid; i < last; i += kSelectThreads) {
+      const uint32_t key = keys[i];
+      c[0] += key == 0xFFFFFFFFu ? 1 : 0;
+      c[1] += key > above0 ? 1 : 0;
+      c[2] += key >= below0 ? 1 : 0;
+    }
+    count3(c[0], c[1], c[2], all);
+    // a NaN key may hide a score of any size (zero times an infinite bound of the other side)
+    const bool known = isfinite(score) && isfinite(slack) && all[0] == 0;
+    const uint32_t above = known ? above0 : 0xFFFFFFFFu, below = known ? below0 : 0u;
+    const bool settled = known && all[2] == want;  // everything in doubt is in
+    for (int i = tid; i < last; i += kSelectThreads) {
+      const uint32_t key = keys[i];
+      // refused pages (key 0) stay below everything, NaN keys are summed again
+      const bool doubt = key != 0u && ((key >= below && key <= above) || key == 0xFFFFFFFFu);
+      if (doubt && !settled) doubtful[atomicAdd(&s_doubtful, 1)] = i;
+      keys[i] = doubt ? (settled ? 0xFFFFFFFFu : 0u) : (key > above ? 0xFFFFFFFFu : 0u);
+    }
     __syncthreads();
-    prefix = s_prefix;
-    need = s_need;
-    mask |= 255u << shift;
+    const int tasks = s_doubtful * group;  // (page, head), a half-warp each; in any order
+    for (int task0 = 0; task0 < tasks; task0 += kWarps * 2) {
+      const int task = min(task0 + warp * 2 + lane / kLanes, tasks - 1), which = task / group;
+      const int i = doubtful[which], h = task - which * group;
+      const uint32_t key = exact_key<T>(D, q0 + int64_t(h) * p.q_sh, bounds + int64_t(ids[i]) * 2 * D, lane % kLanes);
+      if (lane % kLanes == 0) atomicMax(&keys[i], key);
+    }
+    __syncthreads();
   }
-  // pages with key > prefix are in; of those equal to it the first `need`
+  uint32_t threshold = 0xFFFFFFFFu;  // keys above it are in, and the first `need` of those equal to it
+  int need = 0;
+  if (want > 0) {
+    threshold = threshold_of();
+    if (exactly) {
+      --threshold;  // exactly `want` keys are above threshold - 1 (threshold >= 1)
+    } else {
+      int c = 0, all[3];
+      for (int i = tid; i < last; i += kSelectThreads) c += keys[i] > threshold ? 1 : 0;
+      count3(c, 0, 0, all);
+      need = want - all[0];
+    }
+  }
 
   // ---- emit in ascending order: warp w takes pages [w * share, (w + 1) * share)
   const int share = (last + kWarps * 32 - 1) / (kWarps * 32) * 32;
   const int first = min(warp * share, last), end = min(first + share, last);
   int equal = 0;
   for (int i = first + lane; i < first + share; i += 32)
-    equal += __popc(__ballot_sync(0xffffffffu, i < end && keys[i] == prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, i < end && keys[i] == threshold));
   if (lane == 0) warp_count[warp] = equal;
   __syncthreads();
   int equal_before = 0;  // equal keys before this warp's
   for (int w = 0; w < warp; ++w) equal_before += warp_count[w];
   __syncthreads();
-  const bool any = p.take > 1;
   int mine = 0, r = equal_before;
   for (int i = first + lane; i < first + share; i += 32) {
-    const bool eq = any && i < end && keys[i] == prefix, gt = any && i < end && keys[i] > prefix;
+    const bool eq = i < end && keys[i] == threshold, gt = i < end && keys[i] > threshold;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
     const bool in = gt || (eq && r + __popc(eqs & ((1u << lane) - 1)) < need);
     mine += __popc(__ballot_sync(0xffffffffu, in));
@@ -321,14 +498,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   for (int w = 0; w < warp; ++w) at += warp_count[w];
   r = equal_before;
   for (int i = first + lane; i < first + share; i += 32) {
-    const bool eq = any && i < end && keys[i] == prefix, gt = any && i < end && keys[i] > prefix;
+    const bool eq = i < end && keys[i] == threshold, gt = i < end && keys[i] > threshold;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
     const bool in = gt || (eq && r + __popc(eqs & ((1u << lane) - 1)) < need);
     const uint32_t ins = __ballot_sync(0xffffffffu, in);
     if (in) {
       const int slot = at + __popc(ins & ((1u << lane) - 1));
       p.selected[out_row + slot] = i;
-      p.pages[out_row + slot] = table[i];
+      p.pages[out_row + slot] = ids[i];
     }
     at += __popc(ins);
     r += __popc(eqs);
@@ -352,9 +529,11 @@ cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t strea
   return cudaGetLastError();
 }
 
-cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stream) {
-  const int group = p.num_q_heads / p.num_kv_heads, units = p.batch * p.num_kv_heads;
+cudaError_t run_select_pages(const SelectParams& params, int dtype, cudaStream_t stream) {
+  SelectParams p = params;
+  const int units = p.batch * p.num_kv_heads;
   const int ranked = p.table_width < kSelectMaxPages ? p.table_width : kSelectMaxPages;
+  p.ranked = ranked;
   // CTAs per unit: enough to give every SM two, none with less than 32 pages
   int ranks = 1;
   while (ranks < 8 && units * ranks < 2 * 148 && ranked >= 64 * ranks) ranks *= 2;
@@ -365,7 +544,7 @@ cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stre
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(units * ranks));
   config.blockDim = dim3(kSelectThreads);
-  config.dynamicSmemBytes = size_t(ranked) * 4;
+  config.dynamicSmemBytes = size_t(ranked) * 12;
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;
@@ -373,16 +552,12 @@ cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stre
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(config.dynamicSmemBytes));
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&config, kernel, p);
   };
-  auto heads = [&](auto type) {
-    using T = decltype(type);
-    if (group == 1) return launch(select_pages_kernel<T, 1>);
-    if (group == 2) return launch(select_pages_kernel<T, 2>);
-    return launch(select_pages_kernel<T, 4>);
-  };
   switch (dtype) {
-    case HYT_DTYPE_BF16: return heads(__nv_bfloat16{});
-    case HYT_DTYPE_F16: return heads(__half{});
-    default: return heads(float{});
+    case HYT_DTYPE_BF16:
+      return p.head_dim <= 128 ? launch(select_pages_kernel<__nv_bfloat16, 4>) : launch(select_pages_kernel<__nv_bfloat16, 8>);
+    case HYT_DTYPE_F16:
+      return p.head_dim <= 128 ? launch(select_pages_kernel<__half, 4>) : launch(select_pages_kernel<__half, 8>);
+    default: return launch(select_pages_kernel<float, 1>);
   }
 }
 

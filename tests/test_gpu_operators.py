@@ -554,3 +554,24 @@ def test_wrappers_check_their_arguments():
         bad[index] = value
         with pytest.raises(kind):
             ops.sparse_attention(*bad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("seed", range(6))
+def test_sparse_attention_scores_that_are_nearly_equal(dtype, seed):
+    """Bounds whose scores differ in their last bits only, and exact ties among them: the pages
+    taken are those of the sums in 64 bits, whatever order they are summed in."""
+    s = Sparse([200 * 128 + 7, 90 * 128], 40, dtype, seed=seed, hq=8, hkv=2)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    base = torch.randn((1, 2, 1, 2, 128), generator=gen, device="cuda")
+    lo, hi = base.amin(dim=3, keepdim=True), base.amax(dim=3, keepdim=True)
+    bounds = torch.cat([lo, hi], dim=3).to(dtype).expand(s.bounds.shape).contiguous()
+    # one element of each page moves by one step or not at all
+    pages = bounds.shape[2]
+    where = torch.randint(0, 128, (pages,), generator=gen, device="cuda")
+    side = torch.randint(0, 2, (pages,), generator=gen, device="cuda")
+    bits = bounds.view(torch.int16)
+    moved = torch.randint(0, 2, (pages,), generator=gen, device="cuda").to(torch.int16)
+    bits[0, :, torch.arange(pages, device="cuda"), side, where] += moved
+    s.bounds = bounds
+    s.check()
