@@ -674,6 +674,71 @@ int move_params(void* k_pool, void* v_pool, int32_t num_layers, int32_t num_kv_h
   return HYT_OK;
 }
 
+int norm_rope_scatter_packed(const void* q, const void* k, const void* v,
+                                 const int64_t* qkv_strides, const void* q_norm_weight,
+                                 const void* k_norm_weight, float eps, const float* cos,
+                                 const float* sin, int32_t rope_positions, void* q_out,
+                                 const int64_t* q_out_strides, void* k_pool, void* v_pool,
+                                 int32_t num_layers, int32_t layer, int64_t capacity_tokens,
+                                 const int32_t* page_table, int32_t page_table_stride,
+                                 const int32_t* cache_lens, const int32_t* q_start,
+                                 const int32_t* token_request, const int32_t* token_depth, int32_t batch,
+                                 int32_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int32_t page_size, int32_t dtype,
+                                 int32_t* error_word, void* stream) {
+  g_last_error.clear();
+  if (!q || !k || !v || !qkv_strides || !q_norm_weight || !k_norm_weight || !cos || !sin ||
+      !q_out || !q_out_strides || !k_pool || !v_pool || !page_table || !cache_lens || !q_start ||
+      !token_request)
+    return fail(HYT_ERR_INVALID, "null pointer argument");
+  if (total_tokens < 1) return fail(HYT_ERR_INVALID, "total_tokens must be positive");
+  Geometry g{num_layers, layer, capacity_tokens, page_table_stride, batch, 1,
+             num_q_heads, num_kv_heads, head_dim, page_size, dtype};
+  int rc = check_geometry(g);
+  if (rc != HYT_OK) return rc;
+  if (head_dim != 128) return fail(HYT_ERR_UNSUPPORTED, "fused norm/RoPE/scatter needs head_dim 128");
+  if (rope_positions < 1) return fail(HYT_ERR_INVALID, "rope_positions must be positive");
+  rc = check_norm_rope_alignment(dtype, q, k, v, q_out, qkv_strides, 6, q_out_strides, 2,
+                                 q_norm_weight, k_norm_weight, k_pool, v_pool, cos, sin);
+  if (rc != HYT_OK) return rc;
+  hyt::NormRopeParams p;
+  p.q = q;
+  p.q_sb = 0; p.q_st = qkv_strides[0]; p.q_sh = qkv_strides[1];
+  p.k = k;
+  p.k_sb = 0; p.k_st = qkv_strides[2]; p.k_sh = qkv_strides[3];
+  p.v = v;
+  p.v_sb = 0; p.v_st = qkv_strides[4]; p.v_sh = qkv_strides[5];
+  p.q_out = q_out;
+  p.o_sb = 0; p.o_st = q_out_strides[0]; p.o_sh = q_out_strides[1];
+  p.q_norm_weight = q_norm_weight;
+  p.k_norm_weight = k_norm_weight;
+  p.eps = eps;
+  p.cos = cos;
+  p.sin = sin;
+  p.rope_positions = rope_positions;
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.capacity = capacity_tokens;
+  p.layer = layer;
+  p.page_table = page_table;
+  p.page_table_stride = page_table_stride;
+  p.cache_lens = cache_lens;
+  p.batch = batch;
+  p.query_len = 1;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.page_shift = log2_int(page_size);
+  p.num_pages = int32_t(capacity_tokens / page_size);
+  p.error_word = error_word;
+  p.q_start = q_start;
+  p.token_request = token_request;
+  p.total_tokens = total_tokens;
+  p.token_depth = token_depth;
+  cudaError_t err = hyt::run_norm_rope_scatter(p, dtype, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "packed norm/RoPE/scatter launch");
+  return HYT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -780,6 +845,7 @@ int hyt_norm_rope_scatter(const void* q, const void* k, const void* v, const int
   p.q_start = nullptr;
   p.token_request = nullptr;
   p.total_tokens = 0;
+  p.token_depth = nullptr;
   cudaError_t err = hyt::run_norm_rope_scatter(p, dtype, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "norm/RoPE/scatter launch");
   return HYT_OK;
@@ -1028,56 +1094,36 @@ int hyt_norm_rope_scatter_packed(const void* q, const void* k, const void* v,
                                  int32_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
                                  int32_t head_dim, int32_t page_size, int32_t dtype,
                                  int32_t* error_word, void* stream) {
-  g_last_error.clear();
-  if (!q || !k || !v || !qkv_strides || !q_norm_weight || !k_norm_weight || !cos || !sin ||
-      !q_out || !q_out_strides || !k_pool || !v_pool || !page_table || !cache_lens || !q_start ||
-      !token_request)
+  return norm_rope_scatter_packed(q, k, v, qkv_strides, q_norm_weight, k_norm_weight, eps, cos,
+                                  sin, rope_positions, q_out, q_out_strides, k_pool, v_pool,
+                                  num_layers, layer, capacity_tokens, page_table,
+                                  page_table_stride, cache_lens, q_start, token_request, nullptr,
+                                  batch, total_tokens, num_q_heads, num_kv_heads, head_dim,
+                                  page_size, dtype, error_word, stream);
+}
+
+int hyt_norm_rope_scatter_tree(const void* q, const void* k, const void* v,
+                                 const int64_t* qkv_strides, const void* q_norm_weight,
+                                 const void* k_norm_weight, float eps, const float* cos,
+                                 const float* sin, int32_t rope_positions, void* q_out,
+                                 const int64_t* q_out_strides, void* k_pool, void* v_pool,
+                                 int32_t num_layers, int32_t layer, int64_t capacity_tokens,
+                                 const int32_t* page_table, int32_t page_table_stride,
+                                 const int32_t* cache_lens, const int32_t* q_start,
+                                 const int32_t* token_request, const int32_t* token_depth, int32_t batch,
+                                 int32_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int32_t page_size, int32_t dtype,
+                                 int32_t* error_word, void* stream) {
+  if (token_depth == nullptr) {
+    g_last_error.clear();
     return fail(HYT_ERR_INVALID, "null pointer argument");
-  if (total_tokens < 1) return fail(HYT_ERR_INVALID, "total_tokens must be positive");
-  Geometry g{num_layers, layer, capacity_tokens, page_table_stride, batch, 1,
-             num_q_heads, num_kv_heads, head_dim, page_size, dtype};
-  int rc = check_geometry(g);
-  if (rc != HYT_OK) return rc;
-  if (head_dim != 128) return fail(HYT_ERR_UNSUPPORTED, "fused norm/RoPE/scatter needs head_dim 128");
-  if (rope_positions < 1) return fail(HYT_ERR_INVALID, "rope_positions must be positive");
-  rc = check_norm_rope_alignment(dtype, q, k, v, q_out, qkv_strides, 6, q_out_strides, 2,
-                                 q_norm_weight, k_norm_weight, k_pool, v_pool, cos, sin);
-  if (rc != HYT_OK) return rc;
-  hyt::NormRopeParams p;
-  p.q = q;
-  p.q_sb = 0; p.q_st = qkv_strides[0]; p.q_sh = qkv_strides[1];
-  p.k = k;
-  p.k_sb = 0; p.k_st = qkv_strides[2]; p.k_sh = qkv_strides[3];
-  p.v = v;
-  p.v_sb = 0; p.v_st = qkv_strides[4]; p.v_sh = qkv_strides[5];
-  p.q_out = q_out;
-  p.o_sb = 0; p.o_st = q_out_strides[0]; p.o_sh = q_out_strides[1];
-  p.q_norm_weight = q_norm_weight;
-  p.k_norm_weight = k_norm_weight;
-  p.eps = eps;
-  p.cos = cos;
-  p.sin = sin;
-  p.rope_positions = rope_positions;
-  p.k_pool = k_pool;
-  p.v_pool = v_pool;
-  p.capacity = capacity_tokens;
-  p.layer = layer;
-  p.page_table = page_table;
-  p.page_table_stride = page_table_stride;
-  p.cache_lens = cache_lens;
-  p.batch = batch;
-  p.query_len = 1;
-  p.num_q_heads = num_q_heads;
-  p.num_kv_heads = num_kv_heads;
-  p.page_shift = log2_int(page_size);
-  p.num_pages = int32_t(capacity_tokens / page_size);
-  p.error_word = error_word;
-  p.q_start = q_start;
-  p.token_request = token_request;
-  p.total_tokens = total_tokens;
-  cudaError_t err = hyt::run_norm_rope_scatter(p, dtype, static_cast<cudaStream_t>(stream));
-  if (err != cudaSuccess) return cuda_fail(err, "packed norm/RoPE/scatter launch");
-  return HYT_OK;
+  }
+  return norm_rope_scatter_packed(q, k, v, qkv_strides, q_norm_weight, k_norm_weight, eps, cos,
+                                  sin, rope_positions, q_out, q_out_strides, k_pool, v_pool,
+                                  num_layers, layer, capacity_tokens, page_table,
+                                  page_table_stride, cache_lens, q_start, token_request,
+                                  token_depth, batch, total_tokens, num_q_heads, num_kv_heads,
+                                  head_dim, page_size, dtype, error_word, stream);
 }
 
 static int packed_attention(const void* q, const int64_t* q_strides, const void* k_pool,

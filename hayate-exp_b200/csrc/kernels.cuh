@@ -174,6 +174,9 @@ struct NormRopeParams {
   const int32_t* q_start;
   const int32_t* token_request;
   int32_t total_tokens;
+  // Drafted tree (token_depth != nullptr, packed): token i is rotated at position
+  // cache_lens[b] + token_depth[i]; its slot stays cache_lens[b] + i - q_start[b].
+  const int32_t* token_depth;
 };
 cudaError_t run_norm_rope_scatter(const NormRopeParams& p, int dtype, cudaStream_t stream);
 

@@ -13,7 +13,8 @@
 // fp32 products of that rounded value with the fp32 tables (separate multiply and add,
 // as torch evaluates them) and is rounded once more.
 //
-// Packed batches (token_request set) look each token's request and position up.
+// Packed batches (token_request set) look each token's request and position up; nodes of a
+// drafted tree (token_depth set) are rotated at their depth past the context.
 //
 // One CTA per token, one half-warp per head row at a time; each lane holds 8 consecutive
 // features, so the rotation partner (feature i +/- 64) sits in lane ^ 8. HBM-bound: every
@@ -145,14 +146,16 @@ __global__ void __launch_bounds__(kWarps * 32, 4) norm_rope_scatter_kernel(const
   const int64_t o_tok = packed ? int64_t(token) * p.o_st : b * p.o_sb + int64_t(t) * p.o_st;
   const int pos = p.cache_lens[b] + t;
 
-  // rotation at `pos` (q and k rows) and the pool slot of `pos` (k and v rows)
-  const bool rope_ok = pos >= 0 && pos < p.rope_positions;
+  // rotation at `pos` (a drafted node: at its depth; q and k rows) and the pool slot of `pos`
+  // (k and v rows)
+  const int rope_pos = p.token_depth != nullptr ? p.cache_lens[b] + p.token_depth[token] : pos;
+  const bool rope_ok = rope_pos >= 0 && rope_pos < p.rope_positions;
   uint64_t c2[4], s2[4];
   {
     float c[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sn[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (rope_ok) {
-      load8<float>(p.cos + int64_t(pos) * 128 + d0, c);
-      load8<float>(p.sin + int64_t(pos) * 128 + d0, sn);
+      load8<float>(p.cos + int64_t(rope_pos) * 128 + d0, c);
+      load8<float>(p.sin + int64_t(rope_pos) * 128 + d0, sn);
     } else if (threadIdx.x == 0) {
       flag_error(p.error_word, HYT_DEVERR_TABLE_RANGE);
     }

@@ -63,6 +63,10 @@ SIGNATURES = {
                                                     _c_i32, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_p,
                                                     _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
                                                     _c_i32, _c_p, _c_p]),
+    "hyt_norm_rope_scatter_tree": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_f32, _c_p, _c_p,
+                                                  _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i64,
+                                                  _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32,
+                                                  _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p, _c_p]),
     "hyt_paged_attention_packed": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i64, _c_p,
                                                   _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32,
                                                   _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_p,

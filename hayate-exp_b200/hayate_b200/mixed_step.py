@@ -27,14 +27,16 @@ from .paged_cache import PagedKVBatch
 MAX_PREFILL_BATCH = 8  # hayate/engine/constants.py:11
 
 
-def packed_forward(model, token_ids: torch.Tensor, batch: PagedKVBatch,
-                   sample_rows: torch.Tensor) -> torch.Tensor:
+def packed_forward(model, token_ids: torch.Tensor, batch: PagedKVBatch, sample_rows: torch.Tensor,
+                   num_pages: int | None = None) -> torch.Tensor:
     """Run ``model`` (a hayate ``Qwen3Model``) over a packed batch's tokens.
 
     ``token_ids`` is ``[N]`` (the batch's token axis), ``sample_rows`` the rows whose
     next-token scores are wanted. Returns ``[len(sample_rows), vocab]`` scores, computed
     like ``Qwen3Model.forward`` (``hayate/model/qwen.py:69-175`` with
-    ``block.py`` / ``attention.py``) for those rows.
+    ``block.py`` / ``attention.py``) for those rows. A batch of drafted trees
+    (``begin_tree_batch``) runs the same way. ``num_pages``: a decode step that attends that
+    many pages per KV head (``PagedKVBatch.attend_pages``) instead of the whole context.
     """
     n = token_ids.numel()
     x = model.embed_tokens(token_ids).unsqueeze(0)
@@ -48,7 +50,11 @@ def packed_forward(model, token_ids: torch.Tensor, batch: PagedKVBatch,
         eps = attn.q_norm.eps if attn.q_norm.eps is not None else 1e-6
         q = batch.prepare_layer(layer_idx, q, k, v, attn.q_norm.weight, attn.k_norm.weight,
                                 model.cos, model.sin, eps)
-        context = batch.attend_layer(q, layer_idx).transpose(1, 2).reshape(1, n, -1)
+        if num_pages is None:
+            context = batch.attend_layer(q, layer_idx)
+        else:
+            context, _ = batch.attend_pages(q, layer_idx, num_pages)
+        context = context.transpose(1, 2).reshape(1, n, -1)
         x = attn.o_proj(context) + shortcut
         shortcut = x
         x = block.mlp(block.post_attention_layernorm(x)) + shortcut
@@ -121,12 +127,16 @@ class DecodeGraphs:
     the tokens and the page metadata into the graph's buffers and replays it. Requests
     beyond the real batch are padding rows on the manager's scratch page, their scores
     discarded. Sampling, ``finalize`` and the page bookkeeping are ``decode_batch``'s
-    (``engine.py:285-296``).
+    (``engine.py:285-296``). With ``num_pages`` the graphs attend that many pages per request
+    and KV head (the manager's ``track_page_bounds`` is turned on).
     """
 
     def __init__(self, engine, sizes=(8, 16, 32, 48, 64, 96, 128),
-                 kv_buckets=(2048, 4096, 8192, 16384, 32768)):
+                 kv_buckets=(2048, 4096, 8192, 16384, 32768), num_pages: int | None = None):
         self.engine = engine
+        self.num_pages = num_pages
+        if num_pages is not None:
+            engine.paged_cache.track_page_bounds()
         manager = engine.paged_cache
         limit = min(manager.capacity_tokens, engine.max_position_embeddings)
         self.sizes = sorted({n for n in sizes if n < manager.max_requests} | {manager.max_requests})
@@ -156,11 +166,11 @@ class DecodeGraphs:
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):  # warm-up outside the capture (library set-up)
                 for _ in range(2):
-                    packed_forward(model, tokens, static.batch, rows)
+                    packed_forward(model, tokens, static.batch, rows, self.num_pages)
             torch.cuda.current_stream().wait_stream(side)
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
-                logits = packed_forward(model, tokens, static.batch, rows)
+                logits = packed_forward(model, tokens, static.batch, rows, self.num_pages)
         # every tensor the graph reads must outlive it: rows is kept with the graph
         return graph, static, tokens, host_tokens, logits, rows
 

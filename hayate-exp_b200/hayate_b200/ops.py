@@ -304,10 +304,13 @@ def norm_rope_scatter_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                              v_pool: torch.Tensor, layer: int, page_table: torch.Tensor,
                              cache_lens: torch.Tensor, q_start: torch.Tensor,
                              token_request: torch.Tensor, page_size: int, eps: float = 1e-6,
-                             error_word: torch.Tensor | None = None) -> torch.Tensor:
+                             error_word: torch.Tensor | None = None,
+                             token_depth: torch.Tensor | None = None) -> torch.Tensor:
     """Fused QK-norm + RoPE + scatter on a packed batch: q/k/v are the projections as
     ``[1, N, H, 128]``; returns the rotated q as ``[1, H_q, N, 128]`` (backed by
-    ``[1, N, H_q, 128]`` memory)."""
+    ``[1, N, H_q, 128]`` memory). ``token_depth`` (int32 ``[N]``) rotates token i at position
+    ``cache_lens[b] + token_depth[i]`` (a drafted tree: siblings share a position) while its
+    K/V still go to its own slot."""
     _require_cuda(q, k, v, q_norm_weight, k_norm_weight, cos, sin, k_pool, v_pool, page_table,
                   cache_lens, q_start, token_request)
     _int32_cuda(q_start, token_request)
@@ -330,6 +333,20 @@ def norm_rope_scatter_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out_strides = _lib.int64_array(_th_strides(q_out, "q_out"))
     batch = cache_lens.numel()
     pts = _table_args(page_table, cache_lens, batch)
+    if token_depth is not None:
+        _require_cuda(token_depth)
+        _int32_cuda(token_depth)
+        if token_depth.numel() != total:
+            raise ValueError("token_depth must have one entry per token")
+        rc = _lib.lib().hyt_norm_rope_scatter_tree(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, q_norm_weight.data_ptr(),
+            k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            q_out.data_ptr(), out_strides, k_pool.data_ptr(), v_pool.data_ptr(), num_layers, layer,
+            capacity, page_table.data_ptr(), pts, cache_lens.data_ptr(), q_start.data_ptr(),
+            token_request.data_ptr(), token_depth.data_ptr(), batch, total, num_q_heads, num_kv_heads,
+            head_dim, page_size, dtype_code(q.dtype), _ptr(error_word), _stream_ptr())
+        _lib.check(rc, "hyt_norm_rope_scatter_tree")
+        return q_out
     rc = _lib.lib().hyt_norm_rope_scatter_packed(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, q_norm_weight.data_ptr(),
         k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0],

@@ -29,6 +29,12 @@ What changes underneath:
   would land in a page someone else still holds copies that page first.
 * Pools start zeroed (the reference uses ``torch.empty``): tiles that straddle
   a request's last token read finite bytes, so masked keys contribute exactly 0.
+* ``begin_tree_batch`` / ``commit_tree`` run speculative decoding: a step of drafted token
+  trees (attended along each node's own path), then the accepted path's K/V rows moved
+  up behind the context in every layer. ``fork`` makes handles that share a request's
+  pages but own the page being written.
+* ``track_page_bounds`` keeps each full page's key bounds beside the cache, for
+  ``attend_pages``: one-token decode over the pages that can score highest.
 * ``attend_layer`` returns ``[B, H_q, T, D]`` backed by ``[B, T, H_q, D]``
   memory, so the attention module's ``transpose(1, 2).reshape(...)`` is free.
 
@@ -174,6 +180,10 @@ class PackedLayout:
     token_request: torch.Tensor  # [total_tokens] int32: request of each token row
     decode_ids: torch.Tensor   # requests with one token (split-KV decode kernel)
     prefill_ids: torch.Tensor  # the others (tcgen05 prefill kernel)
+    # a step of drafted trees (begin_tree_batch):
+    parents: list[list[int]] | None = None      # parent of each node, -1: the cached context
+    tree_mask: torch.Tensor | None = None       # [total_tokens, words] int32 visibility bits
+    token_depth: torch.Tensor | None = None     # [total_tokens] int32: position past the context
 
 
 class PagedKVBatch:
@@ -186,7 +196,7 @@ class PagedKVBatch:
 
     __slots__ = ("k_cache", "v_cache", "page_table", "cache_lens", "page_size", "query_len",
                  "max_kv_len", "cache_lens_i32", "layout", "workspace", "_manager", "_meta",
-                 "_host_lens", "_plans")
+                 "_host_lens", "_plans", "_full_pages")
 
     def __init__(self, manager, page_table, cache_lens, cache_lens_i32, query_len, max_kv_len, meta,
                  layout: PackedLayout | None = None, host_lens=None):
@@ -204,9 +214,20 @@ class PagedKVBatch:
         self._meta = meta  # keeps the uploaded buffer alive while kernels read it
         self._host_lens = host_lens  # cache lengths on the host (the prefill schedule's input)
         self._plans = {}             # num_q_heads -> (plan items on the device or None, splits)
+        self._full_pages = None      # pages this step fills up (int32, device), if bounds are kept
 
     def write_layer(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Scatter the step's new K/V ``[B, H_kv, T, D]`` into this layer's pages."""
+        self._scatter(layer_idx, k, v)
+        self._bound_layer(layer_idx)
+
+    def _bound_layer(self, layer_idx: int) -> None:
+        """Key bounds of the pages that this step fills up (``track_page_bounds``)."""
+        if self._full_pages is not None:
+            ops.page_bounds(self.k_cache, self._manager.k_bounds, self._full_pages, self.page_size,
+                            layer=layer_idx, error_word=self._manager.error_word)
+
+    def _scatter(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         if self.layout is not None:
             self._write_packed(layer_idx, k, v)
             return
@@ -227,8 +248,14 @@ class PagedKVBatch:
         ``q``/``k``/``v`` are the projections as ``[B, T, H, D]`` (before the transpose of
         ``hayate/model/attention.py:66-68``); the K/V written to the pages are those the
         unfused path (norm -> transpose -> RoPE -> ``write_layer``) writes. Returns the
-        rotated ``q`` as ``[B, H_q, T, D]``, ready for ``attend_layer``.
+        rotated ``q`` as ``[B, H_q, T, D]``, ready for ``attend_layer``. In a tree batch a node
+        is rotated at its context's length plus its depth.
         """
+        q = self._prepare(layer_idx, q, k, v, q_norm_weight, k_norm_weight, cos, sin, eps)
+        self._bound_layer(layer_idx)
+        return q
+
+    def _prepare(self, layer_idx, q, k, v, q_norm_weight, k_norm_weight, cos, sin, eps):
         if self.layout is not None:
             lay = self.layout
             if q.shape[0] != 1 or q.shape[1] != lay.total_tokens:
@@ -236,7 +263,8 @@ class PagedKVBatch:
             return ops.norm_rope_scatter_packed(
                 q, k, v, q_norm_weight, k_norm_weight, cos, sin, self.k_cache, self.v_cache,
                 layer_idx, self.page_table, self.cache_lens_i32, lay.q_start, lay.token_request,
-                self.page_size, eps=eps, error_word=self._manager.error_word)
+                self.page_size, eps=eps, error_word=self._manager.error_word,
+                token_depth=lay.token_depth)
         if q.shape[1] != self.query_len:
             raise ValueError("q/k/v must carry query_len tokens")
         return ops.norm_rope_scatter(q, k, v, q_norm_weight, k_norm_weight, cos, sin, self.k_cache,
@@ -244,7 +272,8 @@ class PagedKVBatch:
                                      self.page_size, eps=eps, error_word=self._manager.error_word)
 
     def attend_layer(self, q: torch.Tensor, layer_idx: int) -> torch.Tensor:
-        """Causal GQA attention of ``q`` ``[B, H_q, T, D]`` over this layer's paged K/V."""
+        """Causal GQA attention of ``q`` ``[B, H_q, T, D]`` over this layer's paged K/V; in a tree
+        batch each node sees its request's context, its ancestors and itself."""
         if q.stride(-1) != 1:
             q = q.contiguous()
         manager = self._manager
@@ -252,6 +281,11 @@ class PagedKVBatch:
             lay = self.layout
             if q.shape[0] != 1 or q.shape[2] != lay.total_tokens:
                 raise ValueError("a packed batch's q is [1, H_q, total_tokens, head_dim]")
+            if lay.tree_mask is not None:
+                return ops.tree_attention(
+                    q, self.k_cache, self.v_cache, layer_idx, self.page_table, self.cache_lens_i32,
+                    lay.q_start, lay.q_len, lay.tree_mask, self.page_size, self.query_len,
+                    error_word=manager.error_word)
             n_dec = lay.decode_ids.numel()
             workspace = self.workspace
             if workspace is None and n_dec:
@@ -277,6 +311,34 @@ class PagedKVBatch:
                                    workspace=workspace, error_word=manager.error_word,
                                    kernel=manager.kernel, split_tokens=manager.split_tokens)
 
+    def attend_pages(self, q: torch.Tensor, layer_idx: int,
+                     num_pages: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """One-token attention over ``num_pages`` pages per request and KV head: the one being
+        written and those whose key bounds allow the largest scores (``ops.sparse_attention``;
+        every page if there are no more). Needs ``manager.track_page_bounds()``. Takes the
+        ``q`` of ``attend_layer`` (a packed batch of one-token requests too); returns its
+        rows and the logical pages read, int32 ``[B, H_kv, num_pages]``, -1 past the last."""
+        manager = self._manager
+        if manager.k_bounds is None:
+            raise RuntimeError("attend_pages needs page bounds: call track_page_bounds() first")
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        lay = self.layout
+        if lay is None:
+            if self.query_len != 1 or q.shape[2] != 1:
+                raise ValueError("attend_pages takes one token per request")
+            rows = q
+        else:
+            if lay.tree_mask is not None or self.query_len != 1:
+                raise ValueError("attend_pages takes one token per request")
+            if q.shape[0] != 1 or q.shape[2] != lay.total_tokens:
+                raise ValueError("a packed batch's q is [1, H_q, total_tokens, head_dim]")
+            rows = q.permute(2, 1, 0, 3)
+        out, chosen = ops.sparse_attention(
+            rows, self.k_cache, self.v_cache, manager.k_bounds, layer_idx, self.page_table,
+            self.cache_lens_i32, self.page_size, num_pages, error_word=manager.error_word)
+        return (out if lay is None else out.permute(2, 1, 0, 3)), chosen
+
     def write_attend_layer(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
                            q: torch.Tensor) -> torch.Tensor:
         """``write_layer(layer_idx, k, v)`` then ``attend_layer(q, layer_idx)``, the pair
@@ -299,11 +361,13 @@ class PagedKVBatch:
         if q.stride(-1) != 1:
             q = q.contiguous()
         workspace = manager.workspace_for(q.shape[0], self.query_len, q.shape[1], self.max_kv_len)
-        return ops.paged_attention_scatter(q, k, v, self.k_cache, self.v_cache, layer_idx,
-                                           self.page_table, self.cache_lens_i32, self.page_size,
-                                           self.max_kv_len, workspace=workspace,
-                                           error_word=manager.error_word,
-                                           split_tokens=manager.split_tokens)
+        out = ops.paged_attention_scatter(q, k, v, self.k_cache, self.v_cache, layer_idx,
+                                          self.page_table, self.cache_lens_i32, self.page_size,
+                                          self.max_kv_len, workspace=workspace,
+                                          error_word=manager.error_word,
+                                          split_tokens=manager.split_tokens)
+        self._bound_layer(layer_idx)
+        return out
 
     def prefill_schedule(self, q: torch.Tensor):
         """(items, splits) for a planned prefill launch of this batch, or None for the
@@ -320,6 +384,8 @@ class PagedKVBatch:
         if q.data_ptr() % 16 or any(st % 8 for st in q.stride()[:3]) or group % 2:
             return None
         lay = self.layout
+        if lay is not None and lay.tree_mask is not None:
+            return None
         if lay is None:
             if group * self.query_len <= 16:  # the decode kernel's shapes
                 return None
@@ -350,6 +416,26 @@ class PagedKVBatch:
         ops.kv_scatter_packed(k, v, self.k_cache, self.v_cache, layer_idx, self.page_table,
                               self.cache_lens_i32, lay.q_start, lay.token_request, self.page_size,
                               error_word=self._manager.error_word)
+
+
+def _tree_metadata(trees: Sequence[Sequence[int]]) -> tuple[np.ndarray, np.ndarray]:
+    """Depth of every node (0: follows the context) and its visibility bits (int32 ``[N, words]``:
+    its ancestors' and its own), all trees walked up at once, one generation per turn."""
+    counts = [len(tree) for tree in trees]
+    total, words = sum(counts), -(-max(counts) // 32)
+    first = np.repeat(np.cumsum([0] + counts[:-1]), counts)        # row of each node's root tree
+    parent = np.asarray([p for tree in trees for p in tree], dtype=np.int64)
+    depth = np.zeros(total, dtype=np.int32)
+    mask = np.zeros((total, words), dtype=np.uint32)
+    rows = np.arange(total)
+    at = rows - first                                              # the node each row stands on
+    while len(rows):
+        mask[rows, at >> 5] |= np.uint32(1) << (at & 31).astype(np.uint32)
+        at = parent[first[rows] + at]
+        up = at >= 0
+        rows, at = rows[up], at[up]
+        depth[rows] += 1
+    return depth, mask.view(np.int32)
 
 
 class StaticDecodeBatch:
@@ -384,8 +470,13 @@ class StaticDecodeBatch:
                                              manager.head_dim, max_kv_len, manager.k_cache.dtype,
                                              manager.split_tokens)
         self.batch.workspace = ops.new_workspace(need, device) if need else None
+        # pages the step fills up, -1 for requests that fill none: looked at by every replay
+        self.full_pages = None
+        if manager.k_bounds is not None:
+            self.full_pages = torch.full((size,), -1, dtype=torch.int32, device=device)
+            self.batch._full_pages = self.full_pages
         pin = device.type == "cuda"
-        self._staging = [torch.empty(4 * size, dtype=torch.int32, pin_memory=pin) for _ in range(2)]
+        self._staging = [torch.empty(5 * size, dtype=torch.int32, pin_memory=pin) for _ in range(2)]
         self._events: list = [None, None]
         self._flip = 0
         self._manager = manager
@@ -411,8 +502,13 @@ class StaticDecodeBatch:
         h = host.numpy()
         h[: 2 * self.size].view(np.int64)[:] = lens
         h[2 * self.size: 3 * self.size] = lens
-        h[3 * self.size:] = [handle.slot for handle in handles] + [m.max_requests] * pad
-        self.meta.copy_(host, non_blocking=True)
+        h[3 * self.size: 4 * self.size] = [handle.slot for handle in handles] + [m.max_requests] * pad
+        h[4 * self.size:] = -1
+        self.meta.copy_(host[: 4 * self.size], non_blocking=True)
+        if self.full_pages is not None:
+            full = m._pages_filled(handles, lengths, [1] * n)
+            h[4 * self.size: 4 * self.size + len(full)] = full
+            self.full_pages.copy_(host[4 * self.size:], non_blocking=True)
         if m.device.type == "cuda":
             self._events[i] = torch.cuda.Event()
             self._events[i].record()
@@ -475,6 +571,7 @@ class PagedKVCacheManager:
         self._prefill_ws_zero = 0  # leading bytes of the prefill workspace known to be zero
         self._workspace_zero = 0   # leading bytes of the decode workspace known to be zero
         self._num_sms = None
+        self.k_bounds: torch.Tensor | None = None  # see track_page_bounds
 
     # ------------------------------------------------------------------ pages
     def _take_pages(self, count: int) -> list[int]:
@@ -539,23 +636,66 @@ class PagedKVCacheManager:
         self._rows.set_row(handle.slot, handle.pages)
         return handle
 
-    def _make_writable(self, handle: PagedCacheHandle, first: int, last: int) -> None:
-        """Copy-on-write every page holding logical positions ``first..last`` that is shared."""
-        if last < first:
+    def fork(self, source: PagedCacheHandle, count: int) -> list[PagedCacheHandle]:
+        """``count`` new handles that continue ``source``: its full pages are shared, and each
+        gets its own copy of the page being written (one launch for all of them), so that
+        the first step of the forks copies nothing. Nothing is taken if it does not fit."""
+        if source.released:
+            raise RuntimeError("cannot fork a released cache handle")
+        if count < 1:
+            raise ValueError("count must be positive")
+        if len(self._free_slots) < count:
+            raise MemoryError(f"paged cache supports at most {self.max_requests} active requests")
+        partial = source.length % self.page_size != 0
+        if partial and len(self._free_pages) < count:
+            raise MemoryError(f"paged KV cache is full: need {count} additional pages, "
+                              f"but only {len(self._free_pages)} remain")
+        handles = [self.share(source, source.length) for _ in range(count)]
+        if partial:
+            pairs: list[tuple[int, int]] = []
+            for handle in handles:
+                self._make_writable(handle, source.length - 1, source.length - 1, pairs)
+            self._copy_pages(pairs)
+        return handles
+
+    def _copy_pages(self, pairs: Sequence[tuple[int, int]]) -> None:
+        """Copy pages ``(from, to)`` in every layer of both pools: one launch on the GPU."""
+        if not pairs:
             return
-        for logical in range(first // self.page_size, last // self.page_size + 1):
-            old = handle.pages[logical]
-            if self._page_refs[old] <= 1:
-                continue
-            if not self._free_pages:
-                raise MemoryError("paged KV cache is full: no page left to copy a shared page")
-            new = self._take_pages(1)[0]
-            size = self.page_size
+        if self.device.type == "cuda":
+            ids = self._uploader.upload(np.asarray(pairs, dtype=np.int32).T.reshape(-1))
+            n = len(pairs)
+            ops.copy_pages(self.k_cache, self.v_cache, ids[:n], ids[n:], self.page_size,
+                           error_word=self.error_word)
+            return
+        size = self.page_size
+        for old, new in pairs:
             for pool in (self.k_cache, self.v_cache):
                 pool[:, :, :, new * size:(new + 1) * size].copy_(pool[:, :, :, old * size:(old + 1) * size])
-            self._drop_pages([old])
-            handle.pages[logical] = new
-            self._rows.set_entry(handle.slot, logical, new)
+
+    def _make_writable(self, handle: PagedCacheHandle, first: int, last: int,
+                       pairs: list[tuple[int, int]] | None = None) -> None:
+        """Copy-on-write every page holding logical positions ``first..last`` that is shared.
+        With ``pairs`` the copies are only noted there, for one ``_copy_pages`` of a whole step
+        (a page that was copied away keeps its other holders, so its content stays)."""
+        if last < first:
+            return
+        noted: list[tuple[int, int]] = [] if pairs is None else pairs
+        try:
+            for logical in range(first // self.page_size, last // self.page_size + 1):
+                old = handle.pages[logical]
+                if self._page_refs[old] <= 1:
+                    continue
+                if not self._free_pages:
+                    raise MemoryError("paged KV cache is full: no page left to copy a shared page")
+                new = self._take_pages(1)[0]
+                noted.append((old, new))
+                self._drop_pages([old])
+                handle.pages[logical] = new
+                self._rows.set_entry(handle.slot, logical, new)
+        finally:
+            if pairs is None:
+                self._copy_pages(noted)
 
     def allocate_for_request(self, cache=None) -> PagedCacheHandle:
         """Allocate a request handle and optionally import a contiguous prefix."""
@@ -581,6 +721,7 @@ class PagedKVCacheManager:
                 pool[layer, 0].index_copy_(
                     1, slots, src[layer, :, :length].to(device=pool.device, dtype=pool.dtype))
         handle.length = length
+        self.refresh_page_bounds(handle)
 
     def truncate(self, handle: PagedCacheHandle, length: int) -> None:
         """Shorten a cache and drop whole pages beyond its new end."""
@@ -669,9 +810,13 @@ class PagedKVCacheManager:
             self.reserve(handle, target)
         # copy-on-write where an append lands in a page another request still holds (only
         # requests that took part in share() can hold such pages)
-        for handle, length, n in zip(handles, lengths, query_lens):
-            if handle.aliased:
-                self._make_writable(handle, length, length + n - 1)
+        pairs: list[tuple[int, int]] = []
+        try:
+            for handle, length, n in zip(handles, lengths, query_lens):
+                if handle.aliased:
+                    self._make_writable(handle, length, length + n - 1, pairs)
+        finally:
+            self._copy_pages(pairs)
 
         return lengths, query_lens, kv_lengths
 
@@ -702,9 +847,19 @@ class PagedKVCacheManager:
             host[3 * batch:] = slots
             meta = self._uploader.upload(host)
             table = self._rows.gather(meta[3 * batch:].long(), width)
-            return PagedKVBatch(self, table, meta[: 2 * batch].view(torch.int64),
-                                meta[2 * batch: 3 * batch], query_len, max(kv_lengths), (meta, table),
-                                host_lens=list(lengths))
+            built = PagedKVBatch(self, table, meta[: 2 * batch].view(torch.int64),
+                                 meta[2 * batch: 3 * batch], query_len, max(kv_lengths), (meta, table),
+                                 host_lens=list(lengths))
+            built._full_pages = self._upload_filled(handles, lengths, query_lens)
+            return built
+        built = self._packed_batch(handles, lengths, query_lens, kv_lengths, width, slots)
+        built._full_pages = self._upload_filled(handles, lengths, query_lens)
+        return built
+
+    def _packed_batch(self, handles, lengths, query_lens, kv_lengths, width, slots,
+                      tree: tuple | None = None) -> PagedKVBatch:
+        """A packed batch's metadata in one upload; ``tree``: (parents, depths, mask words)."""
+        batch = len(handles)
         q_len = np.asarray(query_lens, dtype=np.int32)
         q_start = np.zeros(batch, dtype=np.int32)
         np.cumsum(q_len[:-1], out=q_start[1:])
@@ -713,21 +868,135 @@ class PagedKVCacheManager:
         prefill_ids = np.nonzero(q_len > 1)[0].astype(np.int32)
         token_request = np.repeat(np.arange(batch, dtype=np.int32), q_len)
         n_dec = len(decode_ids)
-        host = np.concatenate([np.zeros(2 * batch, dtype=np.int32), np.asarray(lengths, dtype=np.int32),
-                               np.asarray(slots, dtype=np.int32), q_start, q_len, decode_ids,
-                               prefill_ids, token_request])
+        parts = [np.zeros(2 * batch, dtype=np.int32), np.asarray(lengths, dtype=np.int32),
+                 np.asarray(slots, dtype=np.int32), q_start, q_len, decode_ids, prefill_ids, token_request]
+        if tree is not None:
+            parts += [tree[1], tree[2].reshape(-1)]
+        host = np.concatenate(parts)
         host[: 2 * batch].view(np.int64)[:] = lengths
         meta = self._uploader.upload(host)
         o = 4 * batch
         table = self._rows.gather(meta[3 * batch: o].long(), width)
+        end = o + 3 * batch + total
         layout = PackedLayout(query_lens=query_lens, total_tokens=total,
                               q_start=meta[o: o + batch], q_len=meta[o + batch: o + 2 * batch],
                               decode_ids=meta[o + 2 * batch: o + 2 * batch + n_dec],
                               prefill_ids=meta[o + 2 * batch + n_dec: o + 3 * batch],
-                              token_request=meta[o + 3 * batch:])
+                              token_request=meta[o + 3 * batch: end])
+        if tree is not None:
+            layout.parents = tree[0]
+            layout.token_depth = meta[end: end + total]
+            layout.tree_mask = meta[end + total:].view(total, -1)
         return PagedKVBatch(self, table, meta[: 2 * batch].view(torch.int64), meta[2 * batch: 3 * batch],
                             max(query_lens), max(kv_lengths), (meta, table), layout,
                             host_lens=list(lengths))
+
+    # ------------------------------------------------------------------ drafted trees
+    def begin_tree_batch(self, handles: Sequence[PagedCacheHandle],
+                         parents: Sequence[Sequence[int]]) -> PagedKVBatch:
+        """A step of drafted token trees: ``parents[b][i]`` is the node that request b's node i
+        follows, an earlier one, or -1 for the cached context.
+
+        The batch is packed (``[1, H, N, D]`` tensors, request after request): its
+        ``write_layer`` puts node i's K/V at the context's length plus i, ``prepare_layer``
+        rotates it at the context's length plus its depth, and in ``attend_layer`` a node
+        sees the context, its ancestors and itself. ``commit_tree`` ends the step.
+        """
+        if not handles:
+            raise ValueError("cannot build paged cache metadata for an empty batch")
+        if len(parents) != len(handles):
+            raise ValueError("a tree batch needs one list of parents per request")
+        trees = [[int(p) for p in tree] for tree in parents]
+        for tree in trees:
+            if any(p < -1 or p >= i for i, p in enumerate(tree)):
+                raise ValueError("a node's parent must be an earlier node of its tree, or -1")
+        lengths, query_lens, kv_lengths = self._prepare_step(handles, [len(tree) for tree in trees], True)
+        depths, mask = _tree_metadata(trees)
+        self._rows.flush()
+        width = math.ceil(max(kv_lengths) / self.page_size)
+        slots = [handle.slot for handle in handles]
+        return self._packed_batch(handles, lengths, query_lens, kv_lengths, width, slots, (trees, depths, mask))
+
+    def commit_tree(self, batch: PagedKVBatch, handles: Sequence[PagedCacheHandle],
+                    accepted: Sequence[Sequence[int]]) -> None:
+        """End a tree step: ``accepted[b]`` is a path of request b's tree from the context down
+        (its nodes in order, possibly none). Their K/V rows move up to follow the context in
+        every layer, in one launch, and the requests grow by the paths' lengths."""
+        layout = batch.layout
+        if layout is None or layout.parents is None:
+            raise ValueError("commit_tree ends a batch of begin_tree_batch")
+        if len(handles) != len(layout.parents) or len(accepted) != len(handles):
+            raise ValueError("commit_tree needs the step's handles and one path per request")
+        paths = [[int(i) for i in path] for path in accepted]
+        for handle, path, tree, length in zip(handles, paths, layout.parents, batch._host_lens):
+            if handle.released:
+                raise RuntimeError("cannot commit a released cache handle")
+            if handle.length != length or length + len(tree) > len(handle.pages) * self.page_size:
+                raise RuntimeError("the cache handle changed since its tree batch began")
+            if any(i < 0 or i >= len(tree) for i in path) or any(
+                    tree[i] != before for i, before in zip(path, [-1] + path)):
+                raise ValueError("an accepted path must follow its tree's parents from the context")
+        moved = sum(i != at for path in paths for at, i in enumerate(path))
+        if moved:
+            flat = [i for path in paths for i in path]
+            start = np.concatenate([[0], np.cumsum([len(path) for path in paths])])
+            if self.device.type == "cuda":
+                meta = self._uploader.upload(np.concatenate([start, flat]).astype(np.int32))
+                ops.compact_rows(self.k_cache, self.v_cache, batch.page_table, batch.cache_lens_i32,
+                                 meta[len(start):], meta[: len(start)], self.page_size,
+                                 error_word=self.error_word)
+            else:
+                for handle, path in zip(handles, paths):
+                    slots = self._slots_of(handle, handle.length + np.asarray(path, dtype=np.int64))
+                    to = self._slots_of(handle, handle.length + np.arange(len(path)))
+                    for pool in (self.k_cache, self.v_cache):
+                        pool[:, :, :, to] = pool[:, :, :, slots]
+        grown = [len(path) for path in paths]
+        filled = self._upload_filled(handles, batch._host_lens, grown)
+        if filled is not None:
+            ops.page_bounds(self.k_cache, self.k_bounds, filled, self.page_size, error_word=self.error_word)
+        for handle, n in zip(handles, grown):
+            handle.length += n
+
+    # ------------------------------------------------------------------ page bounds
+    def track_page_bounds(self) -> None:
+        """Keep the elementwise minimum and maximum of every full page's keys from now on
+        (``k_bounds``, ``[layers, H_kv, num_pages, 2, head_dim]``: 2 / page_size of the K pool), for
+        ``PagedKVBatch.attend_pages``. Steps, imports and accepted trees keep them up to date;
+        call ``refresh_page_bounds`` after writing to the pools yourself. Batches that exist
+        already do not keep them."""
+        if self.k_bounds is not None:
+            return
+        if self.device.type != "cuda":
+            raise RuntimeError("hayate_b200 kernels run on CUDA tensors only (no CPU fallback)")
+        self.k_bounds = torch.zeros((self.num_layers, self.num_kv_heads, self.num_pages, 2, self.head_dim),
+                                    dtype=self.k_cache.dtype, device=self.device)
+        self._bound_pages(np.nonzero(self._page_refs)[0])
+
+    def refresh_page_bounds(self, handle: PagedCacheHandle) -> None:
+        """Compute the bounds of all full pages of a request (nothing if they are not kept)."""
+        if handle.released:
+            raise RuntimeError("cannot refresh the bounds of a released cache handle")
+        self._bound_pages(handle.pages[: handle.length // self.page_size])
+
+    def _bound_pages(self, pages) -> None:
+        if self.k_bounds is None or not len(pages):
+            return
+        for first in range(0, len(pages), 32768):
+            ids = self._uploader.upload(np.asarray(pages[first: first + 32768], dtype=np.int32))
+            ops.page_bounds(self.k_cache, self.k_bounds, ids, self.page_size, error_word=self.error_word)
+
+    def _pages_filled(self, handles, lengths, grown) -> list[int]:
+        """Pages whose last token is among the next ``grown`` of each request."""
+        size = self.page_size
+        return [page for handle, length, n in zip(handles, lengths, grown)
+                for page in handle.pages[length // size: (length + n) // size]]
+
+    def _upload_filled(self, handles, lengths, grown) -> torch.Tensor | None:
+        if self.k_bounds is None:
+            return None
+        pages = self._pages_filled(handles, lengths, grown)
+        return self._uploader.upload(np.asarray(pages, dtype=np.int32)) if pages else None
 
     def commit_batch(self, handles: Sequence[PagedCacheHandle], query_len: int | Sequence[int]) -> None:
         """Advance logical lengths after every layer wrote the step's K/V."""
@@ -811,9 +1080,12 @@ class PagedKVCacheManager:
             raise RuntimeError("paged attention kernels refused input: " + "; ".join(problems))
 
     def _physical_positions(self, handle: PagedCacheHandle, length: int) -> torch.Tensor:
-        if length == 0:
+        return self._slots_of(handle, np.arange(length, dtype=np.int64))
+
+    def _slots_of(self, handle: PagedCacheHandle, logical: np.ndarray) -> torch.Tensor:
+        """Pool positions of a request's logical positions."""
+        if len(logical) == 0:
             return torch.empty(0, dtype=torch.long, device=self.device)
-        logical = np.arange(length, dtype=np.int64)
         pages = np.asarray(handle.pages, dtype=np.int64)[logical // self.page_size]
         slots = pages * self.page_size + logical % self.page_size
         return torch.from_numpy(slots).to(self.device)

@@ -246,6 +246,21 @@ int hyt_norm_rope_scatter_packed(const void* q, const void* k, const void* v,
                                  int32_t head_dim, int32_t page_size, int32_t dtype,
                                  int32_t* error_word, void* stream);
 
+/* The same for drafted trees: token i is rotated at position cache_lens[b] + token_depth[i]
+ * (siblings share a position); its K/V go to slot cache_lens[b] + i - q_start[b] as above. */
+int hyt_norm_rope_scatter_tree(const void* q, const void* k, const void* v,
+                               const int64_t* qkv_strides, const void* q_norm_weight,
+                               const void* k_norm_weight, float eps, const float* cos,
+                               const float* sin, int32_t rope_positions, void* q_out,
+                               const int64_t* q_out_strides, void* k_pool, void* v_pool,
+                               int32_t num_layers, int32_t layer, int64_t capacity_tokens,
+                               const int32_t* page_table, int32_t page_table_stride,
+                               const int32_t* cache_lens, const int32_t* q_start,
+                               const int32_t* token_request, const int32_t* token_depth,
+                               int32_t batch, int32_t total_tokens, int32_t num_q_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                               int32_t dtype, int32_t* error_word, void* stream);
+
 /*
  * Packed attend_layer in one call: the requests listed in decode_ids (one query
  * each) go to the split-KV decode kernel, those in prefill_ids (any chunk length up
