@@ -8,10 +8,12 @@
 //
 // compact_rows: request b's row base[b] + src[i] -> base[b] + i, src strictly increasing (so
 // src[i] >= i): the accepted path of a drafted tree moves up behind the context, in place.
-// One thread owns one 16-byte column of one plane of one request and takes its rows in
-// order, kUnroll at a time (all loads of a group before its stores): row i + kUnroll.. is
-// read after rows < i + kUnroll were written, and src[i + kUnroll] >= i + kUnroll, so nothing
-// is read after it was overwritten, and no two threads touch the same bytes.
+// A CTA serves one request: it looks its rows' pool offsets up once, kThreads rows at a time,
+// and every thread owns one 16-byte column of one plane and takes the rows in order, kRowsAhead
+// loads before their stores: row i + kRowsAhead is read after rows < i + kRowsAhead were written,
+// and src[i + kRowsAhead] >= i + kRowsAhead, so nothing is read after it was overwritten, and no
+// two threads touch the same bytes. Bound: HBM, 256-byte pieces (a row of one head), one read
+// and one write of each.
 #include "chunk_schedule.cuh"
 
 namespace hyt {
@@ -74,6 +76,8 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const MoveParams p
 template <int kVec>
 __global__ void __launch_bounds__(kThreads) compact_rows_kernel(const MoveParams p) {
   using V = typename Vec<kVec>::type;
+  constexpr int kRowsAhead = 12;
+  __shared__ int64_t from_s[kThreads], to_s[kThreads];  // byte offsets in a plane, -1: nothing to do
   const int b = blockIdx.y;
   const int begin = p.start[b], end = p.start[b + 1];
   if (begin < 0 || end < begin || end > p.count) {
@@ -83,14 +87,15 @@ __global__ void __launch_bounds__(kThreads) compact_rows_kernel(const MoveParams
   const int chunks = int(p.row_bytes / kVec);
   const int64_t column = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t plane = column / chunks;
-  if (plane >= 2 * int64_t(p.planes)) return;
+  const bool mine = plane < 2 * int64_t(p.planes);
   const int64_t plane_bytes = p.row_bytes * p.capacity;
-  uint8_t* pool = (plane < p.planes ? p.k_pool + plane * plane_bytes : p.v_pool + (plane - p.planes) * plane_bytes) +
-                  (column - plane * chunks) * kVec;
+  uint8_t* pool = !mine ? nullptr
+                        : (plane < p.planes ? p.k_pool + plane * plane_bytes : p.v_pool + (plane - p.planes) * plane_bytes) +
+                              (column - plane * chunks) * kVec;
   const int64_t base = p.base[b];
   const int32_t* table = p.page_table + int64_t(b) * p.page_table_stride;
   int why = 0;
-  auto row = [&](int64_t pos) -> int64_t {  // byte offset of a position's row in the plane, or -1
+  auto row = [&](int64_t pos) -> int64_t {  // byte offset of a position's row in a plane, or -1
     const int64_t lp = pos >> p.page_shift;
     if (pos < 0 || lp >= p.table_width) {
       why |= HYT_DEVERR_TABLE_RANGE;
@@ -103,30 +108,31 @@ __global__ void __launch_bounds__(kThreads) compact_rows_kernel(const MoveParams
     }
     return ((int64_t(page) << p.page_shift) + (pos & ((1 << p.page_shift) - 1))) * p.row_bytes;
   };
-  for (int i0 = begin; i0 < end; i0 += kUnroll) {
-    V v[kUnroll];
-    int64_t to[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      to[u] = -1;
-      const int i = i0 + u;
-      if (i >= end) continue;
+  for (int group = begin; group < end; group += kThreads) {
+    const int here = min(end - group, kThreads);
+    __syncthreads();  // the offsets of the group before have been used
+    if (int(threadIdx.x) < here) {
+      const int i = group + int(threadIdx.x), at = i - begin;
       const int s = p.src[i], prev = i > begin ? p.src[i - 1] : -1;
-      if (s < i - begin || s <= prev) {
-        why |= HYT_DEVERR_MOVE_ORDER;
-        continue;
-      }
-      if (s == i - begin) continue;  // already there
-      const int64_t from = row(base + s), dst = row(base + (i - begin));
-      if (from < 0 || dst < 0) continue;
-      v[u] = *reinterpret_cast<const V*>(pool + from);
-      to[u] = dst;
+      int64_t from = -1, to = -1;
+      if (s < at || s <= prev) why |= HYT_DEVERR_MOVE_ORDER;
+      else if (s != at) from = row(base + s), to = row(base + at);
+      from_s[threadIdx.x] = from < 0 || to < 0 ? -1 : from;
+      to_s[threadIdx.x] = to;
     }
+    __syncthreads();
+    if (!mine) continue;
+    for (int i0 = 0; i0 < here; i0 += kRowsAhead) {
+      V v[kRowsAhead];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (to[u] >= 0) *reinterpret_cast<V*>(pool + to[u]) = v[u];
+      for (int u = 0; u < kRowsAhead; ++u)
+        if (i0 + u < here && from_s[i0 + u] >= 0) v[u] = *reinterpret_cast<const V*>(pool + from_s[i0 + u]);
+#pragma unroll
+      for (int u = 0; u < kRowsAhead; ++u)
+        if (i0 + u < here && from_s[i0 + u] >= 0) *reinterpret_cast<V*>(pool + to_s[i0 + u]) = v[u];
+    }
   }
-  if (why && blockIdx.x == 0 && threadIdx.x == 0) flag_error(p.error_word, why);
+  if (why && blockIdx.x == 0) flag_error(p.error_word, why);
 }
 
 // Widest vector that rows, planes and both pools are aligned to.

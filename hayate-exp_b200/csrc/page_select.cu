@@ -1,8 +1,10 @@
 // Page bounds, and the choice of pages a one-token decode reads.
 //
 // page_bounds: elementwise minimum and maximum of a full page's keys, per layer and KV head.
-// One pass over the page: a thread keeps one 16-byte column of every n-th row, the row groups
-// meet in shared memory. NaN keys give NaN bounds. Bound: HBM reads of the keys.
+// One pass over the page: a thread keeps one 16-byte column of every n-th row (16-bit types as
+// packed pairs: half the instructions of widening them), kAhead loads in flight; lanes of one
+// column meet by shuffles, warps in shared memory. NaN keys give NaN bounds. Bound: HBM reads
+// of the keys.
 //
 // select_pages: score(page) = max over the KV group's query heads of
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
@@ -62,58 +64,120 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&f)[16 / sizeof(
   }
 }
 
+// Minimum and maximum of 32-bit words of one or two values, NaN if either is.
+template <typename T>
+struct MinMax;
+template <>
+struct MinMax<float> {
+  static __device__ __forceinline__ uint32_t lo(uint32_t a, uint32_t b) {
+    return __float_as_uint(min_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ uint32_t hi(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+};
+template <>
+struct MinMax<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t lo(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t hi(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+};
+template <>
+struct MinMax<__half> {
+  static __device__ __forceinline__ uint32_t lo(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t hi(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+};
+
 // Grid: (KV head, page entry, layer).
 template <typename T>
 __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsParams p) {
   constexpr int kPer = 16 / int(sizeof(T));
-  __shared__ float lo_s[kBoundsThreads * kPer], hi_s[kBoundsThreads * kPer];
+  constexpr int kWarps = kBoundsThreads / 32;
+  __shared__ uint4 lo_s[kWarps][64], hi_s[kWarps][64];  // per warp and column (at most 64 of them)
   const int32_t page = p.pages[blockIdx.y];
   if (page == -1) return;
   if (page < 0 || page >= p.num_pages) {
     if (threadIdx.x == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
     return;
   }
-  const int D = p.head_dim, chunks = D / kPer;       // 16-byte columns of a row (<= 64)
-  const int groups = kBoundsThreads / chunks;        // rows read side by side
-  const int c = threadIdx.x % chunks, rg = threadIdx.x / chunks;
-  const int64_t plane = int64_t(p.first_layer + blockIdx.z) * p.num_kv_heads + blockIdx.x;
+  const int D = p.head_dim, chunks = D / kPer;  // 16-byte columns of a row (<= 64)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // columns that divide a warp's lanes: 32 / chunks rows side by side per warp; else a warp takes
+  // whole rows, ceil(chunks / 32) columns per lane, one after the other
+  const bool side_by_side = chunks <= 32 && 32 % chunks == 0;
+  const int per_warp = side_by_side ? 32 / chunks : 1, groups = kWarps * per_warp;
   const int rows = 1 << p.page_shift;
-  const T* keys = static_cast<const T*>(p.k_pool) + (plane * p.capacity + (int64_t(page) << p.page_shift)) * D + c * kPer;
-  float lo[kPer], hi[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
-  if (rg < groups) {
+  const int64_t plane = int64_t(p.first_layer + blockIdx.z) * p.num_kv_heads + blockIdx.x;
+  const T* keys = static_cast<const T*>(p.k_pool) + (plane * p.capacity + (int64_t(page) << p.page_shift)) * D;
+  const int first = side_by_side ? warp * per_warp + lane / chunks : warp;
+  for (int c = side_by_side ? lane % chunks : lane; c < chunks; c += 32) {
+    const T* column = keys + c * kPer;
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    bool any = first < rows;
+    if (any) lo = hi = __ldg(reinterpret_cast<const uint4*>(column + int64_t(first) * D));
     constexpr int kAhead = 8;
-    for (int r0 = rg; r0 < rows; r0 += groups * kAhead) {
+    for (int r0 = first + groups; r0 < rows; r0 += groups * kAhead) {
       uint4 v[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (r0 + u * groups < rows) v[u] = __ldg(reinterpret_cast<const uint4*>(keys + int64_t(r0 + u * groups) * D));
+      for (int u = 0; u < kAhead; ++u) {
+        const int r = r0 + u * groups;
+        v[u] = r < rows ? __ldg(reinterpret_cast<const uint4*>(column + int64_t(r) * D)) : lo;
+      }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if (r0 + u * groups >= rows) break;
-        float f[kPer];
-        unpack16<T>(v[u], f);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) lo[e] = min_nan(lo[e], f[e]), hi[e] = max_nan(hi[e], f[e]);
+        lo.x = MinMax<T>::lo(lo.x, v[u].x), hi.x = MinMax<T>::hi(hi.x, v[u].x);
+        lo.y = MinMax<T>::lo(lo.y, v[u].y), hi.y = MinMax<T>::hi(hi.y, v[u].y);
+        lo.z = MinMax<T>::lo(lo.z, v[u].z), hi.z = MinMax<T>::hi(hi.z, v[u].z);
+        lo.w = MinMax<T>::lo(lo.w, v[u].w), hi.w = MinMax<T>::hi(hi.w, v[u].w);
       }
     }
-  }
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {  // [e][thread]: no bank conflicts
-    lo_s[e * kBoundsThreads + threadIdx.x] = lo[e];
-    hi_s[e * kBoundsThreads + threadIdx.x] = hi[e];
+    if (side_by_side) {  // rows that exist come first: a lane without one takes its partner's
+      for (int off = chunks; off < 32; off <<= 1) {
+        const uint4 a = make_uint4(__shfl_xor_sync(0xffffffffu, lo.x, off), __shfl_xor_sync(0xffffffffu, lo.y, off),
+                                   __shfl_xor_sync(0xffffffffu, lo.z, off), __shfl_xor_sync(0xffffffffu, lo.w, off));
+        const uint4 b = make_uint4(__shfl_xor_sync(0xffffffffu, hi.x, off), __shfl_xor_sync(0xffffffffu, hi.y, off),
+                                   __shfl_xor_sync(0xffffffffu, hi.z, off), __shfl_xor_sync(0xffffffffu, hi.w, off));
+        const bool theirs = __shfl_xor_sync(0xffffffffu, any ? 1 : 0, off) != 0;
+        if (theirs && any) {
+          lo = make_uint4(MinMax<T>::lo(lo.x, a.x), MinMax<T>::lo(lo.y, a.y), MinMax<T>::lo(lo.z, a.z), MinMax<T>::lo(lo.w, a.w));
+          hi = make_uint4(MinMax<T>::hi(hi.x, b.x), MinMax<T>::hi(hi.y, b.y), MinMax<T>::hi(hi.z, b.z), MinMax<T>::hi(hi.w, b.w));
+        } else if (theirs) {
+          lo = a, hi = b;
+        }
+        any |= theirs;
+      }
+    }
+    if (!side_by_side || lane < chunks) {
+      lo_s[warp][c] = lo;
+      hi_s[warp][c] = hi;
+    }
   }
   __syncthreads();
-  T* out = static_cast<T*>(p.k_bounds) + (plane * p.num_pages + page) * 2 * D;
-  for (int d = threadIdx.x; d < 2 * D; d += kBoundsThreads) {
-    const bool is_hi = d >= D;
-    const int dd = is_hi ? d - D : d, cc = dd / kPer, e = dd - cc * kPer;
-    const float* from = (is_hi ? hi_s : lo_s) + e * kBoundsThreads;
-    float x = from[cc];
-    for (int g = 1; g < min(groups, rows); ++g)
-      x = is_hi ? max_nan(x, from[g * chunks + cc]) : min_nan(x, from[g * chunks + cc]);
-    out[d] = Elem<T>::from_float(x);  // exact: x is one of the keys' values
+  const int used = min(kWarps, (rows + per_warp - 1) / per_warp);  // warps that had a row
+  const int words = chunks * 4;
+  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.k_bounds) + (plane * p.num_pages + page) * 2 * D);
+  for (int i = tid; i < 2 * words; i += kBoundsThreads) {
+    const bool is_hi = i >= words;
+    const int w = is_hi ? i - words : i;
+    const uint32_t(*from)[64 * 4] = reinterpret_cast<const uint32_t(*)[64 * 4]>(is_hi ? hi_s : lo_s);
+    uint32_t x = from[0][w];
+    for (int k = 1; k < used; ++k) x = is_hi ? MinMax<T>::hi(x, from[k][w]) : MinMax<T>::lo(x, from[k][w]);
+    out[i] = x;
   }
 }
 
