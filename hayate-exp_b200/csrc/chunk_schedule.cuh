@@ -124,6 +124,48 @@ __device__ __forceinline__ void chunk_find_start(const ChunkParams& P, int c, in
   __syncthreads();
 }
 
+// The same for one full warp on its own (no barrier); the result on every lane.
+__device__ __forceinline__ ChunkStart chunk_find_start_warp(const ChunkParams& P, int c, int ctas) {
+  const int lane = threadIdx.x & 31;
+  wait_for_primary();
+  int64_t before_all = 0, total = 0;
+  int why = 0;
+  for (int b0 = 0; b0 < P.a.batch; b0 += 32)
+    if (b0 + lane < P.a.batch) total += chunk_work(P, chunk_request(P, b0 + lane, why));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+    why |= __shfl_xor_sync(0xffffffffu, why, off);
+  }
+  if (why && c == 0 && lane == 0) flag_error(P.a.error_word, why);
+  ChunkStart start;
+  start.total = total;
+  start.base = chunk_div(total, ctas);
+  start.rem = int(total - start.base * ctas);
+  start.off = 0;
+  start.b = 0;
+  const int64_t begin = start.begin(c);
+  for (int b0 = 0; b0 < P.a.batch && begin < total; b0 += 32) {  // the request that holds `begin`
+    const int64_t mine = b0 + lane < P.a.batch ? chunk_work(P, chunk_request(P, b0 + lane, why)) : 0;
+    int64_t scan = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, scan, off);
+      if (lane >= off) scan += v;
+    }
+    const int64_t before = before_all + scan - mine;
+    const uint32_t holds = __ballot_sync(0xffffffffu, begin >= before && begin < before + mine);
+    if (holds) {
+      const int from = __ffs(holds) - 1;
+      start.b = b0 + from;
+      start.off = begin - __shfl_sync(0xffffffffu, before, from);
+      break;
+    }
+    before_all += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  return start;
+}
+
 struct ChunkSegment {
   int b, g, row0;        // request, KV head, first row of the unit
   int len, queries, kv;  // cached tokens, queries, their sum

@@ -70,8 +70,6 @@ struct Shared {
   int32_t abort;       // a bounded wait gave up: later waits return at once
   int32_t fix[2];      // a drafted node's V is not finite, per segment parity
   int32_t refused[8];  // per tile (ring): page refused, nothing of the tile is visible
-  ChunkStart start;
-  int64_t sums[kThreads / 32];
   ChunkSegment seg[kSegments];  // segment i in entry i % kSegments; no tiles: the end
   float m[2][kRows];         // running maxima of the streams (joined at the end)
   float sum[2][2][kRows];    // [stream][column half][row]
@@ -203,7 +201,7 @@ __global__ void __maxnreg__(96)
   int32_t* err = p.error_word;
   volatile int* abort = &sh->abort;
 
-  if (threadIdx.x == kProducerWarp * 32) {
+  if (threadIdx.x == kMmaWarp * 32) {
     sh->abort = 0;
     sh->fix[0] = sh->fix[1] = 0;
     mbar_init(&sh->q_full, kQThreads);
@@ -218,15 +216,23 @@ __global__ void __maxnreg__(96)
     mbar_init(&sh->drain, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
-    tma_prefetch_desc(&k_map);
-    tma_prefetch_desc(&v_map);
+  }
+  ChunkStart start;  // of the producer warp alone: the others follow its segments
+  if (warp == kProducerWarp) {
+    if (lane == 0) {
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+    }
+    start = chunk_find_start_warp(P, blockIdx.x, P.ctas);
+  } else {
+    wait_for_primary();
   }
   if (warp == 0) {
     tmem_alloc(&sh->tmem_base, kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
-  chunk_find_start<kThreads>(P, blockIdx.x, P.ctas, sh->sums, &sh->start);  // ends with a barrier
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
   const uint32_t smem_base = smem_u32(smem);
@@ -242,7 +248,7 @@ __global__ void __maxnreg__(96)
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      ChunkWalk walk(P, sh->start, blockIdx.x);
+      ChunkWalk walk(P, start, blockIdx.x);
       // an earlier CTA's wait gave up: load nothing, every tile counts as refused
       const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
       const int page_mask = (1 << p.page_shift) - 1;
@@ -258,7 +264,7 @@ __global__ void __maxnreg__(96)
         const bool any = walk.next(P, seg);
         sh->seg[i % kSegments] = seg;
         mbar_arrive(&sh->seg_full[i % kSegments]);
-        if (i == 0) chunk_write_join(P, sh->start, blockIdx.x, any ? &seg : nullptr);
+        if (i == 0) chunk_write_join(P, start, blockIdx.x, any ? &seg : nullptr);
         if (!any) break;
         const int32_t* table = chunk_table(P, seg.b, seg.g);
         const int plane = p.layer * p.num_kv_heads + seg.g;
@@ -431,20 +437,21 @@ __global__ void __maxnreg__(96)
   } else if (warp >= kQWarp) {
     // ------------------------------------------------------------ Q loaders, V checkers
     const int tid = int(threadIdx.x) - kQWarp * 32, D = p.head_dim;
-    constexpr int kRowChunks = kChunks * 8;                         // 16-byte chunks of a padded row
-    constexpr int kEach = (kDual ? 2 : 1) * kRows * kRowChunks / kQThreads;
+    constexpr int kRowChunks = kChunks * 8;            // 16-byte chunks of a padded row
+    constexpr int kStepRows = kQThreads / kRowChunks;  // rows the two warps load at a time
     const int c = tid % kRowChunks;
+    const int step_t = kStepRows / P.group, step_h = kStepRows - step_t * P.group;
+    const int64_t step_off = step_t * p.q_st + step_h * p.q_sh, wrap_off = p.q_st - P.group * p.q_sh;
+    // rows of the 32-row quarters that have any (the others' lanes are never looked at)
     auto load_q = [&](const ChunkSegment& seg) {
-      const ChunkRows unit(P, seg.row0);
       const int rows = seg.queries * P.group - seg.row0;
-      const T* base = static_cast<const T*>(p.q) + att_q_row(p, seg.b, 0) + int64_t(seg.g) * P.group * p.q_sh + c * 8;
+      const int upto = min((kDual ? 2 : 1) * kRows, (rows + 31) & ~31);
+      int qr = tid / kRowChunks, t, hl;
+      ChunkRows(P, seg.row0).at(P, qr, t, hl);
+      const T* src = static_cast<const T*>(p.q) + att_q_row(p, seg.b, t) + int64_t(seg.g * P.group + hl) * p.q_sh + c * 8;
 #pragma unroll 4
-      for (int u = 0; u < kEach; ++u) {
-        const int qr = (u * kQThreads + tid) / kRowChunks;
+      for (; qr < upto; qr += kStepRows) {
         const bool there = qr < rows && c * 8 < D;
-        int t, hl;
-        unit.at(P, there ? qr : 0, t, hl);
-        const T* src = base + int64_t(t) * p.q_st + int64_t(hl) * p.q_sh;
         uint8_t* dst = smem + L::kQ + (qr >> 7) * kTileBytes + sw128_offset(qr & (kRows - 1), c);
         if (kp.q_vec) {
           cp_async16(dst, there ? src : static_cast<const T*>(p.q), there ? 16 : 0);  // 0: zeros
@@ -459,6 +466,9 @@ __global__ void __maxnreg__(96)
           }
           *reinterpret_cast<uint4*>(dst) = v;
         }
+        src += step_off;
+        hl += step_h;
+        if (hl >= P.group) hl -= P.group, src += wrap_off;
       }
     };
     auto q_ready = [&]() {
@@ -478,7 +488,7 @@ __global__ void __maxnreg__(96)
       uint8_t* at0 = smem + L::kV + stage * kTileBytes;
       // an exponent of ones carries into the sign bit when its lowest bit is added
       constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u, kLow = kBf16 ? 0x0080u : 0x0400u;
-      constexpr int kStepRows = kQThreads / kRowChunks, kAtOnce = 8;
+      constexpr int kAtOnce = 8;
       bool found = false;
       for (int vr0 = v0 + tid / kRowChunks; vr0 < kKeys; vr0 += kStepRows * kAtOnce) {
         uint4 v[kAtOnce];
@@ -555,6 +565,10 @@ __global__ void __maxnreg__(96)
       int t, hl;
       unit.at(P, block * kRows + r, t, hl);
       t = min(t, seg.queries - 1);
+      if (half == 0 && active && P.mask != nullptr && (seg.k_hi > seg.len / kKeys)) {  // the row's mask, needed last
+        const int64_t row = p.q_start != nullptr ? int64_t(p.q_start[seg.b]) + t : int64_t(seg.b) * p.query_len + t;
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(P.mask + row * P.mask_words) : "memory");
+      }
       float m_run = -INFINITY, l_run = 0.f;
       for (int i = kDual ? 0 : x; i < n; i += kDual ? 1 : 2, ++sc) {
         mbar_wait(&sh->s_full[x], sc & 1, err, abort);

@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
   const int here = min(rows - int(blockIdx.y) * kMergeRows, kMergeRows);  // rows of this CTA
   if (here <= 0) return;
   const int dims4 = p.head_dim / 4;
-  constexpr int kAhead = 2;
+  constexpr int kAhead = kGroups <= 4 ? 4 : 2;
   float m = -INFINITY, l = 0.f;
   float4 o[kGroups];
 #pragma unroll
