@@ -1562,7 +1562,7 @@ int hyt_sparse_attention(const void* q, const int64_t* q_strides, const void* k_
   if (page_table_width < 1 || (batch > 1 && page_table_width > page_table_stride))
     return fail(HYT_ERR_INVALID, "page_table_width must be positive and at most the row stride");
   if (page_table_width > hyt::kSelectMaxPages)
-    return fail(HYT_ERR_UNSUPPORTED, "a request may have at most 16384 pages");
+    return fail(HYT_ERR_UNSUPPORTED, "a request may have at most 8192 pages");
   if (int64_t(batch) * num_kv_heads * num_pages > INT32_MAX)
     return fail(HYT_ERR_UNSUPPORTED, "batch times KV heads times num_pages is too large");
   const size_t ids = align256(size_t(batch) * num_kv_heads * num_pages * 4), lens = align256(size_t(batch) * 4);

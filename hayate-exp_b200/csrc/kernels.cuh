@@ -271,7 +271,7 @@ struct SelectParams {
   int32_t ranked;        // pages a selection can rank (set by run_select_pages)
   int32_t* error_word;
 };
-constexpr int kSelectMaxPages = 16384;  // pages of one request that a selection can rank
+constexpr int kSelectMaxPages = 8192;   // pages of one request that a selection can rank
 cudaError_t run_select_pages(const SelectParams& p, int dtype, cudaStream_t stream);
 
 // Runs the bounded mbarrier wait into its time limit (see self_test.cu).

@@ -35,7 +35,7 @@ namespace hyt {
 namespace {
 
 constexpr int kBoundsThreads = 256;
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 128;
 
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
@@ -248,8 +248,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   constexpr bool kTensor = sizeof(T) == 2;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int kWarps = kSelectThreads / 32;
-  extern __shared__ __align__(16) uint32_t keys[];  // [last], then as many page ids and list entries; the
-  int32_t* ids = reinterpret_cast<int32_t*>(keys) + p.ranked;  // first CTA's are used
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  // [last] keys, page ids and list entries (the first CTA's are used), then the bounds' ring
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem_raw);
+  int32_t* ids = reinterpret_cast<int32_t*>(keys) + p.ranked;
   int32_t* doubtful = ids + p.ranked;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -265,6 +267,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
 
   const int64_t out_row = (int64_t(b) * p.num_kv_heads + g) * p.take;
   const int32_t* table = p.page_table + int64_t(b) * p.page_table_stride;
+  if (kTensor && warp == 0 && lane < 2 * group && lane / 2 < group)  // q is needed right after the bounds
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T*>(p.q) + int64_t(b) * p.q_sb +
+                                                  (int64_t(g) * group + lane / 2) * p.q_sh + (lane & 1) * min(64, D - 1)));
   const int len = p.cache_lens[b];
   const int last = len >= 0 ? len >> p.page_shift : p.table_width;  // the page being written
   if (last >= p.table_width || last > kSelectMaxPages) {
@@ -310,20 +315,38 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
     const int n = lane >> 2, j = lane & 3, chunks = D / 8;
     const int first = (rank * kWarps + warp) * 8, stride = ranks * kWarps * 8;
     float magnitude = 0.f;
-    int page = page_at(first + n);
-    for (int i0 = first; i0 < last; i0 += stride) {
+    // the bounds of the next kRing - 1 turns are on their way to shared memory, every lane's
+    // 16-byte pieces to its own places (nobody else reads them)
+    constexpr int kRing = kSteps <= 4 ? 3 : 2;
+    uint4* ring = reinterpret_cast<uint4*>(smem_raw + (p.ranked * 12 + 15) / 16 * 16) + tid;
+    int ahead = first, slot = 0;
+    auto fetch = [&]() {
+      const int page = page_at(ahead + n);
       const uint4* lo = reinterpret_cast<const uint4*>(bounds + int64_t(max(page, 0)) * 2 * D);
-      uint4 l4[kSteps], h4[kSteps];  // all loads of the turn go out together
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
         const int c = j + 4 * t;
-        l4[t] = h4[t] = make_uint4(0u, 0u, 0u, 0u);
-        if (c < chunks) {
-          l4[t] = __ldg(lo + c);
-          h4[t] = __ldg(lo + chunks + c);
-        }
+        const bool there = c < chunks && page >= 0;
+        cp_async16(&ring[(slot * 2 * kSteps + 2 * t) * kSelectThreads], there ? lo + c : lo, there ? 16 : 0);
+        cp_async16(&ring[(slot * 2 * kSteps + 2 * t + 1) * kSelectThreads], there ? lo + chunks + c : lo, there ? 16 : 0);
       }
-      const int next = page_at(i0 + stride + n);
+      cp_async_commit();
+      ahead += stride;
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+      return page;
+    };
+    int ids_ahead[kRing];  // pages of this lane's n in the turns to come
+#pragma unroll
+    for (int k = 0; k < kRing - 1; ++k) ids_ahead[k] = fetch();
+    int at = 0;
+    for (int i0 = first; i0 < last; i0 += stride) {
+      const int page = ids_ahead[0];
+      ids_ahead[kRing - 1] = fetch();
+#pragma unroll
+      for (int k = 0; k < kRing - 1; ++k) ids_ahead[k] = ids_ahead[k + 1];
+      cp_async_wait<kRing - 1>();
+      const uint4* here = &ring[at * 2 * kSteps * kSelectThreads];
+      at = at + 1 == kRing ? 0 : at + 1;
       float top[2] = {-INFINITY, -INFINITY};  // best over the heads, pages 2 j and 2 j + 1
       bool nan[2] = {false, false};
       for (int h0 = 0; h0 < group; h0 += 8) {
@@ -347,7 +370,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
         }
 #pragma unroll
         for (int t = 0; t < kSteps; ++t) {
-          const uint32_t lw[4] = {l4[t].x, l4[t].y, l4[t].z, l4[t].w}, hw[4] = {h4[t].x, h4[t].y, h4[t].z, h4[t].w};
+          const uint4 l4 = here[2 * t * kSelectThreads], h4 = here[(2 * t + 1) * kSelectThreads];
+          const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
           const uint32_t qw[4] = {q4[t].x, q4[t].y, q4[t].z, q4[t].w};
           constexpr uint32_t kAbs = 0x7FFF7FFFu;
 #pragma unroll
@@ -392,8 +416,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
           to_id[i] = id;
         }
       }
-      page = next;
     }
+    cp_async_wait<0>();
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) magnitude = max_nan(magnitude, __shfl_xor_sync(0xffffffffu, magnitude, off));
     // bits of floats >= 0 are ordered like the floats, NaN above all
@@ -423,8 +447,15 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   // counts over the CTA of what each thread counted for three questions; one barrier
   int step = 0;
   auto count3 = [&](int a, int b3, int c, int (&all)[3]) {
-    const int mine[3] = {__reduce_add_sync(0xffffffffu, a), __reduce_add_sync(0xffffffffu, b3),
-                         __reduce_add_sync(0xffffffffu, c)};
+    int mine[3];
+    if (last <= 8 * kSelectThreads) {  // a warp's counts fit 10 bits each: one reduction
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, uint32_t(a) | uint32_t(b3) << 10 | uint32_t(c) << 20);
+      mine[0] = sum & 1023u, mine[1] = (sum >> 10) & 1023u, mine[2] = sum >> 20;
+    } else {
+      mine[0] = __reduce_add_sync(0xffffffffu, a);
+      mine[1] = __reduce_add_sync(0xffffffffu, b3);
+      mine[2] = __reduce_add_sync(0xffffffffu, c);
+    }
 #pragma unroll
     for (int k = 0; k < 3; ++k)
       if (lane == k) counts[step & 1][k][warp] = mine[k];
@@ -441,7 +472,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   // The largest value that at least `want` keys reach (want >= 1), two bits at a time from the
   // highest in which the keys differ: they are scores of one query, so a histogram of their
   // leading bits would pile up in one bin. `exactly`: ended early, exactly `want` keys reach it.
-  bool exactly = false;
+  bool exactly = false, settled = false;
   auto threshold_of = [&]() {
     uint32_t ones = 0xFFFFFFFFu, any = 0u;
     for (int i = tid; i < last; i += kSelectThreads) ones &= keys[i], any |= keys[i];
@@ -505,7 +536,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
     // a NaN key may hide a score of any size (zero times an infinite bound of the other side)
     const bool known = isfinite(score) && isfinite(slack) && all[0] == 0;
     const uint32_t above = known ? above0 : 0xFFFFFFFFu, below = known ? below0 : 0u;
-    const bool settled = known && all[2] == want;  // everything in doubt is in
+    settled = known && all[2] == want;  // everything in doubt is in
     for (int i = tid; i < last; i += kSelectThreads) {
       const uint32_t key = keys[i];
       // refused pages (key 0) stay below everything, NaN keys are summed again
@@ -525,7 +556,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   }
   uint32_t threshold = 0xFFFFFFFFu;  // keys above it are in, and the first `need` of those equal to it
   int need = 0;
-  if (want > 0) {
+  if (settled) {
+    threshold = 0xFFFFFFFEu;  // the keys that are in are all ones by now, the others 0
+  } else if (want > 0) {
     threshold = threshold_of();
     if (exactly) {
       --threshold;  // exactly `want` keys are above threshold - 1 (threshold >= 1)
@@ -608,7 +641,9 @@ cudaError_t run_select_pages(const SelectParams& params, int dtype, cudaStream_t
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(units * ranks));
   config.blockDim = dim3(kSelectThreads);
-  config.dynamicSmemBytes = size_t(ranked) * 12;
+  size_t ring = 0;  // 3 (head_dim above 128: 2) turns of two bounds pieces per step and thread
+  if (dtype != HYT_DTYPE_F32) ring = size_t(kSelectThreads) * 2 * 16 * (p.head_dim <= 128 ? 3 * 4 : 2 * 8);
+  config.dynamicSmemBytes = (size_t(ranked) * 12 + 15) / 16 * 16 + ring;
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;

@@ -433,7 +433,7 @@ int hyt_page_bounds(const void* k_pool, void* k_bounds, int32_t num_layers, int3
  * summed in 64 bits and rounded once to fp32; ties go to the lower page, NaN ranks first.
  * The logical pages read are written to selected [batch, num_kv_heads, num_pages],
  * ascending, -1 past the last. q/out strides = {b, h}. k_bounds must hold hyt_page_bounds of
- * every full page. Limits as for hyt_tree_attention, and at most 16384 pages per request.
+ * every full page. Limits as for hyt_tree_attention, and at most 8192 pages per request.
  * The workspace (hyt_sparse_workspace_bytes) needs no initial contents.
  */
 size_t hyt_sparse_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,

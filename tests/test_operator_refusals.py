@@ -87,7 +87,7 @@ def test_page_bounds_refuses(bad, code, message):
 
 @pytest.mark.parametrize("bad, code, message", [
     (dict(q=None), -1, "null pointer"), (dict(selected=None), -1, "null pointer"), (dict(num_pages=0), -1, "num_pages"),
-    (dict(width=9), -1, "page_table_width"), (dict(stride=20000, width=20000), -2, "16384"),
+    (dict(width=9), -1, "page_table_width"), (dict(stride=20000, width=20000), -2, "8192"),
     (dict(scale=0.0), -1, "scale"), (dict(dim=20), -2, "head_dim"), (dict(bounds=24), -1, "aligned"),
     (dict(), -4, "workspace"), (dict(page=32), -2, "page_size"),
     (dict(num_pages=1 << 28), -2, "too large"),
