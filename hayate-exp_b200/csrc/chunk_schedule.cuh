@@ -20,6 +20,7 @@ namespace hyt {
 
 struct ChunkRequest {
   int len, queries;      // cached tokens, queries of this step
+  int start;             // row of the first query on a packed batch's token axis
   int row_blocks, tiles; // units per KV head, key tiles per unit
   bool refused;          // lengths the page table cannot hold: nothing is visible
 };
@@ -29,7 +30,7 @@ struct ChunkRequest {
 // row holds gets one tile in which nothing is visible, so its rows become zeros.
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& P, int b, int& why) {
   const AttentionParams& p = P.a;
-  ChunkRequest r{0, 0, 0, 0, false};
+  ChunkRequest r{0, 0, 0, 0, 0, false};
   const bool packed = p.q_start != nullptr;
   const int len = p.cache_lens[b];  // the loads go out together
   const int s = packed ? p.q_start[b] : 0;
@@ -41,6 +42,7 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& P, int 
   if (n == 0) return r;
   r.len = len;
   r.queries = n;
+  r.start = s;
   r.row_blocks = int((int64_t(n) * P.group + P.unit_rows - 1) >> P.unit_shift);
   const int64_t kv = int64_t(len) + n;
   if (len < 0 || kv > (int64_t(P.table_width) << p.page_shift) || kv > INT32_MAX - 256) {
@@ -170,6 +172,8 @@ struct ChunkSegment {
   int b, g, row0;        // request, KV head, first row of the unit
   int len, queries, kv;  // cached tokens, queries, their sum
   int k_lo, k_hi;        // key tiles [k_lo, k_hi) of the unit
+  int t0, hl0;           // query and local head of row0
+  int64_t q_base, o_base, mask_row;  // query 0 of head group g in q and out (elements), in the mask (rows)
   bool whole, first, refused;
 };
 
@@ -219,6 +223,12 @@ struct ChunkWalk {
       s.refused = r.refused;
       s.first = !started;
       started = true;
+      s.t0 = s.row0 / P.group;
+      s.hl0 = s.row0 - s.t0 * P.group;
+      const bool packed = P.a.q_start != nullptr;
+      s.q_base = (packed ? int64_t(r.start) * P.a.q_st : int64_t(b) * P.a.q_sb) + int64_t(s.g) * P.group * P.a.q_sh;
+      s.o_base = (packed ? int64_t(r.start) * P.a.o_st : int64_t(b) * P.a.o_sb) + int64_t(s.g) * P.group * P.a.o_sh;
+      s.mask_row = packed ? r.start : int64_t(b) * P.a.query_len;
       return true;
     }
     return false;
@@ -240,6 +250,7 @@ __device__ __forceinline__ void chunk_write_join(const ChunkParams& P, const Chu
       j.g = seg->g;
       j.row0 = seg->row0;
       j.rows = min(seg->queries * P.group - seg->row0, P.unit_rows);
+      j.start = int(P.a.q_start != nullptr ? seg->mask_row : 0);
       j.slot0 = (c - 1) * 2 + (before >= unit_begin ? 0 : 1);
       j.parts = 2;
       while (c - 1 + j.parts < P.ctas && start.begin(c - 1 + j.parts) < unit_end) ++j.parts;
@@ -253,10 +264,7 @@ __device__ __forceinline__ void chunk_write_join(const ChunkParams& P, const Chu
 // (group_magic = ceil(2^20 / group), exact for (group - 1) + r < 1024 and group < 1024).
 struct ChunkRows {
   int t0, hl0;  // query and local head of row0
-  __device__ __forceinline__ ChunkRows(const ChunkParams& P, int row0) {
-    t0 = row0 / P.group;
-    hl0 = row0 - t0 * P.group;
-  }
+  __device__ __forceinline__ ChunkRows(int t, int hl) : t0(t), hl0(hl) {}
   __device__ __forceinline__ void at(const ChunkParams& P, int r, int& t, int& hl) const {
     const int x = hl0 + r;
     const int dt = P.group < 512 ? int((uint32_t(x) * P.group_magic) >> 20) : x / P.group;
@@ -270,10 +278,11 @@ __device__ __forceinline__ const int32_t* chunk_table(const ChunkParams& P, int 
   return P.a.page_table + int64_t(b) * P.a.page_table_stride + int64_t(g) * P.table_head_stride;
 }
 
-// Which of the 64 chunk-local nodes node0 .. node0 + 63 query t of request b sees, as bits
-// (negative nodes are cached tokens: seen by all; nodes from `queries` on exist for nobody).
-// Without a mask the chunk is causal.
-__device__ __forceinline__ uint64_t chunk_visible64(const ChunkParams& P, int b, int t, int queries, int node0) {
+// Which of the 64 chunk-local nodes node0 .. node0 + 63 query t of the segment's request sees, as
+// bits (negative nodes are cached tokens: seen by all; nodes from `queries` on exist for
+// nobody). Without a mask the chunk is causal.
+__device__ __forceinline__ uint64_t chunk_visible64(const ChunkParams& P, const ChunkSegment& seg, int t, int node0) {
+  const int queries = seg.queries;
   if (node0 >= queries || node0 <= -64) return node0 <= -64 ? ~0ull : 0ull;
   const int first = max(node0, 0);
   uint64_t bits = 0;
@@ -281,8 +290,7 @@ __device__ __forceinline__ uint64_t chunk_visible64(const ChunkParams& P, int b,
     const int n = t + 1 - first;  // nodes first .. t
     bits = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
   } else {
-    const int64_t row = P.a.q_start != nullptr ? int64_t(P.a.q_start[b]) + t : int64_t(b) * P.a.query_len + t;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.mask) + row * P.mask_words;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(P.mask) + (seg.mask_row + t) * P.mask_words;
     const int w = first >> 5, sh = first & 31;
     const uint32_t w0 = w < P.mask_words ? words[w] : 0u;
     const uint32_t w1 = w + 1 < P.mask_words ? words[w + 1] : 0u;

@@ -185,7 +185,7 @@ cudaError_t run_norm_rope_scatter(const NormRopeParams& p, int dtype, cudaStream
 // the step's own. `a` is the shared description: packed (a.q_start / a.q_len, q_len 0
 // allowed) or uniform (a.query_len queries each); a.req_ids is not used.
 struct ChunkJoin {  // a unit in parts: CTA c - 1's slot0 and slots 2 (c - 1 + i), i = 1 .. parts - 1
-  int32_t b, g, row0, rows, slot0, parts, pad0, pad1;
+  int32_t b, g, row0, rows, slot0, parts, start, pad;  // start: as ChunkRequest's
 };
 struct ChunkParams {
   AttentionParams a;

@@ -162,7 +162,7 @@ __device__ __noinline__ void add_not_finite(const ChunkParams& P, const ChunkSeg
   const int lo = max(seg.k_lo * kKeys, seg.len), hi = min(seg.k_hi * kKeys, seg.kv);
   const int32_t* table = chunk_table(P, seg.b, seg.g);
   for (int pos = lo; pos < hi; ++pos) {
-    if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
+    if (!(chunk_visible64(P, seg, t, pos - seg.len) & 1)) continue;
     const int32_t page = table[pos >> p.page_shift];
     if (page < 0 || page >= p.num_pages) continue;
     const int64_t vrow = (int64_t(p.layer) * p.num_kv_heads + seg.g) * p.capacity +
@@ -347,16 +347,26 @@ __global__ void __maxnreg__(96)
     int n0 = 0;  // tiles before this segment
     // P and V of tile i of the segment (stream x): V in shared memory and, past the cached tokens,
     // looked through by the checkers, who start as soon as it is there
+    bool told = false;  // the checkers know of the next tile's V already
     auto wait_pv = [&](const ChunkSegment& seg, int x, int i) {
       mbar_wait(&sh->v_full[vr.stage], vr.phase, err, abort);
       const bool check = seg.k_lo + i >= first_checked(seg) && (!kDual || x == 0);
-      if (check && lane == 0) mbar_arrive(&sh->v_check);
+      if (check && !told && lane == 0) mbar_arrive(&sh->v_check);
+      if (!kDual || x == 0) told = false;
       mbar_wait(&sh->p_full[x], p_phase[x], err, abort);
       p_phase[x] ^= 1u;
       if (check) {
         mbar_wait(&sh->v_ok, ok_phase, err, abort);
         ok_phase ^= 1u;
       }
+    };
+    // after tile i was issued (vr: the next one): if the next one's V, to be checked, is there, say so
+    // now, so that the check runs beside the softmax
+    auto tell_ahead = [&](const ChunkSegment& seg, int i, int n) {
+      if (i + 1 >= n || seg.k_lo + i + 1 < first_checked(seg)) return;
+      const bool there = __shfl_sync(0xffffffffu, mbar_try_wait(&sh->v_full[vr.stage], vr.phase) ? 1 : 0, 0) != 0;
+      if (there && lane == 0) mbar_arrive(&sh->v_check);
+      told = there;
     };
     for (int i = 0;; ++i) {
       const ChunkSegment* found = segment(i);
@@ -375,7 +385,7 @@ __global__ void __maxnreg__(96)
             if (s == n - 1) umma_commit(&sh->q_empty);  // no further product reads this Q
           });
         }
-        for (int s = 0; s < n; ++s, vr.next()) {
+        for (int s = 0; s < n; ++s, vr.next(), tell_ahead(seg, s - 1, n)) {
           const int x = s & 1;
           const bool more = s + 2 < n;
           wait_pv(seg, x, s);
@@ -405,7 +415,7 @@ __global__ void __maxnreg__(96)
           if (n == 1) umma_commit(&sh->q_empty);  // no further product reads this Q
         });
         kr.next();
-        for (int j = 0; j < n; ++j, vr.next()) {
+        for (int j = 0; j < n; ++j, vr.next(), tell_ahead(seg, j - 1, n)) {
           const bool more = j + 1 < n;
           wait_pv(seg, 0, j);
           const bool refused = tile_refused(sh, seg, n0 + j);
@@ -447,8 +457,8 @@ __global__ void __maxnreg__(96)
       const int rows = seg.queries * P.group - seg.row0;
       const int upto = min((kDual ? 2 : 1) * kRows, (rows + 31) & ~31);
       int qr = tid / kRowChunks, t, hl;
-      ChunkRows(P, seg.row0).at(P, qr, t, hl);
-      const T* src = static_cast<const T*>(p.q) + att_q_row(p, seg.b, t) + int64_t(seg.g * P.group + hl) * p.q_sh + c * 8;
+      ChunkRows(seg.t0, seg.hl0).at(P, qr, t, hl);
+      const T* src = static_cast<const T*>(p.q) + seg.q_base + t * p.q_st + hl * p.q_sh + c * 8;
 #pragma unroll 4
       for (; qr < upto; qr += kStepRows) {
         const bool there = qr < rows && c * 8 < D;
@@ -559,15 +569,14 @@ __global__ void __maxnreg__(96)
       const ChunkSegment& seg = *found;
       const int n = seg.k_hi - seg.k_lo;
       const int rows_left = seg.queries * P.group - seg.row0;  // may exceed the unit's rows
-      const ChunkRows unit(P, seg.row0);
+      const ChunkRows unit(seg.t0, seg.hl0);
       const int my_rows = rows_left - block * kRows;
       const bool active = quarter * 32 < my_rows;  // warp-uniform: some of the warp's rows exist
       int t, hl;
       unit.at(P, block * kRows + r, t, hl);
       t = min(t, seg.queries - 1);
       if (half == 0 && active && P.mask != nullptr && (seg.k_hi > seg.len / kKeys)) {  // the row's mask, needed last
-        const int64_t row = p.q_start != nullptr ? int64_t(p.q_start[seg.b]) + t : int64_t(seg.b) * p.query_len + t;
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(P.mask + row * P.mask_words) : "memory");
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(P.mask + (seg.mask_row + t) * P.mask_words) : "memory");
       }
       float m_run = -INFINITY, l_run = 0.f;
       for (int i = kDual ? 0 : x; i < n; i += kDual ? 1 : 2, ++sc) {
@@ -592,7 +601,7 @@ __global__ void __maxnreg__(96)
           if (masked) {
             const uint64_t seen = none || r >= my_rows
                                       ? 0ull
-                                      : chunk_visible64(P, seg.b, t, seg.queries, k0 + half * 64 - seg.len);
+                                      : chunk_visible64(P, seg, t, k0 + half * 64 - seg.len);
             const uint32_t seen_lo = uint32_t(seen), seen_hi = uint32_t(seen >> 32);
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
@@ -670,7 +679,7 @@ __global__ void __maxnreg__(96)
         const bool mine = r < my_rows;
         const int unit_row = block * kRows + r;
         T* out = static_cast<T*>(p.out) +
-                 (mine ? att_o_row(p, seg.b, t) + int64_t(seg.g * P.group + hl) * p.o_sh : int64_t(0));
+                 (mine ? seg.o_base + t * p.o_st + hl * p.o_sh : int64_t(0));
         const int64_t slot = int64_t(blockIdx.x) * 2 + (seg.first ? 0 : 1);
 #pragma unroll 1
         for (int c = 0; c < kGroups; ++c) {

@@ -84,20 +84,16 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
     const T* kp = static_cast<const T*>(p.k_pool) + plane * D;
     const T* vp = static_cast<const T*>(p.v_pool) + plane * D;
 
-    const ChunkRows unit(P, seg.row0);
-    auto row_at = [&](int r, int64_t head_stride) {  // query of row r, and its head's offset
-      int t, hl;
-      unit.at(P, r, t, hl);
-      return longlong2{t, int64_t(seg.g * P.group + hl) * head_stride};
-    };
+    const ChunkRows unit(seg.t0, seg.hl0);
     __syncthreads();  // the previous segment's shared tiles are done with
     if (tid == 0) nonfinite = 0;
     for (int i = tid; i < kRows * kD; i += kThreads) {
       const int r = i / kD, d = i - r * kD;
       float v = 0.f;
       if (r < rows_left && d < D) {
-        const longlong2 at = row_at(r, p.q_sh);
-        v = Elem<T>::to_float(static_cast<const T*>(p.q)[att_q_row(p, seg.b, int(at.x)) + at.y + d]);
+        int t, hl;
+        unit.at(P, r, t, hl);
+        v = Elem<T>::to_float(static_cast<const T*>(p.q)[seg.q_base + t * p.q_st + hl * p.q_sh + d]);
       }
       qs[r * kLd + d] = v;
     }
@@ -185,8 +181,11 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
         uint64_t seen = ~0ull;
         if (page < 0 || row >= rows_left)
           seen = 0ull;
-        else if (k0 + kKeys > seg.len)
-          seen = chunk_visible64(P, seg.b, int(row_at(row, 0).x), seg.queries, k0 - seg.len);
+        else if (k0 + kKeys > seg.len) {
+          int t, hl;
+          unit.at(P, row, t, hl);
+          seen = chunk_visible64(P, seg, t, k0 - seg.len);
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -251,12 +250,12 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
     for (int i = 0; i < kR; ++i) {
       const int row = ty * kR + i;
       if (row >= rows_left) continue;
-      const longlong2 at = row_at(row, p.o_sh);
-      const int t = int(at.x);
+      int t, hl;
+      unit.at(P, row, t, hl);
       if (fix && !seg.refused) {  // non-finite V of the nodes this row sees, left out above
         const int lo = max(seg.k_lo * kKeys, seg.len), hi = min(seg.k_hi * kKeys, seg.kv);
         for (int pos = lo; pos < hi; ++pos) {
-          if (!(chunk_visible64(P, seg.b, t, seg.queries, pos - seg.len) & 1)) continue;
+          if (!(chunk_visible64(P, seg, t, pos - seg.len) & 1)) continue;
           const int32_t page = table[pos >> p.page_shift];
           if (page < 0 || page >= p.num_pages) continue;
           const T* vrow = vp + ((int64_t(page) << p.page_shift) + (pos & page_mask)) * D;
@@ -273,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(const
       }
       if (seg.whole) {
         const float inv = l_run[i] == 0.f ? 0.f : 1.f / l_run[i];
-        T* out = static_cast<T*>(p.out) + att_o_row(p, seg.b, t) + at.y;
+        T* out = static_cast<T*>(p.out) + seg.o_base + t * p.o_st + hl * p.o_sh;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
   wait_for_primary();
   const int4 j0 = __ldcg(reinterpret_cast<const int4*>(P.ws_join + c));
   const int4 j1 = __ldcg(reinterpret_cast<const int4*>(P.ws_join + c) + 1);
-  const int b = j0.x, g = j0.y, row0 = j0.z, rows = j0.w, slot0 = j1.x, parts = j1.y;
+  const int b = j0.x, g = j0.y, row0 = j0.z, rows = j0.w, slot0 = j1.x, parts = j1.y, start = j1.z;
   const int here = min(rows - int(blockIdx.y) * kMergeRows, kMergeRows);  // rows of this CTA
   if (here <= 0) return;
   const int dims4 = p.head_dim / 4;
@@ -366,11 +365,12 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
     rows_s[lane][d + 3] = Elem<T>::from_float(o[k].w * inv);
   }
   __syncthreads();
-  const ChunkRows unit(P, row0);
+  const ChunkRows unit(row0 / P.group, row0 % P.group);
+  const int64_t o_base = (p.q_start != nullptr ? int64_t(start) * p.o_st : int64_t(b) * p.o_sb) + int64_t(g) * P.group * p.o_sh;
   for (int r = warp; r < here; r += kMergeThreads / 32) {
     int t, hl;
     unit.at(P, int(blockIdx.y) * kMergeRows + r, t, hl);
-    T* out = static_cast<T*>(p.out) + att_o_row(p, b, t) + int64_t(g * P.group + hl) * p.o_sh;
+    T* out = static_cast<T*>(p.out) + o_base + t * p.o_st + hl * p.o_sh;
 #pragma unroll
     for (int d = lane; d < kGroups * 32; d += 32)
       if (d < p.head_dim) out[d] = rows_s[r][d];
