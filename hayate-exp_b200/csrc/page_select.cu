@@ -1,10 +1,12 @@
 // Page bounds, and the choice of pages a one-token decode reads.
 //
 // page_bounds: elementwise minimum and maximum of a full page's keys, per layer and KV head.
-// One pass over the page: a thread keeps one 16-byte column of every n-th row (16-bit types as
-// packed pairs: half the instructions of widening them), kAhead loads in flight; lanes of one
-// column meet by shuffles, warps in shared memory. NaN keys give NaN bounds. Bound: HBM reads
-// of the keys.
+// A page of one head is contiguous (32 KB at 128 x 128 x 16 bits): a CTA walks some heads of a
+// page and brings their blocks into a ring of kBoundsStages stages with bulk copies, so that
+// the next blocks are on their way while one is looked through (16-bit types as packed pairs:
+// half the instructions of widening them); lanes of one column meet by shuffles, warps in
+// shared memory. One block per CTA without the ring took 61 us on 256 pages x 8 heads x 4
+// layers, whose keys need 42. NaN keys give NaN bounds. Bound: HBM reads of the keys.
 //
 // select_pages: score(page) = max over the KV group's query heads of
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
@@ -26,6 +28,7 @@
 // Bound: HBM reads of the bounds on large batches, the chain of barriers on small ones.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "chunk_schedule.cuh"
@@ -103,12 +106,17 @@ struct MinMax<__half> {
   }
 };
 
-// Grid: (KV head, page entry, layer).
+constexpr int kBoundsStages = 3;
+constexpr int kBoundsBlock = 32 * 1024;  // most bytes of a stage
+
+// Grid: (groups of heads_per_cta KV heads, page entry, layer).
 template <typename T>
-__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsParams p) {
+__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsParams p, int heads_per_cta, int stage_rows) {
   constexpr int kPer = 16 / int(sizeof(T));
   constexpr int kWarps = kBoundsThreads / 32;
-  __shared__ uint4 lo_s[kWarps][64], hi_s[kWarps][64];  // per warp and column (at most 64 of them)
+  extern __shared__ __align__(128) uint8_t ring[];  // [kBoundsStages][stage_rows * D], then per warp and column
+  __shared__ uint64_t full[kBoundsStages];
+  __shared__ int abort_s;
   const int32_t page = p.pages[blockIdx.y];
   if (page == -1) return;
   if (page < 0 || page >= p.num_pages) {
@@ -117,68 +125,103 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
   }
   const int D = p.head_dim, chunks = D / kPer;  // 16-byte columns of a row (<= 64)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rows = 1 << p.page_shift, parts = (rows + stage_rows - 1) / stage_rows;
+  const int head0 = int(blockIdx.x) * heads_per_cta, heads = min(heads_per_cta, p.num_kv_heads - head0);
+  const int items = heads * parts, stage_bytes = stage_rows * D * int(sizeof(T));
+  uint4* lo_s = reinterpret_cast<uint4*>(ring + kBoundsStages * stage_bytes);  // [kWarps][chunks]
+  uint4* hi_s = lo_s + kWarps * chunks;
+  const int64_t plane0 = int64_t(p.first_layer + blockIdx.z) * p.num_kv_heads + head0;
+  if (tid == 0) {
+    abort_s = 0;
+    for (int s = 0; s < kBoundsStages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  auto load = [&](int item) {  // thread 0: block `item` into its stage
+    const int h = item / parts, part = item - h * parts, st = item % kBoundsStages;
+    const int here = min(stage_rows, rows - part * stage_rows);
+    const T* src = static_cast<const T*>(p.k_pool) +
+                   ((plane0 + h) * p.capacity + (int64_t(page) << p.page_shift) + part * stage_rows) * D;
+    mbar_arrive_expect_tx(&full[st], uint32_t(here * D * int(sizeof(T))));
+    bulk_load(ring + st * stage_bytes, src, uint32_t(here * D * int(sizeof(T))), &full[st]);
+  };
+  if (tid == 0)
+    for (int i = 0; i < min(items, kBoundsStages); ++i) load(i);
+  __syncthreads();
+
   // columns that divide a warp's lanes: 32 / chunks rows side by side per warp; else a warp takes
-  // whole rows, ceil(chunks / 32) columns per lane, one after the other
+  // whole rows, ceil(chunks / 32) columns per lane
   const bool side_by_side = chunks <= 32 && 32 % chunks == 0;
   const int per_warp = side_by_side ? 32 / chunks : 1, groups = kWarps * per_warp;
-  const int rows = 1 << p.page_shift;
-  const int64_t plane = int64_t(p.first_layer + blockIdx.z) * p.num_kv_heads + blockIdx.x;
-  const T* keys = static_cast<const T*>(p.k_pool) + (plane * p.capacity + (int64_t(page) << p.page_shift)) * D;
   const int first = side_by_side ? warp * per_warp + lane / chunks : warp;
-  for (int c = side_by_side ? lane % chunks : lane; c < chunks; c += 32) {
-    const T* column = keys + c * kPer;
-    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-    bool any = first < rows;
-    if (any) lo = hi = __ldg(reinterpret_cast<const uint4*>(column + int64_t(first) * D));
-    constexpr int kAhead = 8;
-    for (int r0 = first + groups; r0 < rows; r0 += groups * kAhead) {
-      uint4 v[kAhead];
+  const int columns = side_by_side ? 1 : (chunks + 31) / 32;  // at most 2
+  uint4 lo[2], hi[2];
+  bool any = false;
+  for (int item = 0; item < items; ++item) {
+    const int st = item % kBoundsStages, part = item % parts;
+    const int here = min(stage_rows, rows - part * stage_rows);
+    if (part == 0) any = false;
+    mbar_wait(&full[st], (item / kBoundsStages) & 1, p.error_word, &abort_s);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int r = r0 + u * groups;
-        v[u] = r < rows ? __ldg(reinterpret_cast<const uint4*>(column + int64_t(r) * D)) : lo;
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        lo.x = MinMax<T>::lo(lo.x, v[u].x), hi.x = MinMax<T>::hi(hi.x, v[u].x);
-        lo.y = MinMax<T>::lo(lo.y, v[u].y), hi.y = MinMax<T>::hi(hi.y, v[u].y);
-        lo.z = MinMax<T>::lo(lo.z, v[u].z), hi.z = MinMax<T>::hi(hi.z, v[u].z);
-        lo.w = MinMax<T>::lo(lo.w, v[u].w), hi.w = MinMax<T>::hi(hi.w, v[u].w);
+    for (int k = 0; k < 2; ++k) {
+      const int c = side_by_side ? lane % chunks : lane + 32 * k;
+      if (k >= columns || c >= chunks) continue;
+      const uint4* column = reinterpret_cast<const uint4*>(ring + st * stage_bytes) + c;
+      bool begun = any;
+#pragma unroll 4
+      for (int r = first; r < here; r += groups) {
+        const uint4 v = column[r * chunks];
+        if (!begun) lo[k] = hi[k] = v;
+        begun = true;
+        lo[k].x = MinMax<T>::lo(lo[k].x, v.x), hi[k].x = MinMax<T>::hi(hi[k].x, v.x);
+        lo[k].y = MinMax<T>::lo(lo[k].y, v.y), hi[k].y = MinMax<T>::hi(hi[k].y, v.y);
+        lo[k].z = MinMax<T>::lo(lo[k].z, v.z), hi[k].z = MinMax<T>::hi(hi[k].z, v.z);
+        lo[k].w = MinMax<T>::lo(lo[k].w, v.w), hi[k].w = MinMax<T>::hi(hi[k].w, v.w);
       }
     }
+    any = any || first < here;
+    __syncthreads();  // the stage has been read (and the previous head's columns)
+    if (tid == 0 && item + kBoundsStages < items) load(item + kBoundsStages);
+    if (part != parts - 1) continue;
+    bool mine = any;
     if (side_by_side) {  // rows that exist come first: a lane without one takes its partner's
       for (int off = chunks; off < 32; off <<= 1) {
-        const uint4 a = make_uint4(__shfl_xor_sync(0xffffffffu, lo.x, off), __shfl_xor_sync(0xffffffffu, lo.y, off),
-                                   __shfl_xor_sync(0xffffffffu, lo.z, off), __shfl_xor_sync(0xffffffffu, lo.w, off));
-        const uint4 b = make_uint4(__shfl_xor_sync(0xffffffffu, hi.x, off), __shfl_xor_sync(0xffffffffu, hi.y, off),
-                                   __shfl_xor_sync(0xffffffffu, hi.z, off), __shfl_xor_sync(0xffffffffu, hi.w, off));
-        const bool theirs = __shfl_xor_sync(0xffffffffu, any ? 1 : 0, off) != 0;
-        if (theirs && any) {
-          lo = make_uint4(MinMax<T>::lo(lo.x, a.x), MinMax<T>::lo(lo.y, a.y), MinMax<T>::lo(lo.z, a.z), MinMax<T>::lo(lo.w, a.w));
-          hi = make_uint4(MinMax<T>::hi(hi.x, b.x), MinMax<T>::hi(hi.y, b.y), MinMax<T>::hi(hi.z, b.z), MinMax<T>::hi(hi.w, b.w));
+        const uint4 a = make_uint4(__shfl_xor_sync(0xffffffffu, lo[0].x, off), __shfl_xor_sync(0xffffffffu, lo[0].y, off),
+                                   __shfl_xor_sync(0xffffffffu, lo[0].z, off), __shfl_xor_sync(0xffffffffu, lo[0].w, off));
+        const uint4 b = make_uint4(__shfl_xor_sync(0xffffffffu, hi[0].x, off), __shfl_xor_sync(0xffffffffu, hi[0].y, off),
+                                   __shfl_xor_sync(0xffffffffu, hi[0].z, off), __shfl_xor_sync(0xffffffffu, hi[0].w, off));
+        const bool theirs = __shfl_xor_sync(0xffffffffu, mine ? 1 : 0, off) != 0;
+        if (theirs && mine) {
+          lo[0] = make_uint4(MinMax<T>::lo(lo[0].x, a.x), MinMax<T>::lo(lo[0].y, a.y), MinMax<T>::lo(lo[0].z, a.z), MinMax<T>::lo(lo[0].w, a.w));
+          hi[0] = make_uint4(MinMax<T>::hi(hi[0].x, b.x), MinMax<T>::hi(hi[0].y, b.y), MinMax<T>::hi(hi[0].z, b.z), MinMax<T>::hi(hi[0].w, b.w));
         } else if (theirs) {
-          lo = a, hi = b;
+          lo[0] = a, hi[0] = b;
         }
-        any |= theirs;
+        mine |= theirs;
       }
+      if (lane < chunks) lo_s[warp * chunks + lane] = lo[0], hi_s[warp * chunks + lane] = hi[0];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (lane + 32 * k < chunks) lo_s[warp * chunks + lane + 32 * k] = lo[k], hi_s[warp * chunks + lane + 32 * k] = hi[k];
     }
-    if (!side_by_side || lane < chunks) {
-      lo_s[warp][c] = lo;
-      hi_s[warp][c] = hi;
+    __syncthreads();
+    const int used = min(kWarps, (rows + per_warp - 1) / per_warp);  // warps that had a row (of a full first part)
+    const int words = chunks * 4;
+    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.k_bounds) +
+                                                ((plane0 + item / parts) * p.num_pages + page) * 2 * D);
+    for (int i = tid; i < 2 * words; i += kBoundsThreads) {
+      const bool is_hi = i >= words;
+      const int w = is_hi ? i - words : i;
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(is_hi ? hi_s : lo_s);
+      uint32_t x = from[w];
+      for (int k = 1; k < used; ++k) x = is_hi ? MinMax<T>::hi(x, from[k * words + w]) : MinMax<T>::lo(x, from[k * words + w]);
+      out[i] = x;
     }
   }
-  __syncthreads();
-  const int used = min(kWarps, (rows + per_warp - 1) / per_warp);  // warps that had a row
-  const int words = chunks * 4;
-  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.k_bounds) + (plane * p.num_pages + page) * 2 * D);
-  for (int i = tid; i < 2 * words; i += kBoundsThreads) {
-    const bool is_hi = i >= words;
-    const int w = is_hi ? i - words : i;
-    const uint32_t(*from)[64 * 4] = reinterpret_cast<const uint32_t(*)[64 * 4]>(is_hi ? hi_s : lo_s);
-    uint32_t x = from[0][w];
-    for (int k = 1; k < used; ++k) x = is_hi ? MinMax<T>::hi(x, from[k][w]) : MinMax<T>::lo(x, from[k][w]);
-    out[i] = x;
-  }
+  // every block was waited for above; if a wait gave up, see that no copy is in flight at the exit
+  if (tid == 0 && abort_s)
+    for (int i = max(0, items - kBoundsStages); i < items; ++i) mbar_drain(&full[i % kBoundsStages], (i / kBoundsStages) & 1);
 }
 
 // Order-preserving unsigned key of a score; NaN ranks above everything.
@@ -617,13 +660,24 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
 
 cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t stream) {
   if (p.count == 0 || p.layers == 0) return cudaSuccess;
-  const dim3 grid(unsigned(p.num_kv_heads), unsigned(p.count), unsigned(p.layers));
+  const int row_bytes = p.head_dim * (dtype == HYT_DTYPE_F32 ? 4 : 2), rows = 1 << p.page_shift;
+  const int stage_rows = rows * int64_t(row_bytes) <= kBoundsBlock ? rows : kBoundsBlock / row_bytes;
+  // several blocks per CTA once every SM has a dozen: fewer and the CTAs would be too few
+  const int64_t blocks = int64_t(p.num_kv_heads) * p.count * p.layers;
+  const int heads = int(std::min<int64_t>(p.num_kv_heads, std::max<int64_t>(1, blocks / (148 * 12))));
+  const dim3 grid(unsigned((p.num_kv_heads + heads - 1) / heads), unsigned(p.count), unsigned(p.layers));
+  const int smem = kBoundsStages * stage_rows * row_bytes + 2 * (kBoundsThreads / 32) * row_bytes;
+  auto launch = [&](auto kernel) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kBoundsThreads, smem, stream>>>(p, heads, stage_rows);
+    return cudaGetLastError();
+  };
   switch (dtype) {
-    case HYT_DTYPE_BF16: page_bounds_kernel<__nv_bfloat16><<<grid, kBoundsThreads, 0, stream>>>(p); break;
-    case HYT_DTYPE_F16: page_bounds_kernel<__half><<<grid, kBoundsThreads, 0, stream>>>(p); break;
-    default: page_bounds_kernel<float><<<grid, kBoundsThreads, 0, stream>>>(p); break;
+    case HYT_DTYPE_BF16: return launch(page_bounds_kernel<__nv_bfloat16>);
+    case HYT_DTYPE_F16: return launch(page_bounds_kernel<__half>);
+    default: return launch(page_bounds_kernel<float>);
   }
-  return cudaGetLastError();
 }
 
 cudaError_t run_select_pages(const SelectParams& params, int dtype, cudaStream_t stream) {
