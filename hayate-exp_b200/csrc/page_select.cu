@@ -662,9 +662,9 @@ cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t strea
   if (p.count == 0 || p.layers == 0) return cudaSuccess;
   const int row_bytes = p.head_dim * (dtype == HYT_DTYPE_F32 ? 4 : 2), rows = 1 << p.page_shift;
   const int stage_rows = rows * int64_t(row_bytes) <= kBoundsBlock ? rows : kBoundsBlock / row_bytes;
-  // several blocks per CTA once every SM has a dozen: fewer and the CTAs would be too few
+  // several blocks per CTA once every SM has six
   const int64_t blocks = int64_t(p.num_kv_heads) * p.count * p.layers;
-  const int heads = int(std::min<int64_t>(p.num_kv_heads, std::max<int64_t>(1, blocks / (148 * 12))));
+  const int heads = int(std::min<int64_t>(p.num_kv_heads, std::max<int64_t>(1, blocks / (148 * 6))));
   const dim3 grid(unsigned((p.num_kv_heads + heads - 1) / heads), unsigned(p.count), unsigned(p.layers));
   const int smem = kBoundsStages * stage_rows * row_bytes + 2 * (kBoundsThreads / 32) * row_bytes;
   auto launch = [&](auto kernel) {
