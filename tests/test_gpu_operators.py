@@ -104,6 +104,42 @@ def test_tree_attention(case, dtype):
     Tree(dtype=dtype, seed=len(str(case)), **case).check()
 
 
+SMALL_TREES = [
+    dict(lens=[200, 0, 63], counts=[2, 1, 2], hq=4, hkv=2, dim=8, page=64),
+    dict(lens=[200, 0, 130], counts=[2, 1, 2], hq=4, hkv=2, dim=136),
+    dict(lens=[200, 0, 63], counts=[2, 0, 2], hq=4, hkv=2, dim=256, page=64),
+    dict(lens=[2000, 64, 1], counts=[3, 4, 1], hq=4, hkv=2, dim=40),
+    dict(lens=[2000, 64, 1], counts=[8, 4, 1], hq=3, hkv=3, dim=200),
+    dict(lens=[2000, 64, 1], counts=[4, 3, 1], hq=8, hkv=2, dim=256),
+    dict(lens=[2000, 64, 1], counts=[16, 3, 9], hq=1, hkv=1, dim=192),
+    dict(lens=[500], counts=[1], hq=128, hkv=1, dim=128),
+    dict(lens=[500, 30], counts=[1, 2], hq=600, hkv=1, dim=64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("case", SMALL_TREES, ids=lambda c: "-".join(f"{k}{v}" for k, v in c.items()).replace(" ", "")[:60])
+def test_tree_attention_few_rows_and_other_sharing(case, dtype):
+    Tree(dtype=dtype, seed=len(str(case)) + 1, **case).check()
+
+
+@pytest.mark.parametrize("dtype, dim, hq", [(F32, 128, 2), (F32, 256, 2), (BF16, 256, 4), (F16, 40, 2), (F32, 128, 4)], ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=str)
+def test_few_rows_masked_values_that_are_not_finite(dtype, dim, hq, bad):
+    sees = [np.array([[1, 0], [0, 1]], dtype=bool), np.array([[1, 0], [1, 1]], dtype=bool)]
+    clean = Tree([100, 127], [2, 2], dtype, seed=2, hq=hq, hkv=2, dim=dim, sees=sees)
+    expect = clean.run()
+    dirty = Tree([100, 127], [2, 2], dtype, seed=2, hq=hq, hkv=2, dim=dim, sees=sees)
+    for b, n in enumerate(dirty.lens):
+        for pool in (dirty.k, dirty.v):
+            slot = int(dirty.table[b][(n + 1) // 128]) * 128 + (n + 1) % 128
+            pool[:, :, :, slot:(slot // 128 + 1) * 128] = bad   # node 1 and all behind it
+    out = dirty.run()
+    for b in range(2):  # node 0 of both sees no bad value, node 1 sees itself
+        assert torch.equal(out[0, :, 2 * b], expect[0, :, 2 * b])
+        assert not torch.isfinite(out[0, :, 2 * b + 1].float()).any()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
 def test_tree_attention_arbitrary_masks_and_empty_rows(dtype):
     rng = np.random.RandomState(5)
