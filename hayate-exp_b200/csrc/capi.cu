@@ -619,6 +619,7 @@ int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t
     return fail(HYT_ERR_WORKSPACE, "workspace missing, not 16-byte aligned or too small");
   c.group = g.num_q_heads / g.num_kv_heads;
   const int64_t rows = chunk_max_rows(g.num_q_heads, g.num_kv_heads, g.query_len);
+  if (rows > INT32_MAX / 2) return fail(HYT_ERR_UNSUPPORTED, "too many query rows per KV head");
   const bool tensor = g.dtype != HYT_DTYPE_F32 && g.head_dim >= 64 && g.head_dim <= 128 && g.page_size % 128 == 0;
   const hyt::ChunkShape s = tensor ? hyt::chunk_shape_tensor(rows, kSms)
                                    : hyt::chunk_shape_general(rows, g.dtype, g.head_dim, kSms);

@@ -66,6 +66,7 @@ class PagedCacheHandle:
     length: int = 0
     released: bool = False
     aliased: bool = False  # some page may be shared with another request (set by share)
+    bounded: int = 0       # leading full pages whose key bounds are kept (see track_page_bounds)
 
 
 class _MetaUploader:
@@ -182,6 +183,7 @@ class PackedLayout:
     prefill_ids: torch.Tensor  # the others (tcgen05 prefill kernel)
     # a step of drafted trees (begin_tree_batch):
     parents: list[list[int]] | None = None      # parent of each node, -1: the cached context
+    owners: list[tuple] | None = None           # (handle, pages the nodes' rows are in) per request
     tree_mask: torch.Tensor | None = None       # [total_tokens, words] int32 visibility bits
     token_depth: torch.Tensor | None = None     # [total_tokens] int32: position past the context
 
@@ -507,6 +509,8 @@ class StaticDecodeBatch:
         self.meta.copy_(host[: 4 * self.size], non_blocking=True)
         if self.full_pages is not None:
             full = m._pages_filled(handles, lengths, [1] * n)
+            for handle, length in zip(handles, lengths):
+                handle.bounded = (length + 1) // m.page_size
             h[4 * self.size: 4 * self.size + len(full)] = full
             self.full_pages.copy_(host[4 * self.size:], non_blocking=True)
         if m.device.type == "cuda":
@@ -631,6 +635,7 @@ class PagedKVCacheManager:
             self._page_refs[page] += 1
         handle.pages = list(pages)
         handle.length = num_tokens
+        handle.bounded = min(source.bounded, num_tokens // self.page_size)
         if pages:
             handle.aliased = source.aliased = True
         self._rows.set_row(handle.slot, handle.pages)
@@ -817,6 +822,8 @@ class PagedKVCacheManager:
                     self._make_writable(handle, length, length + n - 1, pairs)
         finally:
             self._copy_pages(pairs)
+        if self.k_bounds is not None:
+            self._bound_missed(handles, lengths)
 
         return lengths, query_lens, kv_lengths
 
@@ -850,9 +857,8 @@ class PagedKVCacheManager:
             built = PagedKVBatch(self, table, meta[: 2 * batch].view(torch.int64),
                                  meta[2 * batch: 3 * batch], query_len, max(kv_lengths), (meta, table),
                                  host_lens=list(lengths))
-            built._full_pages = self._upload_filled(handles, lengths, query_lens)
-            return built
-        built = self._packed_batch(handles, lengths, query_lens, kv_lengths, width, slots)
+        else:
+            built = self._packed_batch(handles, lengths, query_lens, kv_lengths, width, slots)
         built._full_pages = self._upload_filled(handles, lengths, query_lens)
         return built
 
@@ -885,6 +891,8 @@ class PagedKVCacheManager:
                               token_request=meta[o + 3 * batch: end])
         if tree is not None:
             layout.parents = tree[0]
+            layout.owners = [(handle, self._pages_of(handle, length, n))
+                             for handle, length, n in zip(handles, lengths, query_lens)]
             layout.token_depth = meta[end: end + total]
             layout.tree_mask = meta[end + total:].view(total, -1)
         return PagedKVBatch(self, table, meta[: 2 * batch].view(torch.int64), meta[2 * batch: 3 * batch],
@@ -928,10 +936,13 @@ class PagedKVCacheManager:
         if len(handles) != len(layout.parents) or len(accepted) != len(handles):
             raise ValueError("commit_tree needs the step's handles and one path per request")
         paths = [[int(i) for i in path] for path in accepted]
-        for handle, path, tree, length in zip(handles, paths, layout.parents, batch._host_lens):
+        for handle, path, tree, length, (owner, pages) in zip(handles, paths, layout.parents,
+                                                              batch._host_lens, layout.owners):
+            if handle is not owner:
+                raise ValueError("commit_tree takes the handles of begin_tree_batch in their order")
             if handle.released:
                 raise RuntimeError("cannot commit a released cache handle")
-            if handle.length != length or length + len(tree) > len(handle.pages) * self.page_size:
+            if handle.length != length or self._pages_of(handle, length, len(tree)) != pages:
                 raise RuntimeError("the cache handle changed since its tree batch began")
             if any(i < 0 or i >= len(tree) for i in path) or any(
                     tree[i] != before for i, before in zip(path, [-1] + path)):
@@ -958,13 +969,18 @@ class PagedKVCacheManager:
         for handle, n in zip(handles, grown):
             handle.length += n
 
+    def _pages_of(self, handle: PagedCacheHandle, first: int, count: int) -> list[int]:
+        """Pages that positions ``first .. first + count - 1`` of a request are in."""
+        return handle.pages[first // self.page_size: -(-(first + count) // self.page_size)]
+
     # ------------------------------------------------------------------ page bounds
     def track_page_bounds(self) -> None:
         """Keep the elementwise minimum and maximum of every full page's keys from now on
         (``k_bounds``, ``[layers, H_kv, num_pages, 2, head_dim]``: 2 / page_size of the K pool), for
-        ``PagedKVBatch.attend_pages``. Steps, imports and accepted trees keep them up to date;
-        call ``refresh_page_bounds`` after writing to the pools yourself. Batches that exist
-        already do not keep them."""
+        ``PagedKVBatch.attend_pages``. Steps, imports and accepted trees keep them up to date
+        (pages that a step without them filled, one begun before this call for instance, are
+        made up for when the request's next step begins); call ``refresh_page_bounds`` after
+        changing cached keys yourself."""
         if self.k_bounds is not None:
             return
         if self.device.type != "cuda":
@@ -978,6 +994,16 @@ class PagedKVCacheManager:
         if handle.released:
             raise RuntimeError("cannot refresh the bounds of a released cache handle")
         self._bound_pages(handle.pages[: handle.length // self.page_size])
+        if self.k_bounds is not None:
+            handle.bounded = handle.length // self.page_size
+
+    def _bound_missed(self, handles, lengths) -> None:
+        """Bounds of the full pages in front of a step that no step before it kept."""
+        size = self.page_size
+        self._bound_pages([page for handle, length in zip(handles, lengths) if handle.bounded < length // size
+                           for page in handle.pages[handle.bounded: length // size]])
+        for handle, length in zip(handles, lengths):
+            handle.bounded = length // size
 
     def _bound_pages(self, pages) -> None:
         if self.k_bounds is None or not len(pages):
@@ -996,6 +1022,8 @@ class PagedKVCacheManager:
         if self.k_bounds is None:
             return None
         pages = self._pages_filled(handles, lengths, grown)
+        for handle, length, n in zip(handles, lengths, grown):
+            handle.bounded = (length + n) // self.page_size
         return self._uploader.upload(np.asarray(pages, dtype=np.int32)) if pages else None
 
     def commit_batch(self, handles: Sequence[PagedCacheHandle], query_len: int | Sequence[int]) -> None:

@@ -173,6 +173,43 @@ def test_forks_decode_apart_from_each_other():
     m.check_device_errors()
 
 
+@pytest.mark.parametrize("how", ["older batch", "tree as a chain", "older graph batch", "shared"])
+def test_bounds_missed_by_a_step_are_made_up_for(how):
+    """Pages filled by steps that keep no bounds have them once the next step begins."""
+    m, hs = manager_with([250, 120], BF16, 11, extra=8)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(1, 8, 40, 128, generator=gen, device="cuda").to(BF16)
+    if how == "older graph batch":
+        static = m.static_decode_batch(2, 2048, 32)
+        m.track_page_bounds()
+        for at in range(20):
+            static.update(hs)
+            for layer in range(LAYERS):
+                static.batch.write_layer(layer, k[:, :, at:at + 2], k[:, :, at:at + 2])
+            m.commit_batch(hs, 1)
+    else:
+        if how == "tree as a chain":
+            m.track_page_bounds()
+            batch = m.begin_tree_batch(hs, [[i - 1 for i in range(20)]] * 2)
+        else:
+            batch = m.begin_batch(hs, [20, 20])
+            m.track_page_bounds()
+        for layer in range(LAYERS):
+            batch.write_layer(layer, k, k)
+        m.commit_batch(hs, [20, 20])
+        if how == "shared":
+            hs = [m.share(h, h.length) for h in hs]
+    batch = m.begin_batch(hs, 1)
+    assert bounds_are_right(m, hs)
+    q, k1, v1 = W.step_inputs(m, hs, 1, 32, gen)
+    for layer in range(LAYERS):
+        batch.write_layer(layer, k1, v1)
+        _, chosen = batch.attend_pages(q, layer, 2)
+        expect = U.selection_reference(q, m.k_bounds, layer, batch.page_table.cpu().numpy(), [h.length for h in hs], 128, 2)
+        assert np.array_equal(chosen.cpu().numpy(), expect)
+    m.check_device_errors()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_page_sparse_decode_through_the_manager(dtype):
     """Bounds kept through prefill, packed, decode, import and shared pages; every step's rows

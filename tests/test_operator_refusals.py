@@ -43,6 +43,7 @@ SPARSE = dict(q=16, qs=S2, k=16, v=16, bounds=16, layers=2, layer=0, capacity=40
     (dict(dim=12), -2, "head_dim"), (dict(dim=264), -2, "head_dim"), (dict(page=32), -2, "page_size"),
     (dict(page=96), -1, "power of two"), (dict(k=8), -1, "aligned"), (dict(), -4, "workspace"),
     (dict(ws=16, ws_bytes=100), -4, "workspace"), (dict(ws=8, ws_bytes=1 << 40), -4, "workspace"),
+    (dict(ws=16, ws_bytes=1 << 40, hq=800, max_query_len=1 << 24, mask=None), -2, "rows"),
 ])
 def test_tree_attention_refuses(bad, code, message):
     rc, said = _call("hyt_tree_attention", TREE, **bad)

@@ -115,6 +115,37 @@ def test_commit_tree_refusals():
         m.commit_tree(batch, [a, b], [[0], []])
 
 
+def test_commit_tree_takes_the_handles_in_their_order():
+    """Two requests of one length and one tree: swapped, each would get the other's path."""
+    m = make_manager()
+    a, b = grown(m, 10), grown(m, 10)
+    batch = m.begin_tree_batch([a, b], [[-1, 0, 0]] * 2)
+    before = m.k_cache.clone()
+    with pytest.raises(ValueError, match="order"):
+        m.commit_tree(batch, [b, a], [[0, 2], [0]])
+    with pytest.raises(ValueError, match="order"):
+        m.commit_tree(batch, [a, a], [[0, 2], [0]])
+    assert torch.equal(m.k_cache, before) and a.length == b.length == 10
+    m.commit_tree(batch, [a, b], [[0, 2], [0]])
+    assert a.length == 12 and b.length == 11
+
+
+def test_commit_tree_refuses_a_request_whose_pages_changed():
+    """The batch's page table is as old as the batch: rows are not moved through a stale one."""
+    m = make_manager()
+    a, b = grown(m, 126), grown(m, 10)
+    batch = m.begin_tree_batch([a], [[-1, 0, 0, 1, 1]])
+    m.truncate(a, 126)        # gives the second page back
+    with pytest.raises(RuntimeError, match="changed"):
+        m.commit_tree(batch, [a], [[0, 2]])
+    m.begin_batch([b], 200)   # and another request takes it
+    m.reserve(a, 131)
+    before = m.k_cache.clone()
+    with pytest.raises(RuntimeError, match="changed"):
+        m.commit_tree(batch, [a], [[0, 2]])
+    assert torch.equal(m.k_cache, before) and a.length == 126
+
+
 def test_fork_shares_full_pages_and_copies_the_one_being_written():
     m = make_manager()
     h = grown(m, 300)
