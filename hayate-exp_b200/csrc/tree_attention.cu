@@ -144,9 +144,9 @@ __device__ __noinline__ void store_unaligned16(void* at, uint4 w) {
   e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
 }
 
-// The CTA's n-th tile, of segment `seg`: nothing of it is visible, its stages hold something else.
-__device__ __forceinline__ bool tile_refused(const Shared* sh, const ChunkSegment& seg, int n) {
-  return seg.refused || *reinterpret_cast<const volatile int32_t*>(&sh->refused[n & 7]) != 0;
+// The CTA's n-th tile: nothing of it is visible, its stages hold something else.
+__device__ __forceinline__ bool tile_refused(const Shared* sh, int n) {
+  return *reinterpret_cast<const volatile int32_t*>(&sh->refused[n & 7]) != 0;
 }
 // First tile of the segment that reaches past the cached tokens: from there on V is checked.
 __device__ __forceinline__ int first_checked(const ChunkSegment& seg) {
@@ -389,7 +389,7 @@ __global__ void __maxnreg__(96)
           const int x = s & 1;
           const bool more = s + 2 < n;
           wait_pv(seg, x, s);
-          const bool refused = tile_refused(sh, seg, n0 + s);
+          const bool refused = tile_refused(sh, n0 + s);
           issue([&] {
             if (!refused) pv(x, vr.stage, (begun >> x) & 1u);
             umma_commit(&sh->v_empty[vr.stage]);
@@ -418,7 +418,7 @@ __global__ void __maxnreg__(96)
         for (int j = 0; j < n; ++j, vr.next(), tell_ahead(seg, j - 1, n)) {
           const bool more = j + 1 < n;
           wait_pv(seg, 0, j);
-          const bool refused = tile_refused(sh, seg, n0 + j);
+          const bool refused = tile_refused(sh, n0 + j);
           if (more) mbar_wait(&sh->k_full[kr.stage], kr.phase, err, abort);
           issue([&] {
             if (!refused) pv(0, vr.stage, begun != 0u);
@@ -528,8 +528,8 @@ __global__ void __maxnreg__(96)
       fence_proxy_async_smem();
       mbar_arrive(&sh->v_ok);
     };
-    // Per segment: the tiles to check but the last; then, once the segment's last S is done, the
-    // next segment's Q on its way; then the last tile
+    // Per segment: the tiles to check; then, once the segment's last S is done, the next segment's Q
+    // (Q before the last tile's check held up that tile's PV by 9,000 cycles)
     const ChunkSegment* now = segment(0);
     if (now != nullptr) {
       load_q(*now);
@@ -539,12 +539,13 @@ __global__ void __maxnreg__(96)
       const ChunkSegment seg = *now;
       const int n = seg.k_hi - seg.k_lo;
       const int first = first_checked(seg);
-      for (int tile = first; tile < seg.k_hi - 1; ++tile) check_v(seg, i, tile, n0 + tile - seg.k_lo);
+      for (int tile = first; tile < seg.k_hi; ++tile) check_v(seg, i, tile, n0 + tile - seg.k_lo);
       mbar_wait(&sh->q_empty, i & 1, err, abort);
       now = segment(i + 1);
-      if (now != nullptr) load_q(*now);
-      if (first < seg.k_hi) check_v(seg, i, seg.k_hi - 1, n0 + n - 1);
-      if (now != nullptr) q_ready();
+      if (now != nullptr) {
+        load_q(*now);
+        q_ready();
+      }
       n0 += n;
     }
   } else {
@@ -569,29 +570,34 @@ __global__ void __maxnreg__(96)
       const ChunkSegment& seg = *found;
       const int n = seg.k_hi - seg.k_lo;
       const int rows_left = seg.queries * P.group - seg.row0;  // may exceed the unit's rows
-      const ChunkRows unit(seg.t0, seg.hl0);
       const int my_rows = rows_left - block * kRows;
       const bool active = quarter * 32 < my_rows;  // warp-uniform: some of the warp's rows exist
-      int t, hl;
-      unit.at(P, block * kRows + r, t, hl);
-      t = min(t, seg.queries - 1);
+      auto query = [&](int& t, int& hl) {  // of this row
+        ChunkRows(seg.t0, seg.hl0).at(P, block * kRows + r, t, hl);
+        t = min(t, seg.queries - 1);
+      };
       if (half == 0 && active && P.mask != nullptr && (seg.k_hi > seg.len / kKeys)) {  // the row's mask, needed last
+        int t, hl;
+        query(t, hl);
         asm volatile("prefetch.global.L1 [%0];" ::"l"(P.mask + (seg.mask_row + t) * P.mask_words) : "memory");
       }
       float m_run = -INFINITY, l_run = 0.f;
-      for (int i = kDual ? 0 : x; i < n; i += kDual ? 1 : 2, ++sc) {
+      // of the CTA's tiles: the segment's end and the first that reaches past the cached tokens
+      const int end = n0 + n, tail = n0 + max(seg.len / kKeys - seg.k_lo, 0);
+      for (int i = n0 + (kDual ? 0 : x); i < end; i += kDual ? 1 : 2) {
+        if constexpr (kDual) sc = uint32_t(i);
         mbar_wait(&sh->s_full[x], sc & 1, err, abort);
         tc_fence_after();
-        const int k0 = (seg.k_lo + i) * kKeys;
-        const bool none = tile_refused(sh, seg, n0 + i);
-        const bool masked = none || k0 + kKeys > seg.len;
         __syncwarp();
         if (active) {
           float s[64];
+          bool none, masked;
           {
             uint32_t raw[2][32];
             tmem_ld32(s_addr, raw[0]);
             tmem_ld32(s_addr + 32, raw[1]);
+            none = tile_refused(sh, i);  // beside the loads
+            masked = none || i >= tail;
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -599,9 +605,11 @@ __global__ void __maxnreg__(96)
               for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(raw[c][e]);
           }
           if (masked) {
+            int t, hl;
+            query(t, hl);
             const uint64_t seen = none || r >= my_rows
                                       ? 0ull
-                                      : chunk_visible64(P, seg, t, k0 + half * 64 - seg.len);
+                                      : chunk_visible64(P, seg, t, (seg.k_hi - (end - i)) * kKeys + half * 64 - seg.len);
             const uint32_t seen_lo = uint32_t(seen), seen_hi = uint32_t(seen >> 32);
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
@@ -627,8 +635,10 @@ __global__ void __maxnreg__(96)
             m_run = m_new;
           }
           const float tile_sum = exp_tile<T>(s, scale2, m_run == -INFINITY ? 0.f : m_run, p_addr);
+          const float l_before = l_run;
           l_run = l_run * alpha + tile_sum;
-          if (moves && i >= (kDual ? 1 : 2)) {  // O_x is stable: its last PV completed before S_x did
+          // O_x holds something (each row's, or zeros), and is stable: its last PV completed before S_x did
+          if (moves && __any_sync(0xffffffffu, l_before != 0.f)) {
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               uint32_t o[32];
@@ -643,6 +653,7 @@ __global__ void __maxnreg__(96)
         }
         tc_fence_before();
         mbar_arrive(&sh->p_full[x]);
+        if constexpr (!kDual) ++sc;
       }
 
       // ---- epilogue
@@ -677,6 +688,8 @@ __global__ void __maxnreg__(96)
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const bool mine = r < my_rows;
+        int t, hl;
+        query(t, hl);
         const int unit_row = block * kRows + r;
         T* out = static_cast<T*>(p.out) +
                  (mine ? seg.o_base + t * p.o_st + hl * p.o_sh : int64_t(0));
@@ -736,7 +749,7 @@ __global__ void __maxnreg__(96)
       // is two segments on, after another of these barriers)
       named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
       if (threadIdx.x == 0) sh->fix[segs & 1] = 0;
-      n0 += n;
+      n0 = end;
       ++segs;
     }
   }

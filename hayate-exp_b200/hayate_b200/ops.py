@@ -43,21 +43,23 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _bht_strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
-    if t.dim() != 4:
+    strides = t.stride()
+    if len(strides) != 4:
         raise ValueError(f"{name} must be [batch, heads, tokens, head_dim]")
-    if t.stride(3) != 1 and t.size(3) > 1:
+    if strides[3] != 1 and t.size(3) > 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    return t.stride(0), t.stride(1), t.stride(2)
+    return strides[0], strides[1], strides[2]
 
 
 def _pool_geometry(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple[int, int, int, int]:
-    if k_pool.dim() != 5 or k_pool.size(1) != 1:
+    shape = k_pool.shape
+    if len(shape) != 5 or shape[1] != 1:
         raise ValueError("pools must be [num_layers, 1, num_kv_heads, capacity_tokens, head_dim]")
-    if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+    if v_pool is not k_pool and (shape != v_pool.shape or k_pool.dtype != v_pool.dtype):
         raise ValueError("K and V pools must have the same shape and dtype")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("pools must be contiguous")
-    num_layers, _, heads, capacity, head_dim = k_pool.shape
+    num_layers, _, heads, capacity, head_dim = shape
     return num_layers, heads, capacity, head_dim
 
 
@@ -260,11 +262,12 @@ def paged_attention_scatter(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.T
 # ---------------------------------------------------------------------------- packed batches
 def _th_strides(t: torch.Tensor, name: str) -> tuple[int, int]:
     """Element strides {token, head} of a ``[1, H, N, D]`` packed tensor."""
-    if t.dim() != 4 or t.shape[0] != 1:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 4 or shape[0] != 1:
         raise ValueError(f"{name} must be [1, heads, total_tokens, head_dim]")
-    if t.stride(3) != 1 and t.size(3) > 1:
+    if strides[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    return t.stride(2), t.stride(1)
+    return strides[2], strides[1]
 
 
 def _int32_cuda(*tensors: torch.Tensor) -> None:
@@ -556,29 +559,30 @@ def _int32_vector(t: torch.Tensor, name: str, numel: int | None = None) -> None:
 
 def _page_rows(page_table: torch.Tensor, batch: int) -> tuple[int, int]:
     """(entries between rows, entries of a row) of an int32 ``[batch, pages]`` table."""
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.size(0) != batch:
+    shape, strides = page_table.shape, page_table.stride()
+    if page_table.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch:
         raise ValueError("page_table must be an int32 [batch, pages] tensor")
-    width = page_table.size(1)
-    if width < 1 or (width > 1 and page_table.stride(1) != 1):
+    width, row = shape[1], strides[0]
+    if width < 1 or (width > 1 and strides[1] != 1):
         raise ValueError("page_table must have at least one page per row and contiguous rows")
-    if batch > 1 and page_table.stride(0) < width:
+    if batch > 1 and row < width:
         raise ValueError("page_table rows must not overlap")
-    return max(page_table.stride(0), width), width
+    return max(row, width), width
 
 
 def _output(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     """``out`` checked against ``like`` ``[B, H, T, D]``, or a new one in ``[B, T, H, D]`` memory."""
     if out is None:
         b, h, t, d = like.shape
-        return torch.empty_strided((b, h, t, d), (t * h * d, d, h * d, 1), dtype=like.dtype, device=like.device)
+        return like.new_empty_strided((b, h, t, d), (t * h * d, d, h * d, 1))
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError("out must match q")
     return out
 
 
-def _scratch(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
+def _scratch(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
+        return like.new_empty(need, dtype=torch.uint8)
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
         raise RuntimeError(f"the workspace must be a contiguous uint8 tensor of at least {need} bytes")
     return workspace
@@ -613,25 +617,27 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     num_layers, num_kv_heads, capacity, head_dim = _pool_geometry(k_pool, v_pool)
     qs = _th_strides(q, "q")
     _, num_q_heads, total, d = q.shape
-    if d != head_dim or q.dtype != k_pool.dtype:
+    dtype = q.dtype
+    if d != head_dim or dtype != k_pool.dtype:
         raise ValueError("q must match the pool's head_dim and dtype")
     batch = cache_lens.numel()
-    for t, name in ((cache_lens, "cache_lens"), (q_start, "q_start"), (q_len, "q_len")):
-        _int32_vector(t, name, batch)
+    _int32_vector(cache_lens, "cache_lens", batch)
+    _int32_vector(q_start, "q_start", batch)
+    _int32_vector(q_len, "q_len", batch)
     stride, width = _page_rows(page_table, batch)
     words = 0
     if tree_mask is not None:
         if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or not tree_mask.is_contiguous():
             raise TypeError("tree_mask must be a contiguous int32 [tokens, words] tensor")
-        words = tree_mask.size(1)
-        if tree_mask.size(0) != total or words * 32 < max_query_len:
+        rows, words = tree_mask.shape
+        if rows != total or words * 32 < max_query_len:
             raise ValueError("tree_mask must have a row per token and a bit per node")
     out = _output(out, q)
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     if total == 0:
         return out
-    need = tree_workspace_bytes(max_query_len, num_q_heads, num_kv_heads, head_dim, q.dtype)
-    workspace = _scratch(workspace, need, q.device)
+    need = tree_workspace_bytes(max_query_len, num_q_heads, num_kv_heads, head_dim, dtype)
+    workspace = _scratch(workspace, need, q)
     rc = _on_device(
         index, _lib.lib().hyt_tree_attention, q.data_ptr(), _lib.int64_array(qs), k_pool.data_ptr(),
         v_pool.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride, width,
@@ -750,9 +756,9 @@ def sparse_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     if num_pages < 1:
         raise ValueError("num_pages must be positive")
-    selected = torch.empty((batch, num_kv_heads, num_pages), dtype=torch.int32, device=q.device)
+    selected = cache_lens.new_empty((batch, num_kv_heads, num_pages))
     need = sparse_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_pages, q.dtype)
-    workspace = _scratch(workspace, need, q.device)
+    workspace = _scratch(workspace, need, q)
     rc = _on_device(
         index, _lib.lib().hyt_sparse_attention, q.data_ptr(), _lib.int64_array(qs[:2]), k_pool.data_ptr(),
         v_pool.data_ptr(), k_bounds.data_ptr(), num_layers, layer, capacity, page_table.data_ptr(), stride,
