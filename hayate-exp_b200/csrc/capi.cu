@@ -589,6 +589,30 @@ int check_scale(float scale) {
   return HYT_OK;
 }
 
+// Map of a chunk's q as (dim, head, token) for boxes of 64 dims x a KV group's heads x as many
+// tokens as make 32 rows; false where the layout has none (rows off 16-byte boundaries, heads
+// further apart than tokens, groups that do not divide 32): the kernel loads such rows itself.
+bool chunk_q_map(const hyt::ChunkParams& c, const Geometry& g, CUtensorMap* out) {
+  const int64_t eb = elem_bytes(g.dtype);
+  const int64_t tokens = c.a.q_start != nullptr ? c.a.total_tokens : g.batch;
+  const int64_t sh = c.a.q_sh * eb;
+  int64_t st = (c.a.q_start != nullptr ? c.a.q_st : c.a.q_sb) * eb;
+  if (tokens == 1) st = sh * g.num_q_heads;  // any valid stride
+  if (32 % c.group || reinterpret_cast<uintptr_t>(c.a.q) % 16 || sh <= 0 || st < sh || sh % 16 || st % 16 ||
+      st >= (int64_t(1) << 40))
+    return false;
+  EncodeTiledFn encode = encode_fn();
+  if (encode == nullptr) return false;
+  cuuint64_t dims[3] = {cuuint64_t(g.head_dim), cuuint64_t(g.num_q_heads), cuuint64_t(tokens)};
+  cuuint64_t strides[2] = {cuuint64_t(sh), cuuint64_t(st)};
+  cuuint32_t box[3] = {64, cuuint32_t(c.group), cuuint32_t(32 / c.group)};
+  cuuint32_t estrides[3] = {1, 1, 1};
+  return encode(out, g.dtype == HYT_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                3, const_cast<void*>(c.a.q), dims, strides, box, estrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Pool rows that 16-byte loads can read, and pages that no 64-key tile crosses.
 int check_chunk_geometry(const Geometry& g, const void* k_pool, const void* v_pool) {
   if (g.head_dim % 8 || g.head_dim > 256)
@@ -641,9 +665,11 @@ int launch_chunk(hyt::ChunkParams& c, const Geometry& g, void* workspace, size_t
     if (rc != HYT_OK) return rc;
     rc = pool_tensor_map(c.a.v_pool, g.dtype, g.head_dim, g.capacity, planes, kTensorKeys, &v_map);
     if (rc != HYT_OK) return rc;
+    CUtensorMap q_map;
+    const bool q_tma = chunk_q_map(c, g, &q_map);
     const int64_t qs[3] = {c.a.q_sb, c.a.q_sh, c.a.q_st}, os[3] = {c.a.o_sb, c.a.o_sh, c.a.o_st};
     err = hyt::run_chunk_attention_tensor(c, rows_16b_aligned(c.a.q, qs), rows_16b_aligned(c.a.out, os), k_map,
-                                          v_map, g.dtype, stream);
+                                          v_map, q_tma ? &q_map : nullptr, g.dtype, stream);
   } else {
     err = hyt::run_chunk_attention_general(c, g.dtype, stream);
   }

@@ -217,7 +217,7 @@ cudaError_t run_chunk_attention_general(const ChunkParams& p, int dtype, cudaStr
 // bf16 / f16, head_dim 64 .. 128 (a multiple of 8), page_size % 128 == 0; maps with 128-row boxes.
 ChunkShape chunk_shape_tensor(int64_t max_rows, int num_sms);
 cudaError_t run_chunk_attention_tensor(const ChunkParams& p, bool q_vec, bool o_vec, const CUtensorMap& k_map,
-                                       const CUtensorMap& v_map, int dtype, cudaStream_t stream);
+                                       const CUtensorMap& v_map, const CUtensorMap* q_map, int dtype, cudaStream_t stream);
 // Joins the partials of units that several CTAs of `p` shared.
 cudaError_t run_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t stream);
 

@@ -133,6 +133,7 @@ struct Ring {
 struct TreeKernelParams {
   ChunkParams c;
   int32_t q_vec, o_vec;  // q / out rows start on 16-byte boundaries
+  int32_t q_tma;         // q_map holds q as (dim, head, token), boxes of 64 dims x a group's heads x 32 / group tokens
 };
 
 // The rare paths are kept out of line: the code between two segments is fetched cold (the
@@ -186,6 +187,7 @@ template <typename T, bool kDual, int kChunks>
 __global__ void __maxnreg__(96)
     tree_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map,
+                          const __grid_constant__ CUtensorMap q_map,
                           const __grid_constant__ TreeKernelParams kp) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   using L = Layout<kDual>;
@@ -204,7 +206,7 @@ __global__ void __maxnreg__(96)
   if (threadIdx.x == kMmaWarp * 32) {
     sh->abort = 0;
     sh->fix[0] = sh->fix[1] = 0;
-    mbar_init(&sh->q_full, kQThreads);
+    mbar_init(&sh->q_full, kp.q_tma ? 1 : kQThreads);
     mbar_init(&sh->q_empty, 1);
     mbar_init(&sh->v_check, 1);
     mbar_init(&sh->v_ok, kQThreads);
@@ -452,10 +454,24 @@ __global__ void __maxnreg__(96)
     const int c = tid % kRowChunks;
     const int step_t = kStepRows / P.group, step_h = kStepRows - step_t * P.group;
     const int64_t step_off = step_t * p.q_st + step_h * p.q_sh, wrap_off = p.q_st - P.group * p.q_sh;
-    // rows of the 32-row quarters that have any (the others' lanes are never looked at)
+    // rows of the 32-row quarters that have any (the others' lanes are never looked at). By TMA,
+    // rows past the request's are its neighbours' on the token axis: no result comes of them
     auto load_q = [&](const ChunkSegment& seg) {
       const int rows = seg.queries * P.group - seg.row0;
       const int upto = min((kDual ? 2 : 1) * kRows, (rows + 31) & ~31);
+      if (kp.q_tma) {
+        if (tid != 0) return;
+        constexpr int kPartBytes = 32 * 128;  // 32 rows of 64 dims
+        int token = int(seg.mask_row) + seg.t0;
+        mbar_arrive_expect_tx(&sh->q_full, uint32_t(upto / 32 * kChunks * kPartBytes));
+        for (int qr = 0; qr < upto; qr += 32, token += 32 / P.group) {
+          uint8_t* dst = smem + L::kQ + (qr >> 7) * kTileBytes + ((qr & (kRows - 1)) >> 5) * kPartBytes;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(dst + c * kChunkBytes, &q_map, &sh->q_full, c * 64, seg.g * P.group, token);
+        }
+        return;
+      }
       int qr = tid / kRowChunks, t, hl;
       ChunkRows(seg.t0, seg.hl0).at(P, qr, t, hl);
       const T* src = static_cast<const T*>(p.q) + seg.q_base + t * p.q_st + hl * p.q_sh + c * 8;
@@ -482,6 +498,7 @@ __global__ void __maxnreg__(96)
       }
     };
     auto q_ready = [&]() {
+      if (kp.q_tma) return;
       cp_async_wait_all();
       fence_proxy_async_smem();
       mbar_arrive(&sh->q_full);
@@ -530,12 +547,14 @@ __global__ void __maxnreg__(96)
     };
     // Per segment: the tiles to check; then, once the segment's last S is done, the next segment's Q
     // (Q before the last tile's check held up that tile's PV by 9,000 cycles)
+    if (kp.q_tma && tid == 0) tma_prefetch_desc(&q_map);
     const ChunkSegment* now = segment(0);
     if (now != nullptr) {
       load_q(*now);
       q_ready();
     }
-    for (int i = 0, n0 = 0; now != nullptr; ++i) {
+    int i = 0;
+    for (int n0 = 0; now != nullptr; ++i) {
       const ChunkSegment seg = *now;
       const int n = seg.k_hi - seg.k_lo;
       const int first = first_checked(seg);
@@ -548,6 +567,7 @@ __global__ void __maxnreg__(96)
       }
       n0 += n;
     }
+    if (kp.q_tma && tid == 0 && i > 0) mbar_drain(&sh->q_full, (i - 1) & 1);  // nothing in flight when the CTA exits
   } else {
     // ------------------------------------------------------------ softmax warps
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
@@ -765,24 +785,24 @@ __global__ void __maxnreg__(96)
 
 template <typename T, bool kDual, int kChunks>
 cudaError_t launch_tree(const TreeKernelParams& kp, const CUtensorMap& k_map, const CUtensorMap& v_map,
-                        cudaStream_t stream) {
+                        const CUtensorMap& q_map, cudaStream_t stream) {
   auto kernel = tree_attention_kernel<T, kDual, kChunks>;
   constexpr int smem = Layout<kDual>::kBytes;
   static_assert(smem <= 227 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  if (kp.c.after_selection) return launch_after(kernel, dim3(kp.c.ctas), kThreads, smem, stream, k_map, v_map, kp);
-  kernel<<<kp.c.ctas, kThreads, smem, stream>>>(k_map, v_map, kp);
+  if (kp.c.after_selection) return launch_after(kernel, dim3(kp.c.ctas), kThreads, smem, stream, k_map, v_map, q_map, kp);
+  kernel<<<kp.c.ctas, kThreads, smem, stream>>>(k_map, v_map, q_map, kp);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_tree_shape(const TreeKernelParams& kp, const CUtensorMap& k_map, const CUtensorMap& v_map,
-                              cudaStream_t stream) {
+                              const CUtensorMap& q_map, cudaStream_t stream) {
   const bool dual = kp.c.unit_rows > kRows;
   if (kp.c.a.head_dim <= 64)
-    return dual ? launch_tree<T, true, 1>(kp, k_map, v_map, stream) : launch_tree<T, false, 1>(kp, k_map, v_map, stream);
-  return dual ? launch_tree<T, true, 2>(kp, k_map, v_map, stream) : launch_tree<T, false, 2>(kp, k_map, v_map, stream);
+    return dual ? launch_tree<T, true, 1>(kp, k_map, v_map, q_map, stream) : launch_tree<T, false, 1>(kp, k_map, v_map, q_map, stream);
+  return dual ? launch_tree<T, true, 2>(kp, k_map, v_map, q_map, stream) : launch_tree<T, false, 2>(kp, k_map, v_map, q_map, stream);
 }
 
 }  // namespace
@@ -792,10 +812,11 @@ ChunkShape chunk_shape_tensor(int64_t max_rows, int num_sms) {
 }
 
 cudaError_t run_chunk_attention_tensor(const ChunkParams& p, bool q_vec, bool o_vec, const CUtensorMap& k_map,
-                                       const CUtensorMap& v_map, int dtype, cudaStream_t stream) {
-  const TreeKernelParams kp{p, q_vec ? 1 : 0, o_vec ? 1 : 0};
-  return dtype == HYT_DTYPE_F16 ? launch_tree_shape<__half>(kp, k_map, v_map, stream)
-                                : launch_tree_shape<__nv_bfloat16>(kp, k_map, v_map, stream);
+                                       const CUtensorMap& v_map, const CUtensorMap* q, int dtype, cudaStream_t stream) {
+  const TreeKernelParams kp{p, q_vec ? 1 : 0, o_vec ? 1 : 0, q != nullptr ? 1 : 0};
+  const CUtensorMap& q_map = q != nullptr ? *q : k_map;
+  return dtype == HYT_DTYPE_F16 ? launch_tree_shape<__half>(kp, k_map, v_map, q_map, stream)
+                                : launch_tree_shape<__nv_bfloat16>(kp, k_map, v_map, q_map, stream);
 }
 
 }  // namespace hyt
