@@ -145,6 +145,38 @@ __device__ __noinline__ void store_unaligned16(void* at, uint4 w) {
   e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
 }
 
+// acc + 0 * x for a pair of values: +-0 where both are finite so far
+template <typename T>
+__device__ __forceinline__ uint32_t times_zero(uint32_t x, uint32_t acc) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  return r;
+}
+
+// Zeros for the values that are not finite in 16-byte chunk `chunk` of rows first, first + step ..
+// of a tile; whether one is in a row below `rows`.
+template <typename T>
+__device__ __noinline__ bool zero_not_finite(uint8_t* tile, int first, int step, int chunk, int rows) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  bool found = false;
+  for (int r = first; r < kKeys; r += step) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(tile + sw128_offset(r, chunk));
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t was = at[e];
+      uint32_t w = was;
+      if ((w & kExp) == kExp) w &= 0xFFFF0000u;
+      if ((w & (kExp << 16)) == (kExp << 16)) w &= 0x0000FFFFu;
+      if (w == was) continue;
+      at[e] = w;
+      found |= r < rows;
+    }
+  }
+  return found;
+}
+
 // The CTA's n-th tile: nothing of it is visible, its stages hold something else.
 __device__ __forceinline__ bool tile_refused(const Shared* sh, int n) {
   return *reinterpret_cast<const volatile int32_t*>(&sh->refused[n & 7]) != 0;
@@ -504,44 +536,25 @@ __global__ void __maxnreg__(96)
       mbar_arrive(&sh->q_full);
     };
     // V of the CTA's n-th tile: values that are not finite become zeros among the rows past the
-    // cached tokens
+    // cached tokens. A finite value times zero is zero, another is NaN: one FMA per pair of values
     uint32_t check_phase = 0u;
     auto check_v = [&](const ChunkSegment& seg, int i, int tile, int n) {
       const int stage = n % kVStages;
       mbar_wait(&sh->v_check, check_phase, err, abort);
       check_phase ^= 1u;
       mbar_wait(&sh->v_full[stage], (n / kVStages) & 1, err, abort);  // done; orders TMA's writes before the reads
-      const int k0 = tile * kKeys, v0 = max(seg.len - k0, 0);
+      const int k0 = tile * kKeys, v0 = max(seg.len - k0, 0) + tid / kRowChunks;
       uint8_t* at0 = smem + L::kV + stage * kTileBytes;
-      // an exponent of ones carries into the sign bit when its lowest bit is added
-      constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u, kLow = kBf16 ? 0x0080u : 0x0400u;
-      constexpr int kAtOnce = 8;
-      bool found = false;
-      for (int vr0 = v0 + tid / kRowChunks; vr0 < kKeys; vr0 += kStepRows * kAtOnce) {
-        uint4 v[kAtOnce];
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          const int vr = vr0 + u * kStepRows;
-          v[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (vr < kKeys) v[u] = *reinterpret_cast<const uint4*>(at0 + sw128_offset(vr, c));
-        }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w}, ones = 0u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ones |= (w[e] & (kExp * 0x10001u)) + kLow * 0x10001u;
-          if (!(ones & 0x80008000u)) continue;
-          const int vr = vr0 + u * kStepRows;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if ((w[e] & kExp) == kExp) w[e] &= 0xFFFF0000u;
-            if ((w[e] & (kExp << 16)) == (kExp << 16)) w[e] &= 0x0000FFFFu;
-          }
-          *reinterpret_cast<uint4*>(at0 + sw128_offset(vr, c)) = make_uint4(w[0], w[1], w[2], w[3]);
-          found |= k0 + vr < seg.kv;
-        }
+      uint32_t zero[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 8
+      for (int vr = v0; vr < kKeys; vr += kStepRows) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at0 + sw128_offset(vr, c));
+        zero[0] = times_zero<T>(v.x, zero[0]), zero[1] = times_zero<T>(v.y, zero[1]);
+        zero[2] = times_zero<T>(v.z, zero[2]), zero[3] = times_zero<T>(v.w, zero[3]);
       }
-      if (found) *reinterpret_cast<volatile int32_t*>(&sh->fix[i & 1]) = 1;
+      if (((zero[0] | zero[1]) | (zero[2] | zero[3])) & 0x7FFF7FFFu) {
+        if (zero_not_finite<T>(at0, v0, kStepRows, c, seg.kv - k0)) *reinterpret_cast<volatile int32_t*>(&sh->fix[i & 1]) = 1;
+      }
       fence_proxy_async_smem();
       mbar_arrive(&sh->v_ok);
     };
