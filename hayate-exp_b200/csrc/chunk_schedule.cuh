@@ -126,13 +126,20 @@ __device__ __forceinline__ void chunk_find_start(const ChunkParams& P, int c, in
   __syncthreads();
 }
 
-// The same for one full warp on its own (no barrier); the result on every lane.
-__device__ __forceinline__ ChunkStart chunk_find_start_warp(const ChunkParams& P, int c, int ctas) {
+// The same for one full warp on its own (no barrier); the result on every lane, with request
+// start.b in `r`.
+__device__ __forceinline__ ChunkStart chunk_find_start_warp(const ChunkParams& P, int c, int ctas, ChunkRequest& r) {
   const int lane = threadIdx.x & 31;
   wait_for_primary();
-  int64_t before_all = 0, total = 0;
+  int64_t before_all = 0, mine = 0;
   int why = 0;
-  for (int b0 = 0; b0 < P.a.batch; b0 += 32)
+  r = ChunkRequest{0, 0, 0, 0, 0, false};
+  if (lane < P.a.batch) {  // the first 32 requests are looked at once
+    r = chunk_request(P, lane, why);
+    mine = chunk_work(P, r);
+  }
+  int64_t total = mine;
+  for (int b0 = 32; b0 < P.a.batch; b0 += 32)
     if (b0 + lane < P.a.batch) total += chunk_work(P, chunk_request(P, b0 + lane, why));
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -148,7 +155,13 @@ __device__ __forceinline__ ChunkStart chunk_find_start_warp(const ChunkParams& P
   start.b = 0;
   const int64_t begin = start.begin(c);
   for (int b0 = 0; b0 < P.a.batch && begin < total; b0 += 32) {  // the request that holds `begin`
-    const int64_t mine = b0 + lane < P.a.batch ? chunk_work(P, chunk_request(P, b0 + lane, why)) : 0;
+    if (b0 > 0) {
+      mine = 0;
+      if (b0 + lane < P.a.batch) {
+        r = chunk_request(P, b0 + lane, why);
+        mine = chunk_work(P, r);
+      }
+    }
     int64_t scan = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -161,6 +174,12 @@ __device__ __forceinline__ ChunkStart chunk_find_start_warp(const ChunkParams& P
       const int from = __ffs(holds) - 1;
       start.b = b0 + from;
       start.off = begin - __shfl_sync(0xffffffffu, before, from);
+      r.len = __shfl_sync(0xffffffffu, r.len, from);
+      r.queries = __shfl_sync(0xffffffffu, r.queries, from);
+      r.start = __shfl_sync(0xffffffffu, r.start, from);
+      r.row_blocks = __shfl_sync(0xffffffffu, r.row_blocks, from);
+      r.tiles = __shfl_sync(0xffffffffu, r.tiles, from);
+      r.refused = __shfl_sync(0xffffffffu, r.refused ? 1 : 0, from) != 0;
       break;
     }
     before_all += __shfl_sync(0xffffffffu, scan, 31);
@@ -192,6 +211,15 @@ struct ChunkWalk {
     started = false;
     work = 0;
     if (left > 0) load(P);
+  }
+  // with request s.b at hand
+  __device__ __forceinline__ ChunkWalk(const ChunkParams& P, const ChunkStart& s, int c, const ChunkRequest& first) {
+    left = s.begin(c + 1) - s.begin(c);
+    off = s.off;
+    b = s.b;
+    started = false;
+    r = first;
+    work = chunk_work(P, r);
   }
   __device__ __forceinline__ void load(const ChunkParams& P) {
     int why = 0;

@@ -57,7 +57,9 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
-constexpr int kUnitCost = 6;  // measured: 0, 2, 3, 4 and 6 tiles take 238, 225, 213, 210 and 206 us on 64 requests x 16 nodes
+// measured on 64 requests x 16 nodes, 8 x 256 nodes and 32 requests over chosen pages: 3 tiles take 205, 127 and
+// 133 us, 4 take 206, 127 and 132, 6 take 208, 128 and 131; one user (8 units of 8 tiles) 13.7, 13.6 and 14.2
+constexpr int kUnitCost = 4;
 
 struct Shared {
   uint64_t q_full, q_empty;
@@ -252,12 +254,13 @@ __global__ void __maxnreg__(96)
     fence_proxy_async_smem();
   }
   ChunkStart start;  // of the producer warp alone: the others follow its segments
+  ChunkRequest first_request;
   if (warp == kProducerWarp) {
     if (lane == 0) {
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
     }
-    start = chunk_find_start_warp(P, blockIdx.x, P.ctas);
+    start = chunk_find_start_warp(P, blockIdx.x, P.ctas, first_request);
   } else {
     wait_for_primary();
   }
@@ -282,7 +285,7 @@ __global__ void __maxnreg__(96)
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      ChunkWalk walk(P, start, blockIdx.x);
+      ChunkWalk walk(P, start, blockIdx.x, first_request);
       // an earlier CTA's wait gave up: load nothing, every tile counts as refused
       const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
       const int page_mask = (1 << p.page_shift) - 1;
@@ -298,8 +301,10 @@ __global__ void __maxnreg__(96)
         const bool any = walk.next(P, seg);
         sh->seg[i % kSegments] = seg;
         mbar_arrive(&sh->seg_full[i % kSegments]);
-        if (i == 0) chunk_write_join(P, start, blockIdx.x, any ? &seg : nullptr);
-        if (!any) break;
+        if (!any) {
+          if (i == 0) chunk_write_join(P, start, blockIdx.x, nullptr);
+          break;
+        }
         const int32_t* table = chunk_table(P, seg.b, seg.g);
         const int plane = p.layer * p.num_kv_heads + seg.g;
         for (int tile = seg.k_lo; tile < seg.k_hi; ++tile, ++n) {
@@ -329,6 +334,7 @@ __global__ void __maxnreg__(96)
           } else {
             mbar_arrive(&sh->v_full[vs]);
           }
+          if (n == 0) chunk_write_join(P, start, blockIdx.x, &seg);  // beside the first loads
         }
       }
       // nothing in flight when the CTA exits
