@@ -4,7 +4,7 @@
 // that get their own copy of the page being written, and copy-on-write. A page of a plane is
 // one contiguous block (32 KB at 128 tokens x 128 bf16), so the copy is a plain stream:
 // 16-byte loads, kUnroll in flight per thread, then the stores. Bound: HBM, one read and one
-// write of every byte.
+// write of every byte: 64 pages x 36 layers x 8 heads (2.42 GB) take 384 us, 6.3 TB/s.
 //
 // compact_rows: request b's row base[b] + src[i] -> base[b] + i, src strictly increasing (so
 // src[i] >= i): the accepted path of a drafted tree moves up behind the context, in place.
@@ -13,7 +13,8 @@
 // loads before their stores: row i + kRowsAhead is read after rows < i + kRowsAhead were written,
 // and src[i + kRowsAhead] >= i + kRowsAhead, so nothing is read after it was overwritten, and no
 // two threads touch the same bytes. Bound: HBM, 256-byte pieces (a row of one head), one read
-// and one write of each.
+// and one write of each: 64 paths of 6 to 12 rows x 36 layers x 8 heads (171 MB) take 32 us, 5.3
+// TB/s (offsets looked up by every thread for itself: 39 us).
 #include "chunk_schedule.cuh"
 
 namespace hyt {

@@ -5,8 +5,9 @@
 // page and brings their blocks into a ring of kBoundsStages stages with bulk copies, so that
 // the next blocks are on their way while one is looked through (16-bit types as packed pairs:
 // half the instructions of widening them); lanes of one column meet by shuffles, warps in
-// shared memory. One block per CTA without the ring took 61 us on 256 pages x 8 heads x 4
-// layers, whose keys need 42. NaN keys give NaN bounds. Bound: HBM reads of the keys.
+// shared memory. NaN keys give NaN bounds. Bound: HBM reads of the keys, and the barriers between
+// blocks: 256 pages x 8 heads x 4 layers (273 MB) take 54 us, 5.0 TB/s; one block per CTA without
+// the ring took 61.
 //
 // select_pages: score(page) = max over the KV group's query heads of
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
@@ -21,9 +22,10 @@
 // pages whose place is in doubt are summed that way: all are scored first on the tensor
 // cores (the dot product of [q > 0, q < 0] with [max, min], 8 pages and 8 heads per mma, each
 // bound read once), with the sum of the terms' magnitudes beside it, which bounds the error;
-// pages further than that from the threshold are in or out for certain. Exact sums of every
-// page took 62 us on 64 requests x 256 pages x 8 KV heads x 4 heads, conversions to 64 bits
-// 80; the bounds' bytes need 10.
+// pages further than that from the threshold are in or out for certain. 64 requests x 256 pages
+// x 8 KV heads x 4 heads take 34 us; exact sums of every page took 62, conversions to 64 bits
+// 80; the bounds' bytes need 10. Bound: the latency of a CTA's passes (scores, search, lists).
+// A product outside the range of fp32 makes its page's score infinite or NaN.
 //
 // Bound: HBM reads of the bounds on large batches, the chain of barriers on small ones.
 #include <cooperative_groups.h>

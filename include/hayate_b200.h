@@ -430,7 +430,8 @@ int hyt_page_bounds(const void* k_pool, void* k_bounds, int32_t num_layers, int3
  * already in place) attends, per KV head, the page being written and the num_pages - 1 full
  * pages with the largest score, or all pages if there are no more than num_pages:
  *   score = max over the KV head's query heads of sum_d q_d * (q_d >= 0 ? max_d : min_d)
- * summed in 64 bits and rounded once to fp32; ties go to the lower page, NaN ranks first.
+ * the exact sum rounded once to fp32 (products within the range of fp32); ties go to the lower
+ * page, NaN ranks first.
  * The logical pages read are written to selected [batch, num_kv_heads, num_pages],
  * ascending, -1 past the last. q/out strides = {b, h}. k_bounds must hold hyt_page_bounds of
  * every full page. Limits as for hyt_tree_attention, and at most 8192 pages per request.

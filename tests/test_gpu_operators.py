@@ -236,6 +236,40 @@ def test_tree_attention_strides_and_alignment(dtype):
     assert torch.equal(ops.tree_attention(*args), expect)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("hq, hkv, dim", [(4, 4, 128), (8, 4, 64), (8, 1, 128), (16, 1, 96), (64, 2, 128), (6, 2, 128),
+                                          (64, 1, 72)], ids=str)
+def test_tree_attention_rows_of_q_in_any_layout(dtype, hq, hkv, dim):
+    """q whose heads or tokens are next to each other, with room between rows, or off 16-byte
+    boundaries; NaN in the rows that no request owns, beside those that one does."""
+    tree = Tree([300, 0, 129], [5, 1, 70], dtype, seed=3, hq=hq, hkv=hkv, dim=dim, gap=3)
+    owned = np.zeros(tree.q.shape[2], dtype=bool)
+    for s, c in zip(tree.starts, tree.counts):
+        owned[s:s + c] = True
+    tree.q[0, :, torch.from_numpy(~owned).cuda()] = math.nan
+    base, n = tree.q, tree.q.shape[2]
+    expect = tree.run()
+    tree.check(expect)
+    rows = torch.from_numpy(owned).cuda()
+    layouts = [torch.empty(1, hq, n, dim, dtype=dtype, device="cuda"),                             # heads apart
+               torch.empty(1, n, hq, dim + 8, dtype=dtype, device="cuda").transpose(1, 2)[..., :dim],
+               torch.empty(1, n, hq, dim + 1, dtype=dtype, device="cuda").transpose(1, 2)[..., 1:],
+               torch.empty(1, n, 2 * hq, dim, dtype=dtype, device="cuda").transpose(1, 2)[:, hq:]]
+    for q in layouts:
+        q.copy_(base)
+        tree.q = q
+        assert torch.equal(tree.run()[:, :, rows], expect[:, :, rows])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_tree_attention_many_requests(dtype):
+    """More requests than a warp has lanes, of lengths far apart, some without nodes."""
+    rng = np.random.RandomState(4)
+    lens = (rng.randint(0, 300, 101) * rng.choice([0, 1, 9], 101)).tolist()
+    counts = (rng.randint(1, 6, 101) * rng.choice([0, 1, 1], 101)).tolist()
+    Tree(lens, counts, dtype, seed=5, hq=4, hkv=2, dim=64).check()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_tree_attention_bad_metadata_is_flagged_and_contained(dtype):
     t = Tree([300, 200, 50], [6, 5, 4], dtype)
