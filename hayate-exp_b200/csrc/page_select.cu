@@ -20,11 +20,13 @@
 // are exact in fp32, fp32 ones keep their rounding error by an FMA; the sums carry their
 // rounding errors along, Knuth's two-sum; lanes meet in 64 bits). For 16-bit types only the
 // pages whose place is in doubt are summed that way: all are scored first on the tensor
-// cores (the dot product of [q > 0, q < 0] with [max, min], 8 pages and 8 heads per mma, each
+// cores (the dot product of [q > 0, q < 0] with [max, min], 8 pages and 4 heads per mma, each
 // bound read once), with the sum of the terms' magnitudes beside it, which bounds the error;
 // pages further than that from the threshold are in or out for certain. 64 requests x 256 pages
-// x 8 KV heads x 4 heads take 34 us; exact sums of every page took 62, conversions to 64 bits
-// 80; the bounds' bytes need 10. Bound: the latency of a CTA's passes (scores, search, lists).
+// x 8 KV heads x 4 heads take 25 us; with maxima and minima as operands of their own (four
+// mma instead of two per 16 dims) and a second search for the pages in doubt 34, exact sums of
+// every page 62, conversions to 64 bits 80; the bounds' bytes need 10. Bound: the latency of a
+// CTA's passes (scores 13 us, search and lists 7).
 // A product outside the range of fp32 makes its page's score infinite or NaN.
 //
 // Bound: HBM reads of the bounds on large batches, the chain of barriers on small ones.
@@ -281,8 +283,9 @@ __device__ __forceinline__ uint32_t exact_key(int head_dim, const T* qh, const T
 }
 
 // The tensor cores' fp32 accumulation of 16 products and the running sum may drop bits below
-// 2^-23 of the largest of them; 4 steps of 17 terms per 32 dims keep the error of a score
-// under 2^-20 of the sum of the terms' magnitudes per dim, with a factor of 3 to spare.
+// 2^-23 of the largest of them; 2 steps of 17 terms per 32 dims for the maxima and 2 for the
+// minima keep the error of a score under 2^-20 of the sum of the terms' magnitudes per dim,
+// with a factor of 3 to spare.
 __device__ __forceinline__ float score_slack(int head_dim, float magnitude) {
   return magnitude * float((head_dim + 31) / 32 * 32) * 9.5367432e-7f;
 }
@@ -354,9 +357,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
   int32_t* to_id = cluster.map_shared_rank(ids, 0);
   if constexpr (kTensor) {
     // 8 pages per warp and turn: lane (n = lane / 4, j = lane % 4) reads 16-byte chunks j + 4 t
-    // of page n's two rows; a chunk's words 0, 1 and 2, 3 are the B operands of two k = 16
-    // steps, and q's chunks, read the same way for head n, the A operands: the order of
-    // the dims differs from memory's, alike on both sides
+    // of page n's two rows. A operand: row n the maxima, row n + 8 the minima of page n; B
+    // operand: column n the positive (n < 4) or negative values of head n % 4 of four, read the
+    // same way: the order of the dims differs from memory's, alike on both sides. Of the
+    // product, maxima x positive and minima x negative make the scores
     const int n = lane >> 2, j = lane & 3, chunks = D / 8;
     const int first = (rank * kWarps + warp) * 8, stride = ranks * kWarps * 8;
     float magnitude = 0.f;
@@ -380,9 +384,36 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
       slot = slot + 1 == kRing ? 0 : slot + 1;
       return page;
     };
+    uint32_t qw[kSteps][4];
+    auto load_q = [&](int h0) {
+      const T* qh = q0 + int64_t(min(h0 + (n & 3), group - 1)) * p.q_sh;
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const int c = j + 4 * t;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (c < chunks) {
+          if (p.q_vec) {
+            v = __ldg(reinterpret_cast<const uint4*>(qh) + c);
+          } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(qh + c * 8);
+            v.x = e[0] | (uint32_t(e[1]) << 16);
+            v.y = e[2] | (uint32_t(e[3]) << 16);
+            v.z = e[4] | (uint32_t(e[5]) << 16);
+            v.w = e[6] | (uint32_t(e[7]) << 16);
+          }
+        }
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t negative = ((w[k] & 0x80008000u) >> 15) * 0xFFFFu;  // ones where q < 0
+          qw[t][k] = w[k] & (n < 4 ? ~negative : negative);
+        }
+      }
+    };
     int ids_ahead[kRing];  // pages of this lane's n in the turns to come
 #pragma unroll
     for (int k = 0; k < kRing - 1; ++k) ids_ahead[k] = fetch();
+    if (group <= 4) load_q(0);
     int at = 0;
     for (int i0 = first; i0 < last; i0 += stride) {
       const int page = ids_ahead[0];
@@ -392,74 +423,41 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
       cp_async_wait<kRing - 1>();
       const uint4* here = &ring[at * 2 * kSteps * kSelectThreads];
       at = at + 1 == kRing ? 0 : at + 1;
-      float top[2] = {-INFINITY, -INFINITY};  // best over the heads, pages 2 j and 2 j + 1
-      bool nan[2] = {false, false};
-      for (int h0 = 0; h0 < group; h0 += 8) {
+      float top = -INFINITY;  // best over the heads (lanes j = 0, 1)
+      bool nan = false;
+      for (int h0 = 0; h0 < group; h0 += 4) {
+        if (group > 4) load_q(h0);
         float s[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
-        const T* qh = q0 + int64_t(min(h0 + n, group - 1)) * p.q_sh;
-        uint4 q4[kSteps];
-#pragma unroll
-        for (int t = 0; t < kSteps; ++t) {
-          const int c = j + 4 * t;
-          q4[t] = make_uint4(0u, 0u, 0u, 0u);
-          if (c >= chunks) continue;
-          if (p.q_vec) {
-            q4[t] = __ldg(reinterpret_cast<const uint4*>(qh) + c);
-          } else {
-            const uint16_t* e = reinterpret_cast<const uint16_t*>(qh + c * 8);
-            q4[t].x = e[0] | (uint32_t(e[1]) << 16);
-            q4[t].y = e[2] | (uint32_t(e[3]) << 16);
-            q4[t].z = e[4] | (uint32_t(e[5]) << 16);
-            q4[t].w = e[6] | (uint32_t(e[7]) << 16);
-          }
-        }
 #pragma unroll
         for (int t = 0; t < kSteps; ++t) {
           const uint4 l4 = here[2 * t * kSelectThreads], h4 = here[(2 * t + 1) * kSelectThreads];
           const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
-          const uint32_t qw[4] = {q4[t].x, q4[t].y, q4[t].z, q4[t].w};
           constexpr uint32_t kAbs = 0x7FFF7FFFu;
 #pragma unroll
           for (int w = 0; w < 4; w += 2) {
-            uint32_t plus[4] = {0u, 0u, 0u, 0u}, minus[4] = {0u, 0u, 0u, 0u};  // rows 8 .. 15 unused
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t sign = qw[w + k] & 0x80008000u, mask = (sign >> 15) * 0xFFFFu;  // ones where q < 0
-              plus[2 * k] = qw[w + k] & ~mask;
-              minus[2 * k] = qw[w + k] & mask;
-            }
-            mma_16816<kHalf>(s, plus, hw[w], hw[w + 1]);
-            mma_16816<kHalf>(s, minus, lw[w], lw[w + 1]);
-            mma_16816<kHalf>(m, plus, hw[w] & kAbs, hw[w + 1] & kAbs);
-            const uint32_t minus_abs[4] = {minus[0] & kAbs, 0u, minus[2] & kAbs, 0u};
-            mma_16816<kHalf>(m, minus_abs, lw[w] & kAbs, lw[w + 1] & kAbs);
+            const uint32_t x[4] = {hw[w], lw[w], hw[w + 1], lw[w + 1]};
+            const uint32_t x_abs[4] = {x[0] & kAbs, x[1] & kAbs, x[2] & kAbs, x[3] & kAbs};
+            mma_16816<kHalf>(s, x, qw[t][w], qw[t][w + 1]);
+            mma_16816<kHalf>(m, x_abs, qw[t][w] & kAbs, qw[t][w + 1] & kAbs);
           }
         }
-        if (h0 + n < group) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            nan[e] |= isnan(s[e]);
-            top[e] = fmaxf(top[e], s[e]);
-            if (i0 + 2 * j + e < last) magnitude = max_nan(magnitude, m[e]);
-          }
-        }
-      }
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {  // over the heads
+        // lanes j = 0, 1: maxima x heads h0 + 2 j, + 1; j = 2, 3: minima x the same heads
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], off));
-          nan[e] |= __shfl_xor_sync(0xffffffffu, nan[e] ? 1 : 0, off) != 0;
+          const float score = s[e] + __shfl_xor_sync(0xffffffffu, s[2 + e], 2);
+          const float size = m[e] + __shfl_xor_sync(0xffffffffu, m[2 + e], 2);
+          if (j < 2 && h0 + 2 * j + e < group) {
+            nan |= isnan(score);
+            top = fmaxf(top, score);
+            if (i0 + n < last) magnitude = max_nan(magnitude, size);
+          }
         }
       }
-      const int even = __shfl_sync(0xffffffffu, page, 8 * j), odd = __shfl_sync(0xffffffffu, page, 8 * j + 4);
-      if (n < 2) {
-        const int i = i0 + 2 * j + n, id = n == 0 ? even : odd;
-        const uint32_t key = (n == 0 ? nan[0] : nan[1]) ? 0xFFFFFFFFu : score_key(n == 0 ? top[0] : top[1]);
-        if (i < last) {
-          to[i] = id < 0 ? 0u : key;
-          to_id[i] = id;
-        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      nan |= __shfl_xor_sync(0xffffffffu, nan ? 1 : 0, 1) != 0;
+      if (j == 0 && i0 + n < last) {
+        to[i0 + n] = page < 0 ? 0u : (nan ? 0xFFFFFFFFu : score_key(top));
+        to_id[i0 + n] = page;
       }
     }
     cp_async_wait<0>();
@@ -598,6 +596,24 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
       if (lane % kLanes == 0) atomicMax(&keys[i], key);
     }
     __syncthreads();
+    // a few in doubt: a warp ranks them (a search over all keys takes 9,000 cycles). Those for which
+    // there is room are in
+    if (known && !settled && s_doubtful <= 32) {
+      if (warp == 0) {
+        const int left = s_doubtful, i = lane < left ? doubtful[lane] : last;
+        const uint32_t key = lane < left ? keys[i] : 0u;
+        int better = 0;
+        for (int o = 0; o < left; ++o) {
+          const uint32_t other = __shfl_sync(0xffffffffu, key, o);
+          const int other_i = __shfl_sync(0xffffffffu, i, o);
+          better += other > key || (other == key && other_i < i) ? 1 : 0;
+        }
+        __syncwarp();
+        if (lane < left) keys[i] = better < want - all[1] ? 0xFFFFFFFFu : 0u;
+      }
+      settled = true;
+      __syncthreads();
+    }
   }
   uint32_t threshold = 0xFFFFFFFFu;  // keys above it are in, and the first `need` of those equal to it
   int need = 0;
