@@ -1,13 +1,13 @@
 // Page bounds, and the choice of pages a one-token decode reads.
 //
 // page_bounds: elementwise minimum and maximum of a full page's keys, per layer and KV head.
-// A page of one head is contiguous (32 KB at 128 x 128 x 16 bits): a CTA walks some heads of a
-// page and brings their blocks into a ring of kBoundsStages stages with bulk copies, so that
-// the next blocks are on their way while one is looked through (16-bit types as packed pairs:
-// half the instructions of widening them); lanes of one column meet by shuffles, warps in
-// shared memory. NaN keys give NaN bounds. Bound: HBM reads of the keys, and the barriers between
-// blocks: 256 pages x 8 heads x 4 layers (273 MB) take 54 us, 5.0 TB/s; one block per CTA without
-// the ring took 61.
+// A page of one head is contiguous (32 KB at 128 x 128 x 16 bits). As many CTAs as the SMs hold
+// walk an equal share of the (layer, page, head) list each, through a ring of kBoundsStages
+// stages that bulk copies fill, so that the next blocks are on their way while one is looked
+// through (16-bit types as packed pairs: half the instructions of widening them); lanes of one
+// column meet by shuffles, warps in shared memory. NaN keys give NaN bounds. Bound: HBM reads
+// of the keys: 256 pages x 8 heads x 4 layers (273 MB) take 49.5 us, 5.5 TB/s; a CTA per page
+// (its start and the last wave) took 54, a CTA per block without the ring 61.
 //
 // select_pages: score(page) = max over the KV group's query heads of
 //   sum_d q_d * (q_d >= 0 ? max_d : min_d),
@@ -113,44 +113,73 @@ struct MinMax<__half> {
 constexpr int kBoundsStages = 3;
 constexpr int kBoundsBlock = 32 * 1024;  // most bytes of a stage
 
-// Grid: (groups of heads_per_cta KV heads, page entry, layer).
+// A place in the list of blocks: a part (stage_rows rows) of a head of a page entry of a layer.
+struct BoundsCursor {
+  int part, head, entry, layer;
+  __device__ __forceinline__ BoundsCursor(const BoundsParams& p, int64_t item) {
+    part = 0;
+    head = int(item % p.num_kv_heads);
+    const int64_t rest = item / p.num_kv_heads;
+    entry = int(rest % p.count);
+    layer = int(rest / p.count);
+  }
+  __device__ __forceinline__ void next(const BoundsParams& p, int parts) {
+    if (++part < parts) return;
+    part = 0;
+    if (++head < p.num_kv_heads) return;
+    head = 0;
+    if (++entry < p.count) return;
+    entry = 0;
+    ++layer;
+  }
+};
+
+// CTA c of G takes items (layer, page entry, KV head) [c, c + 1) * items / G.
 template <typename T>
-__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsParams p, int heads_per_cta, int stage_rows) {
+__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsParams p, int64_t items, int stage_rows) {
   constexpr int kPer = 16 / int(sizeof(T));
   constexpr int kWarps = kBoundsThreads / 32;
   extern __shared__ __align__(128) uint8_t ring[];  // [kBoundsStages][stage_rows * D], then per warp and column
   __shared__ uint64_t full[kBoundsStages];
+  __shared__ int32_t page_s[kBoundsStages];  // page of the stage's block, -1: skipped
   __shared__ int abort_s;
-  const int32_t page = p.pages[blockIdx.y];
-  if (page == -1) return;
-  if (page < 0 || page >= p.num_pages) {
-    if (threadIdx.x == 0) flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
-    return;
-  }
   const int D = p.head_dim, chunks = D / kPer;  // 16-byte columns of a row (<= 64)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = 1 << p.page_shift, parts = (rows + stage_rows - 1) / stage_rows;
-  const int head0 = int(blockIdx.x) * heads_per_cta, heads = min(heads_per_cta, p.num_kv_heads - head0);
-  const int items = heads * parts, stage_bytes = stage_rows * D * int(sizeof(T));
-  uint4* lo_s = reinterpret_cast<uint4*>(ring + kBoundsStages * stage_bytes);  // [kWarps][chunks]
-  uint4* hi_s = lo_s + kWarps * chunks;
-  const int64_t plane0 = int64_t(p.first_layer + blockIdx.z) * p.num_kv_heads + head0;
+  const int stage_bytes = stage_rows * D * int(sizeof(T));
+  const int64_t item0 = items * blockIdx.x / gridDim.x;
+  const int64_t blocks = (items * (blockIdx.x + 1) / gridDim.x - item0) * parts;
+  // [2][lo, hi][kWarps][chunks]: the warps' results of a head and of the one after
+  uint4* results = reinterpret_cast<uint4*>(ring + kBoundsStages * stage_bytes);
   if (tid == 0) {
     abort_s = 0;
     for (int s = 0; s < kBoundsStages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  auto load = [&](int item) {  // thread 0: block `item` into its stage
-    const int h = item / parts, part = item - h * parts, st = item % kBoundsStages;
-    const int here = min(stage_rows, rows - part * stage_rows);
-    const T* src = static_cast<const T*>(p.k_pool) +
-                   ((plane0 + h) * p.capacity + (int64_t(page) << p.page_shift) + part * stage_rows) * D;
-    mbar_arrive_expect_tx(&full[st], uint32_t(here * D * int(sizeof(T))));
-    bulk_load(ring + st * stage_bytes, src, uint32_t(here * D * int(sizeof(T))), &full[st]);
+  BoundsCursor ahead(p, item0), at = ahead;
+  auto load = [&](int st) {  // thread 0: the next block into stage st
+    int32_t page = p.pages[ahead.entry];
+    if (page < -1 || page >= p.num_pages) {
+      flag_error(p.error_word, HYT_DEVERR_PAGE_RANGE);
+      page = -1;
+    }
+    page_s[st] = page;
+    if (page >= 0) {
+      const uint32_t bytes = uint32_t(min(stage_rows, rows - ahead.part * stage_rows) * D * int(sizeof(T)));
+      const int64_t plane = int64_t(p.first_layer + ahead.layer) * p.num_kv_heads + ahead.head;
+      mbar_arrive_expect_tx(&full[st], bytes);
+      bulk_load(ring + st * stage_bytes,
+                static_cast<const T*>(p.k_pool) +
+                    (plane * p.capacity + (int64_t(page) << p.page_shift) + ahead.part * stage_rows) * D,
+                bytes, &full[st]);
+    } else {
+      mbar_arrive(&full[st]);
+    }
+    ahead.next(p, parts);
   };
   if (tid == 0)
-    for (int i = 0; i < min(items, kBoundsStages); ++i) load(i);
+    for (int i = 0; i < kBoundsStages && i < blocks; ++i) load(i);
   __syncthreads();
 
   // columns that divide a warp's lanes: 32 / chunks rows side by side per warp; else a warp takes
@@ -161,15 +190,17 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
   const int columns = side_by_side ? 1 : (chunks + 31) / 32;  // at most 2
   uint4 lo[2], hi[2];
   bool any = false;
-  for (int item = 0; item < items; ++item) {
-    const int st = item % kBoundsStages, part = item % parts;
-    const int here = min(stage_rows, rows - part * stage_rows);
-    if (part == 0) any = false;
-    mbar_wait(&full[st], (item / kBoundsStages) & 1, p.error_word, &abort_s);
+  int st = 0, which = 0;
+  uint32_t phase = 0u;
+  for (int64_t i = 0; i < blocks; ++i, at.next(p, parts)) {
+    const int here = min(stage_rows, rows - at.part * stage_rows);
+    if (at.part == 0) any = false;
+    mbar_wait(&full[st], phase, p.error_word, &abort_s);
+    const int32_t page = page_s[st];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int c = side_by_side ? lane % chunks : lane + 32 * k;
-      if (k >= columns || c >= chunks) continue;
+      if (k >= columns || c >= chunks || page < 0) continue;
       const uint4* column = reinterpret_cast<const uint4*>(ring + st * stage_bytes) + c;
       bool begun = any;
 #pragma unroll 4
@@ -184,11 +215,12 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
       }
     }
     any = any || first < here;
-    __syncthreads();  // the stage has been read (and the previous head's columns)
-    if (tid == 0 && item + kBoundsStages < items) load(item + kBoundsStages);
-    if (part != parts - 1) continue;
+    const bool ends = at.part == parts - 1 && page >= 0;
+    uint4* lo_s = results + which * 2 * kWarps * chunks;
+    uint4* hi_s = lo_s + kWarps * chunks;
     bool mine = any;
-    if (side_by_side) {  // rows that exist come first: a lane without one takes its partner's
+    if (!ends) {
+    } else if (side_by_side) {  // rows that exist come first: a lane without one takes its partner's
       for (int off = chunks; off < 32; off <<= 1) {
         const uint4 a = make_uint4(__shfl_xor_sync(0xffffffffu, lo[0].x, off), __shfl_xor_sync(0xffffffffu, lo[0].y, off),
                                    __shfl_xor_sync(0xffffffffu, lo[0].z, off), __shfl_xor_sync(0xffffffffu, lo[0].w, off));
@@ -209,11 +241,17 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
       for (int k = 0; k < 2; ++k)
         if (lane + 32 * k < chunks) lo_s[warp * chunks + lane + 32 * k] = lo[k], hi_s[warp * chunks + lane + 32 * k] = hi[k];
     }
+    // the stage has been read and the head's results are there; those of the head before last,
+    // whose place the next head's take, went out before this barrier
     __syncthreads();
+    if (tid == 0 && i + kBoundsStages < blocks) load(st);
+    if (++st == kBoundsStages) st = 0, phase ^= 1u;
+    if (!ends) continue;
+    which ^= 1;
     const int used = min(kWarps, (rows + per_warp - 1) / per_warp);  // warps that had a row (of a full first part)
     const int words = chunks * 4;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.k_bounds) +
-                                                ((plane0 + item / parts) * p.num_pages + page) * 2 * D);
+                                                ((int64_t(p.first_layer + at.layer) * p.num_kv_heads + at.head) * p.num_pages + page) * 2 * D);
     for (int i = tid; i < 2 * words; i += kBoundsThreads) {
       const bool is_hi = i >= words;
       const int w = is_hi ? i - words : i;
@@ -225,7 +263,8 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
   }
   // every block was waited for above; if a wait gave up, see that no copy is in flight at the exit
   if (tid == 0 && abort_s)
-    for (int i = max(0, items - kBoundsStages); i < items; ++i) mbar_drain(&full[i % kBoundsStages], (i / kBoundsStages) & 1);
+    for (int64_t i = blocks > kBoundsStages ? blocks - kBoundsStages : 0; i < blocks; ++i)
+      mbar_drain(&full[i % kBoundsStages], uint32_t(i / kBoundsStages) & 1u);
 }
 
 // Order-preserving unsigned key of a score; NaN ranks above everything.
@@ -679,16 +718,17 @@ __global__ void __launch_bounds__(kSelectThreads) select_pages_kernel(const Sele
 cudaError_t run_page_bounds(const BoundsParams& p, int dtype, cudaStream_t stream) {
   if (p.count == 0 || p.layers == 0) return cudaSuccess;
   const int row_bytes = p.head_dim * (dtype == HYT_DTYPE_F32 ? 4 : 2), rows = 1 << p.page_shift;
-  const int stage_rows = rows * int64_t(row_bytes) <= kBoundsBlock ? rows : kBoundsBlock / row_bytes;
-  // several blocks per CTA once every SM has six
-  const int64_t blocks = int64_t(p.num_kv_heads) * p.count * p.layers;
-  const int heads = int(std::min<int64_t>(p.num_kv_heads, std::max<int64_t>(1, blocks / (148 * 6))));
-  const dim3 grid(unsigned((p.num_kv_heads + heads - 1) / heads), unsigned(p.count), unsigned(p.layers));
-  const int smem = kBoundsStages * stage_rows * row_bytes + 2 * (kBoundsThreads / 32) * row_bytes;
+  const int block = row_bytes >= 512 ? kBoundsBlock * 3 / 4 : kBoundsBlock;  // so that an SM holds two CTAs
+  const int stage_rows = rows * int64_t(row_bytes) <= block ? rows : block / row_bytes;
+  const int smem = kBoundsStages * stage_rows * row_bytes + 4 * (kBoundsThreads / 32) * row_bytes;
+  // as many CTAs as fit the SMs at once, an equal share of the items each
+  const int64_t items = int64_t(p.num_kv_heads) * p.count * p.layers;
+  const int64_t slots = 148 * std::min<int64_t>(8, (220 << 10) / (smem + 1024));
+  const unsigned grid = unsigned(std::min(items, slots));
   auto launch = [&](auto kernel) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kBoundsThreads, smem, stream>>>(p, heads, stage_rows);
+    kernel<<<grid, kBoundsThreads, smem, stream>>>(p, items, stage_rows);
     return cudaGetLastError();
   };
   switch (dtype) {
