@@ -149,7 +149,7 @@ _int64_arrays: dict = {}
 def int64_array(values) -> ctypes.Array:
     """A ctypes int64 array of ``values`` (the C side only reads it: equal tuples share one,
     so per-call stride arrays cost a dictionary lookup)."""
-    key = tuple(int(v) for v in values)
+    key = values if type(values) is tuple else tuple(int(v) for v in values)
     arr = _int64_arrays.get(key)
     if arr is None:
         if len(_int64_arrays) > 4096:
