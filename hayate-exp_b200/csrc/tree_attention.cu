@@ -39,7 +39,7 @@
 // 128, take 207 us for 1.23 GB with the merge (5.9 TB/s). Above, by the chain of a stream's
 // softmax and its 16 MMAs, 3,250 to 3,400 cycles per 256 x 128 tile of which the MMAs are 2,048:
 // 4 x 33..64 nodes over 32K tokens 142 us (0.70 PFLOP/s of visible pairs), 8 x 256 nodes over 2K to
-// 4K 127 us (0.78). Two row blocks per unit instead of one: a K/V tile is read half as often (the
+// 4K 125 us (0.79). Two row blocks per unit instead of one: a K/V tile is read half as often (the
 // first kernel, with one, took 199 us on the latter). A unit's ends cost about 4 tiles: the first
 // tile runs on cold instructions, and O goes out as 128 KB of partials.
 #include <type_traits>
@@ -153,6 +153,25 @@ __device__ __noinline__ void store_unaligned16(void* at, uint4 w) {
   uint16_t* e = static_cast<uint16_t*>(at);
   e[0] = uint16_t(w.x), e[1] = uint16_t(w.x >> 16), e[2] = uint16_t(w.y), e[3] = uint16_t(w.y >> 16);
   e[4] = uint16_t(w.z), e[5] = uint16_t(w.z >> 16), e[6] = uint16_t(w.w), e[7] = uint16_t(w.w >> 16);
+}
+
+// One half of a 4 x 4 exchange of pieces: lanes that differ in bit kBit swap w[v] (v with the bit) of
+// the lane without it for w[v - kBit] of the lane with it.
+template <int kBit>
+__device__ __forceinline__ void swap_pieces(uint4 (&w)[4], int lane) {
+  const bool upper = (lane & kBit) != 0;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    if (!(v & kBit)) continue;
+    uint32_t* lo = reinterpret_cast<uint32_t*>(&w[v - kBit]);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(&w[v]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo[e] : hi[e], kBit);
+      if (upper) lo[e] = got;
+      else hi[e] = got;
+    }
+  }
 }
 
 // acc + 0 * x for a pair of values: +-0 where both are finite so far
@@ -762,32 +781,52 @@ __global__ void __maxnreg__(96)
                 if (use1) f[e] = fmaf(__uint_as_float(o[e]), f1, f[e]);
             }
           }
-          if (mine) {
-          if (seg.whole) {
+          if (kDual && seg.whole && kp.o_vec) {
+            // four lanes exchange 16-byte pieces of their rows, so that a store writes 64 bytes in a
+            // row of 8 rows each, not 16 of 32 (8 x 256 nodes: 126.5 -> 124 us; with one row block,
+            // of which often few rows exist, 64 x 16 nodes 202 -> 203, so those store directly)
+            uint4 w[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              if (col + v * 8 >= D) break;
-              uint4 w;
-              w.x = Elem<T>::pack2(f[8 * v + 0] * inv, f[8 * v + 1] * inv);
-              w.y = Elem<T>::pack2(f[8 * v + 2] * inv, f[8 * v + 3] * inv);
-              w.z = Elem<T>::pack2(f[8 * v + 4] * inv, f[8 * v + 5] * inv);
-              w.w = Elem<T>::pack2(f[8 * v + 6] * inv, f[8 * v + 7] * inv);
-              if (kp.o_vec) *reinterpret_cast<uint4*>(out + col + v * 8) = w;
-              else store_unaligned16(out + col + v * 8, w);
+            for (int v = 0; v < 4; ++v)
+              w[v] = make_uint4(Elem<T>::pack2(f[8 * v] * inv, f[8 * v + 1] * inv),
+                                Elem<T>::pack2(f[8 * v + 2] * inv, f[8 * v + 3] * inv),
+                                Elem<T>::pack2(f[8 * v + 4] * inv, f[8 * v + 5] * inv),
+                                Elem<T>::pack2(f[8 * v + 6] * inv, f[8 * v + 7] * inv));
+            swap_pieces<2>(w, lane);
+            swap_pieces<1>(w, lane);  // w[k]: piece lane % 4 of row k of the four
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int owner = (lane & ~3) | k;
+              T* row = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), owner));
+              const int at = col + (lane & 3) * 8;
+              if (quarter * 32 + owner < my_rows && at < D) *reinterpret_cast<uint4*>(row + at) = w[k];
             }
-          } else {
-            float4* wo = chunk_partial_o(P, slot);
+            __syncwarp();  // before values that are not finite are added
+          } else if (mine) {
+            if (seg.whole) {
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-              if (col + v * 4 < D)
-                wo[int64_t(col / 4 + v) * P.unit_rows + unit_row] =
-                    make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
-            if (col == 0) chunk_partial_ml(P, slot)[unit_row] = make_float2(m, l);
+              for (int v = 0; v < 4; ++v) {
+                if (col + v * 8 >= D) break;
+                const uint4 w = make_uint4(Elem<T>::pack2(f[8 * v] * inv, f[8 * v + 1] * inv),
+                                           Elem<T>::pack2(f[8 * v + 2] * inv, f[8 * v + 3] * inv),
+                                           Elem<T>::pack2(f[8 * v + 4] * inv, f[8 * v + 5] * inv),
+                                           Elem<T>::pack2(f[8 * v + 6] * inv, f[8 * v + 7] * inv));
+                if (!kDual && kp.o_vec) *reinterpret_cast<uint4*>(out + col + v * 8) = w;
+                else store_unaligned16(out + col + v * 8, w);
+              }
+            } else {
+              float4* wo = chunk_partial_o(P, slot);
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                if (col + v * 4 < D)
+                  wo[int64_t(col / 4 + v) * P.unit_rows + unit_row] =
+                      make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+              if (col == 0) chunk_partial_ml(P, slot)[unit_row] = make_float2(m, l);
+            }
           }
-          if (fix)
+          if (fix && mine)
             add_not_finite<T>(P, seg, t, col, min(32, D - col), out + col,
                               reinterpret_cast<float*>(chunk_partial_o(P, slot)) + unit_row * 4);
-          }
           __syncwarp();
         }
       }

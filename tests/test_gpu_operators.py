@@ -261,6 +261,29 @@ def test_tree_attention_rows_of_q_in_any_layout(dtype, hq, hkv, dim):
         assert torch.equal(tree.run()[:, :, rows], expect[:, :, rows])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("dim", [64, 72, 96, 128])
+@pytest.mark.parametrize("bad", [math.nan, -math.inf], ids=str)
+def test_wide_trees_with_a_node_that_is_not_finite(dtype, dim, bad):
+    """Units of more rows than an MMA holds, some whole, some cut: rows that do not see the node
+    are those of a clean run, bit for bit, and right; rows that see it are not finite."""
+    make = dict(lens=[100, 127, 40, 700] * 12, counts=[70, 90, 65, 130] * 12, dtype=dtype, seed=6, hq=16, hkv=4, dim=dim)
+    clean, dirty = Tree(**make), Tree(**make)
+    expect = clean.run()
+    clean.check(expect)
+    for b, n in enumerate(dirty.lens):
+        pos = n + 5
+        slot = int(dirty.table[b][pos // 128]) * 128 + pos % 128
+        dirty.k[:, :, :, slot] = bad
+        dirty.v[:, :, :, slot] = bad
+    out = dirty.run()
+    for s, c, sees in zip(dirty.starts, dirty.counts, dirty.sees):
+        hit = torch.from_numpy(np.ascontiguousarray(sees[:, 5])).cuda()
+        got, ref = out[0, :, s:s + c], expect[0, :, s:s + c]
+        assert torch.equal(got[:, ~hit], ref[:, ~hit])
+        assert not torch.isfinite(got[:, hit].float()).any()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_tree_attention_many_requests(dtype):
     """More requests than a warp has lanes, of lengths far apart, some without nodes."""
