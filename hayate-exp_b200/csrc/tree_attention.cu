@@ -18,8 +18,10 @@
 // 640 threads: warps 0-7 softmax of stream 0, 8-15 of stream 1 (in a stream, warps w and
 // w + 4 own rows 32 (w % 4) .. and half of the 128 key columns each), warp 16 the TMA
 // producer, which also walks the CTA's segments and hands them to the others through a
-// shared ring, warp 17 the MMA issuer, warps 18-19 load the next segment's Q rows as soon
-// as the last S of the one before is done. Per tile, S = Q K^T (shared x shared), P goes back over
+// shared ring, warp 17 the MMA issuer, warps 18-19 look through V past the cached tokens and,
+// once the last S of a segment is done, bring the next one's Q: by TMA (boxes of 32 rows: a
+// group's heads x 32 / group tokens), or row by row where q's layout has no such map or the
+// group does not divide 32 (64 KB took 9,000 to 12,000 cycles that way, 1,000 by TMA). Per tile, S = Q K^T (shared x shared), P goes back over
 // S's columns as 16-bit pairs, O += P V (TMEM x shared). Issue order PV(s), QK(s + 2).
 // TMEM (512 columns): S_0/P_0 [0,128), S_1/P_1 [128,256), O_0 [256,384), O_1 [384,512).
 // Shared memory: Q 32 KB per row block, 2 K stages, 3 (one row block) or 2 V stages of 32 KB.
