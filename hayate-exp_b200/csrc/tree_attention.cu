@@ -66,6 +66,7 @@ constexpr int kKStages = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kUnseen = 2.0f;  // rescale factor, else at most 1, of a row that saw nothing yet (O and sum are 0)
 
 // measured on 64 requests x 16 nodes, 8 x 256 nodes and 64 requests over 16 chosen pages: 3 tiles take 205, 127
 // and 133 us, 4 take 206, 127 and 132, 6 take 208, 128 and 131; one user (8 units of 8 tiles) 13.7, 13.6 and 14.2
@@ -699,14 +700,15 @@ __global__ void __maxnreg__(96)
           const bool moves = __any_sync(0xffffffffu, m_new > m_run + kRescaleThreshold);
           float alpha = 1.f;
           if (moves) {
-            alpha = m_run == -INFINITY ? 0.f : ex2(m_run - m_new);
+            alpha = m_run == -INFINITY ? kUnseen : ex2(m_run - m_new);
             m_run = m_new;
           }
           const float tile_sum = exp_tile<T>(s, scale2, m_run == -INFINITY ? 0.f : m_run, p_addr);
-          const float l_before = l_run;
           l_run = l_run * alpha + tile_sum;
-          // O_x holds something (each row's, or zeros), and is stable: its last PV completed before S_x did
-          if (moves && __any_sync(0xffffffffu, l_before != 0.f)) {
+          // If a row saw a tile before, O_x holds products, and is stable: its last PV completed before
+          // S_x did. l_run cannot tell: it is the sum over this half's keys, O's dims hold both halves'
+          if (moves && __any_sync(0xffffffffu, alpha != kUnseen)) {
+            if (alpha == kUnseen) alpha = 0.f;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               uint32_t o[32];
