@@ -447,7 +447,14 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// 2^x on the FMA pipe, for x <= 64 (x below -126, -inf included, gives 0).
+// The same, NaN if a value is NaN.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x on the FMA pipe, for x <= 64 (x below -126, -inf included, gives 0; NaN gives 2^-126).
 // Cody-Waite split x = i + f, i = floor(x) taken from the mantissa of x + 1.5 * 2^23
 // rounded down, f in [0, 1); 2^f from a cubic fitted here to 2^f on [0, 1) in relative
 // error (iteratively reweighted least squares; max relative error 7.5e-5, far below the

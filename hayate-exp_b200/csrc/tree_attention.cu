@@ -32,7 +32,7 @@
 // looked through (by the Q warps, beside the softmax) before they are multiplied: values that
 // are not finite become zeros, and those of drafted nodes are added at the end to the rows
 // that see them (0 * inf would be NaN in every row). A tile whose page was refused is not
-// multiplied.
+// multiplied. A visible score that is NaN or +inf makes its row NaN.
 //
 // P is rounded to the storage type (the MMA's operand type); scores, running maximum and
 // sum, and O are fp32. The running maximum may lag by up to 2^8 (O / l is exact all the same).
@@ -106,9 +106,14 @@ __device__ __forceinline__ uint32_t sw128_offset(int r, int chunk) {
 }
 
 // P = 2^(s * scale_log2 - m) of 64 scores, written to TMEM as packed 16-bit pairs; returns
-// their sum. 7 of 8 exponentials on MUFU, 1 of 8 on the FMA pipe.
+// their sum. 7 of 8 exponentials on MUFU, 1 of 8 on the FMA pipe, where a NaN would get lost: a score
+// there that is NaN or +inf makes m, and with it the row, NaN (elsewhere s - m is NaN already).
 template <typename T>
 __device__ __forceinline__ float exp_tile(const float (&s)[64], uint64_t scale2, float m, uint32_t p_addr) {
+  float top = 0.f;
+#pragma unroll
+  for (int c = 7; c < 64; c += 16) top = fmax3_nan(top, s[c], s[c + 8]);
+  m = fmaf(top, 0.f, m);
   const uint64_t neg_m2 = f2_pack(-m, -m);
   uint64_t sum2a = f2_pack(0.f, 0.f), sum2b = sum2a;
 #pragma unroll
