@@ -81,8 +81,9 @@ def _prompt_chunk(engine, request):
     return request.prompt_tokens[cache_pos:end], end == len(request.prompt_tokens)
 
 
-def _run_group(engine, prefill, decode, device):
-    """One packed forward pass over ``prefill`` chunks and ``decode`` tokens."""
+def _run_group(engine, prefill, decode, device, num_pages=None):
+    """One packed forward pass over ``prefill`` chunks and ``decode`` tokens (with ``num_pages``,
+    which ``packed_forward`` takes: decode tokens alone)."""
     requests, tokens, lengths, sampled = [], [], [], []
     for request in prefill:
         chunk, completes = _prompt_chunk(engine, request)
@@ -103,7 +104,7 @@ def _run_group(engine, prefill, decode, device):
     rows = [i for i, s in enumerate(sampled) if s]
     token_ids = torch.tensor(tokens, dtype=torch.long, device=device)
     with torch.inference_mode():
-        logits = packed_forward(engine.model, token_ids, batch, ends[rows].to(device))
+        logits = packed_forward(engine.model, token_ids, batch, ends[rows].to(device), num_pages)
     engine.paged_cache.commit_batch(handles, lengths)
     if not rows:
         return
@@ -127,8 +128,10 @@ class DecodeGraphs:
     the tokens and the page metadata into the graph's buffers and replays it. Requests
     beyond the real batch are padding rows on the manager's scratch page, their scores
     discarded. Sampling, ``finalize`` and the page bookkeeping are ``decode_batch``'s
-    (``engine.py:285-296``). With ``num_pages`` the graphs attend that many pages per request
-    and KV head (the manager's ``track_page_bounds`` is turned on).
+    (``engine.py:285-296``). With ``num_pages`` decoding requests attend that many pages per
+    request and KV head (the manager's ``track_page_bounds`` is turned on), in every tick of
+    ``mixed_generate``: beside prompt chunks, which attend their whole context, they are a pass
+    of their own.
     """
 
     def __init__(self, engine, sizes=(8, 16, 32, 48, 64, 96, 128),
@@ -201,7 +204,8 @@ def mixed_generate(engine, graphs: DecodeGraphs | None = None) -> bool:
     """Run one scheduler tick of ``engine`` (a hayate ``Engine`` whose ``paged_cache`` is a
     ``hayate_b200.PagedKVCacheManager``) with packed forward passes; return whether any
     request remains active (``Engine.generate``'s contract). With ``graphs``, ticks in which
-    every request decodes replay a CUDA graph."""
+    every request decodes replay a CUDA graph; with graphs over chosen pages, so do the
+    decoding requests of every tick, and a tick that no graph serves attends chosen pages too."""
     previous = list(engine.scheduler.current_batch)
     batch = engine.scheduler.tick()
     active = {id(request) for request in batch}
@@ -212,9 +216,16 @@ def mixed_generate(engine, graphs: DecodeGraphs | None = None) -> bool:
         return False
     prefill = [r for r in batch if r.is_prefill]
     decode = [r for r in batch if not r.is_prefill]
-    if graphs is not None and not prefill and graphs.step(decode):
-        return True
     device = engine.paged_cache.device
+    num_pages = graphs.num_pages if graphs is not None else None
+    if graphs is not None and decode and (num_pages is not None or not prefill):
+        if graphs.step(decode):
+            decode = []
+        elif num_pages is not None:  # no graph is large enough: the same pages, run eagerly
+            _run_group(engine, [], decode, device, num_pages)
+            decode = []
+        if not prefill and not decode:
+            return True
     groups = [prefill[i:i + MAX_PREFILL_BATCH] for i in range(0, len(prefill), MAX_PREFILL_BATCH)] or [[]]
     for index, group in enumerate(groups):
         _run_group(engine, group, decode if index == 0 else [], device)
