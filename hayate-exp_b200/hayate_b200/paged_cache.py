@@ -998,10 +998,12 @@ class PagedKVCacheManager:
             handle.bounded = handle.length // self.page_size
 
     def _bound_missed(self, handles, lengths) -> None:
-        """Bounds of the full pages in front of a step that no step before it kept."""
+        """Bounds of the full pages in front of a step that no step before it kept, each once
+        however many requests share it."""
         size = self.page_size
-        self._bound_pages([page for handle, length in zip(handles, lengths) if handle.bounded < length // size
-                           for page in handle.pages[handle.bounded: length // size]])
+        self._bound_pages(sorted({page for handle, length in zip(handles, lengths)
+                                  if handle.bounded < length // size
+                                  for page in handle.pages[handle.bounded: length // size]}))
         for handle, length in zip(handles, lengths):
             handle.bounded = length // size
 
