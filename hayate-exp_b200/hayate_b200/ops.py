@@ -17,6 +17,7 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.HYT_DTYPE_BF16, torch.float16: _lib.HYT_DTYPE_F16,
            torch.float32: _lib.HYT_DTYPE_F32}
+KERNEL_DTYPES = tuple(_DTYPES)
 
 KERNELS = ("auto", "decode", "prefill", "generic")
 

@@ -664,10 +664,11 @@ class PagedKVCacheManager:
         return handles
 
     def _copy_pages(self, pairs: Sequence[tuple[int, int]]) -> None:
-        """Copy pages ``(from, to)`` in every layer of both pools: one launch on the GPU."""
+        """Copy pages ``(from, to)`` in every layer of both pools: one launch on the GPU (pools of
+        other types than the kernels take, which the bookkeeping serves too, page by page)."""
         if not pairs:
             return
-        if self.device.type == "cuda":
+        if self.device.type == "cuda" and self.k_cache.dtype in ops.KERNEL_DTYPES:
             ids = self._uploader.upload(np.asarray(pairs, dtype=np.int32).T.reshape(-1))
             n = len(pairs)
             ops.copy_pages(self.k_cache, self.v_cache, ids[:n], ids[n:], self.page_size,
