@@ -986,8 +986,12 @@ class PagedKVCacheManager:
             return
         if self.device.type != "cuda":
             raise RuntimeError("hayate_b200 kernels run on CUDA tensors only (no CPU fallback)")
-        self.k_bounds = torch.zeros((self.num_layers, self.num_kv_heads, self.num_pages, 2, self.head_dim),
-                                    dtype=self.k_cache.dtype, device=self.device)
+        bounds = torch.zeros((self.num_layers, self.num_kv_heads, self.num_pages, 2, self.head_dim),
+                             dtype=self.k_cache.dtype, device=self.device)
+        # pools that the kernel does not take are refused here, not by the step that fills a page
+        ops.page_bounds(self.k_cache, bounds, torch.empty(0, dtype=torch.int32, device=self.device),
+                        self.page_size)
+        self.k_bounds = bounds
         self._bound_pages(np.nonzero(self._page_refs)[0])
 
     def refresh_page_bounds(self, handle: PagedCacheHandle) -> None:

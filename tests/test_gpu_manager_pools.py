@@ -31,3 +31,21 @@ def test_copy_on_write_of_any_pool_type(dtype):
     forks = m.fork(a, 2)
     m.import_cache(forks[0], before)
     assert torch.equal(m.snapshot(forks[1]).k, before.k) and torch.equal(m.snapshot(forks[0]).v, before.v)
+
+
+@pytest.mark.parametrize("dim, dtype, error", [(100, torch.bfloat16, RuntimeError), (264, torch.float32, RuntimeError),
+                                               (128, torch.float64, TypeError)], ids=str)
+def test_bounds_of_pools_that_the_kernel_does_not_take_are_refused_at_once(dim, dtype, error):
+    """Not by the step that fills the first page: an untracked manager keeps working."""
+    m = PagedKVCacheManager(1, 2, dim, 8 * 128, 128, 4, dtype, "cuda")
+    with pytest.raises(error):
+        m.track_page_bounds()
+    assert m.k_bounds is None
+    if dtype is not torch.float64:
+        h = m.allocate()
+        batch = m.begin_batch([h], 130)
+        k = torch.ones(1, 2, 130, dim, dtype=dtype, device="cuda")
+        batch.write_layer(0, k, k)
+        m.commit_batch([h], 130)
+        assert bool((m.snapshot(h).k == 1).all())
+        m.check_device_errors()
