@@ -380,6 +380,17 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// The same; whether `mine` held for every thread.
+__device__ __forceinline__ bool named_bar_all(int id, int threads, bool mine) {
+  int all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"(mine ? 1 : 0)
+      : "memory");
+  return all != 0;
+}
+
 // ---------------------------------------------------------------- numerics
 // Hardware base-2 exponential (MUFU.EX2); ex2(-inf) = +0.
 __device__ __forceinline__ float ex2(float x) {

@@ -309,7 +309,8 @@ __global__ void __maxnreg__(96)
   const uint32_t tmem = sh->tmem_base;
   const uint32_t smem_base = smem_u32(smem);
   // segment i of the CTA, once the producer has published it; null past the last (or once a
-  // wait gave up)
+  // wait gave up: then not for all threads alike, so those that meet at barriers or in warp
+  // operations vote before they go on)
   auto segment = [&](int i) -> const ChunkSegment* {
     if (!mbar_wait(&sh->seg_full[i % kSegments], (i / kSegments) & 1, err, abort)) return nullptr;
     const ChunkSegment* seg = &sh->seg[i % kSegments];
@@ -324,13 +325,14 @@ __global__ void __maxnreg__(96)
       // an earlier CTA's wait gave up: load nothing, every tile counts as refused
       const bool dead = err != nullptr && (*reinterpret_cast<volatile int32_t*>(err) & HYT_DEVERR_WAIT_TIMEOUT);
       const int page_mask = (1 << p.page_shift) - 1;
-      int n = 0;  // tiles so far
+      int n = 0, k_loads = 0, v_loads = 0;  // tiles so far, those whose K and V stages were filled
+      bool gave_up = false;  // a wait of the CTA ran out: nothing more is published or loaded
       auto pool_row = [&](const int32_t* table, int tile) {
         const int tok = tile * kKeys;
         const int32_t page = table[tok >> p.page_shift];
         return page < 0 || page >= p.num_pages ? -1 : (page << p.page_shift) + (tok & page_mask);
       };
-      for (int i = 0;; ++i) {
+      for (int i = 0; !gave_up; ++i) {
         ChunkSegment seg;
         seg.k_lo = seg.k_hi = 0;
         const bool any = walk.next(P, seg);
@@ -349,8 +351,10 @@ __global__ void __maxnreg__(96)
             if (row < 0) flag_error(err, HYT_DEVERR_PAGE_RANGE);
           }
           const int ks = n % kKStages, vs = n % kVStages;
-          if (n >= kKStages) mbar_wait(&sh->k_empty[ks], (n / kKStages - 1) & 1, err, abort);
-          if (*abort) row = -1;
+          if (n >= kKStages && (!mbar_wait(&sh->k_empty[ks], (n / kKStages - 1) & 1, err, abort) || *abort)) {
+            gave_up = true;
+            break;
+          }
           sh->refused[n & 7] = row < 0;
           if (row >= 0) {
             uint8_t* dst = smem + L::kK + ks * kTileBytes;
@@ -360,8 +364,12 @@ __global__ void __maxnreg__(96)
           } else {
             mbar_arrive(&sh->k_full[ks]);
           }
-          if (n >= kVStages) mbar_wait(&sh->v_empty[vs], (n / kVStages - 1) & 1, err, abort);
-          if (row >= 0 && !*abort) {
+          ++k_loads;
+          if (n >= kVStages && (!mbar_wait(&sh->v_empty[vs], (n / kVStages - 1) & 1, err, abort) || *abort)) {
+            gave_up = true;
+            break;
+          }
+          if (row >= 0) {
             uint8_t* dst = smem + L::kV + vs * kTileBytes;
             mbar_arrive_expect_tx(&sh->v_full[vs], kLoadBytes);
 #pragma unroll
@@ -369,12 +377,13 @@ __global__ void __maxnreg__(96)
           } else {
             mbar_arrive(&sh->v_full[vs]);
           }
+          ++v_loads;
           if (n == 0) chunk_write_join(P, start, blockIdx.x, &seg);  // beside the first loads
         }
       }
       // nothing in flight when the CTA exits
-      for (int i = max(0, n - kKStages); i < n; ++i) mbar_drain(&sh->k_full[i % kKStages], (i / kKStages) & 1);
-      for (int i = max(0, n - kVStages); i < n; ++i) mbar_drain(&sh->v_full[i % kVStages], (i / kVStages) & 1);
+      for (int i = max(0, k_loads - kKStages); i < k_loads; ++i) mbar_drain(&sh->k_full[i % kKStages], (i / kKStages) & 1);
+      for (int i = max(0, v_loads - kVStages); i < v_loads; ++i) mbar_drain(&sh->v_full[i % kVStages], (i / kVStages) & 1);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
@@ -445,7 +454,7 @@ __global__ void __maxnreg__(96)
     };
     for (int i = 0;; ++i) {
       const ChunkSegment* found = segment(i);
-      if (found == nullptr) break;
+      if (!__all_sync(0xffffffffu, found != nullptr)) break;
       const ChunkSegment& seg = *found;
       const int n = seg.k_hi - seg.k_lo;
       uint32_t begun = 0u;  // streams whose O holds something of this segment
@@ -607,21 +616,22 @@ __global__ void __maxnreg__(96)
       load_q(*now);
       q_ready();
     }
-    int i = 0;
-    for (int n0 = 0; now != nullptr; ++i) {
+    int loads = now != nullptr ? 1 : 0;
+    for (int i = 0, n0 = 0; now != nullptr; ++i) {
       const ChunkSegment seg = *now;
       const int n = seg.k_hi - seg.k_lo;
       const int first = first_checked(seg);
       for (int tile = first; tile < seg.k_hi; ++tile) check_v(seg, i, tile, n0 + tile - seg.k_lo);
-      mbar_wait(&sh->q_empty, i & 1, err, abort);
+      if (!mbar_wait(&sh->q_empty, i & 1, err, abort)) break;  // Q may still be read
       now = segment(i + 1);
       if (now != nullptr) {
         load_q(*now);
         q_ready();
+        ++loads;
       }
       n0 += n;
     }
-    if (kp.q_tma && tid == 0 && i > 0) mbar_drain(&sh->q_full, (i - 1) & 1);  // nothing in flight when the CTA exits
+    if (kp.q_tma && tid == 0 && loads > 0) mbar_drain(&sh->q_full, (loads - 1) & 1);  // nothing in flight when the CTA exits
   } else {
     // ------------------------------------------------------------ softmax warps
     const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
@@ -640,7 +650,11 @@ __global__ void __maxnreg__(96)
 
     for (;;) {
       const ChunkSegment* found = segment(segs);
-      if (found == nullptr) break;
+      // All softmax warps go on, or none: they meet at barriers below. O, the sums and `fix` of the
+      // segment before have been read by everyone (the entry's next user is one segment on,
+      // after another of these barriers)
+      if (!named_bar_all(kSoftmaxBar, kSoftmaxThreads, found != nullptr)) break;
+      if (threadIdx.x == 0 && segs > 0) sh->fix[(segs - 1) & 1] = 0;
       const ChunkSegment& seg = *found;
       const int n = seg.k_hi - seg.k_lo;
       const int rows_left = seg.queries * P.group - seg.row0;  // may exceed the unit's rows
@@ -840,10 +854,6 @@ __global__ void __maxnreg__(96)
         }
       }
       tc_fence_before();
-      // O, the sums and this segment's `fix` have been read by everyone (the entry's next user
-      // is two segments on, after another of these barriers)
-      named_bar_sync(kSoftmaxBar, kSoftmaxThreads);
-      if (threadIdx.x == 0) sh->fix[segs & 1] = 0;
       n0 = end;
       ++segs;
     }
