@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
     fence_proxy_async_smem();
   }
   BoundsCursor ahead(p, item0), at = ahead;
+  int64_t loaded = 0;  // blocks, of thread 0
   auto load = [&](int st) {  // thread 0: the next block into stage st
     int32_t page = p.pages[ahead.entry];
     if (page < -1 || page >= p.num_pages) {
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
       mbar_arrive(&full[st]);
     }
     ahead.next(p, parts);
+    ++loaded;
   };
   if (tid == 0)
     for (int i = 0; i < kBoundsStages && i < blocks; ++i) load(i);
@@ -244,7 +246,10 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
     // the stage has been read and the head's results are there; those of the head before last,
     // whose place the next head's take, went out before this barrier
     __syncthreads();
-    if (tid == 0 && i + kBoundsStages < blocks) load(st);
+    if (tid == 0 && i + kBoundsStages < blocks) {
+      if (*const_cast<volatile int*>(&abort_s) == 0) load(st);
+      else page_s[st] = -1;  // a wait gave up: its stage may still be written, the rest is skipped
+    }
     if (++st == kBoundsStages) st = 0, phase ^= 1u;
     if (!ends) continue;
     which ^= 1;
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
   }
   // every block was waited for above; if a wait gave up, see that no copy is in flight at the exit
   if (tid == 0 && abort_s)
-    for (int64_t i = blocks > kBoundsStages ? blocks - kBoundsStages : 0; i < blocks; ++i)
+    for (int64_t i = loaded > kBoundsStages ? loaded - kBoundsStages : 0; i < loaded; ++i)
       mbar_drain(&full[i % kBoundsStages], uint32_t(i / kBoundsStages) & 1u);
 }
 
