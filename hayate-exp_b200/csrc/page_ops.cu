@@ -77,6 +77,8 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const MoveParams p
 template <int kVec>
 __global__ void __launch_bounds__(kThreads) compact_rows_kernel(const MoveParams p) {
   using V = typename Vec<kVec>::type;
+  // 36 layers, us with 4 / 12 / 16 rows ahead: 64 paths of 2 to 4 rows 9 / 13 / 18, of 6 to 12 31 / 32 / 37,
+  // 16 of 32 29 / 30 / 29; 300 rows of 4 requests 89 / 67 / 63, 1,000 of one 229 / 145 / 136
   constexpr int kRowsAhead = 12;
   __shared__ int64_t from_s[kThreads], to_s[kThreads];  // byte offsets in a plane, -1: nothing to do
   const int b = blockIdx.y;

@@ -38,10 +38,10 @@
 // sum, and O are fp32. The running maximum may lag by up to 2^8 (O / l is exact all the same).
 //
 // Bound by HBM up to 128 rows a unit: 64 requests x 16 nodes over 1K to 8K tokens, 32 / 8 heads of
-// 128, take 207 us for 1.23 GB with the merge (5.9 TB/s). Above, by the chain of a stream's
+// 128, take 205 us for 1.23 GB with the merge (6.0 TB/s). Above, by the chain of a stream's
 // softmax and its 16 MMAs, 3,250 to 3,400 cycles per 256 x 128 tile of which the MMAs are 2,048:
-// 4 x 33..64 nodes over 32K tokens 142 us (0.70 PFLOP/s of visible pairs), 8 x 256 nodes over 2K to
-// 4K 125 us (0.79). Two row blocks per unit instead of one: a K/V tile is read half as often (the
+// 4 x 33..64 nodes over 32K tokens 143 us (0.70 PFLOP/s of visible pairs), 8 x 256 nodes over 2K to
+// 4K 128 us (0.77). Two row blocks per unit instead of one: a K/V tile is read half as often (the
 // first kernel, with one, took 199 us on the latter). A unit's ends cost about 4 tiles: the first
 // tile runs on cold instructions, and O goes out as 128 KB of partials.
 #include <type_traits>
@@ -68,8 +68,8 @@ constexpr uint32_t kOCol = 256;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kUnseen = 2.0f;  // rescale factor, else at most 1, of a row that saw nothing yet (O and sum are 0)
 
-// measured on 64 requests x 16 nodes, 8 x 256 nodes and 64 requests over 16 chosen pages: 3 tiles take 205, 127
-// and 133 us, 4 take 206, 127 and 132, 6 take 208, 128 and 131; one user (8 units of 8 tiles) 13.7, 13.6 and 14.2
+// measured on 64 requests x 16 nodes, 8 x 256 nodes and 64 requests over 16 chosen pages: 3 tiles take 207, 127
+// and 123 us, 4 take 205, 129 and 123, 6 take 206, 130 and 123; one user (8 units of 8 tiles) 13.5, 13.5 and 13.8
 constexpr int kUnitCost = 4;
 
 struct Shared {

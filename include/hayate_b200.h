@@ -368,7 +368,8 @@ int hyt_read_probe(const void* src, size_t bytes, uint32_t* sink, int32_t ctas, 
  * q_start[b] + q_len[b] - 1 of the token axis (q_len may be 0), their K/V already in slots
  * cache_lens[b] + i. Node i sees every cached token and node j of its request if bit j % 32 of
  * word j / 32 of its row of tree_mask [total_tokens, mask_words] is set (its own bit
- * included); a node that sees nothing gets zeros. tree_mask NULL: the chunk is causal. q/out
+ * included); a node that sees nothing gets zeros, one that sees a score of NaN or +inf gets NaN, and
+ * values it does not see never matter. tree_mask NULL: the chunk is causal. q/out
  * strides = {t, h}. page_table_width: entries of a table row (page_table_stride is the
  * distance between rows). head_dim a multiple of 8 up to 256, page_size >= 64, scale > 0.
  * The workspace (hyt_tree_workspace_bytes, 16-byte aligned) needs no initial contents and
